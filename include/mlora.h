@@ -397,6 +397,72 @@ int mlora_gather_rows(const void* src, const int32_t* perm, int64_t rows, int32_
 int mlora_scatter_rows(const void* src, const int32_t* perm, int64_t rows, int32_t cols,
                        int32_t dtype, void* dst, void* stream);
 
+/* ---- 8-bit integers: a backbone held in 8 bits, and inputs saved in 8 bits
+ * for the backward.  No counterpart in the reference (whose backbone and saved
+ * tensors keep the compute type).
+ *
+ * An 8-bit matrix holds int8 rows q with one float scale s per row and stands
+ * for s[i] q[i, k].  Rows are mlora_q8_ld(cols) bytes apart (cols rounded up
+ * to 16), start on 16-byte boundaries, and the bytes past cols are zero.
+ * mlora_q8_quantize makes it from a matrix x whose rows are ld_src elements
+ * apart:
+ *     s[i] = fl32(max_k |x[i, k]| / 127),  q[i, k] = round_half_even(x[i, k] / s[i])
+ * with the quotient rounded exactly; with col_scale (float [cols] or NULL) x is
+ * fl32(x[i, k] col_scale[k]) instead.  A row of zeros has s = 0; a row with an
+ * infinity or a NaN has s = NaN and q = 0, so that every value computed from
+ * that row, and from no other, is NaN.  mlora_q8_dequantize writes the dense
+ * matrix of s[i] q[i, k], each rounded once to dtype. */
+int64_t mlora_q8_ld(int64_t cols);
+int mlora_q8_quantize(const void* src, int64_t rows, int64_t cols, int64_t ld_src, int32_t dtype,
+                      const float* col_scale, int8_t* q, float* scale, void* stream);
+int mlora_q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64_t cols, int32_t dtype,
+                        void* dst, void* stream);
+
+/* Longest contraction (d_in of the forward, d_out of dX) of an 8-bit product:
+ * the 32-bit integer accumulator cannot overflow up to it. */
+#define MLORA_Q8_MAX_K 131072
+
+/* Matrix product in 8-bit integers, scales per token and per output channel:
+ *     Y[i, j] = x_scale[i] w_scale[j] sum_k Xq[i, k] Wq[j, k] + bias[j]
+ * and the gradient of its input through the 8-bit rows of dY w_scale,
+ *     dX[i, k] = g_scale[i] sum_j Gq[i, j] Wq[j, k].
+ * prob gives rows, d_in, d_out, dtype (of X, bias, Y, dY, dX), max_ctas and
+ * err_word.  X (rows ld_x elements apart) is quantized into Xq / x_scale
+ * first; with X NULL they hold the 8-bit rows already.  dY is quantized into
+ * the scratch Gq [rows, mlora_q8_ld(d_out)] / g_scale [rows].  The integer
+ * sums are exact; one rounding to dtype at the end. */
+int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t ld_x, int8_t* Xq, float* x_scale,
+                    const int8_t* Wq, const float* w_scale, const void* bias, void* Y, void* stream);
+int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale, const int8_t* Wq,
+                       const float* w_scale, void* dX, void* stream);
+
+/* The 8-bit operands of mlora_forward_q8 and mlora_backward_q8 (device
+ * memory of the caller). */
+typedef struct mlora_q8 {
+  const int8_t* Wq;      /* [d_out, ld(d_in)] the backbone in 8 bits (W is NULL then), or NULL: W as it is */
+  const float* w_scale;  /* [d_out] */
+  int8_t* Xq;            /* [rows, ld(d_in)].  Forward: receives the 8-bit rows of X (required with Wq).
+                            Backward: those rows, read for dA instead of X (X may be NULL), or NULL: X as it is */
+  float* x_scale;        /* [rows] */
+  int8_t* Gq;            /* [rows, ld(d_out)] scratch of a backward with Wq that writes dX */
+  float* g_scale;        /* [rows] */
+} mlora_q8;
+
+/* mlora_forward with the backbone product in 8 bits (q8->Wq), and / or with X
+ * also written in 8 bits (q8->Xq) for the backward.  The LoRA term reads X as
+ * it is.  Rows are in adapter order, as in mlora_forward. */
+int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
+                     const void* X, const void* W, const void* bias, const void* A_pack, const void* B_pack,
+                     void* Y, void* zsave, void* workspace, size_t workspace_bytes, void* stream);
+/* mlora_backward with dX through the 8-bit backbone (q8->Wq) and / or dA from
+ * the saved 8-bit rows (q8->Xq):
+ *     dA_a = sum_seg (s_a dY_seg B_a)^T (x_scale Xq)_seg.
+ * X is read for dA only. */
+int mlora_backward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
+                      const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
+                      const void* zsave, void* dX, void* dA_pack, void* dB_pack, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Library-wide device error word on the current device: bit 0 = a bounds
  * check fired, bit 1 = a bounded wait timed out.  Only calls made with a NULL
  * err_word report into it.  mlora_clear_error resets it. */

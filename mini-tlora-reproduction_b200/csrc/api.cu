@@ -4,6 +4,7 @@
 #include <initializer_list>
 
 #include "common.cuh"
+#include "q8.cuh"
 #include "simt.cuh"
 #include "tc.cuh"
 
@@ -108,6 +109,19 @@ int choose_impl(const mlora_problem* prob, std::initializer_list<const void*> pt
   return (tc_ok && tc_available()) ? MLORA_IMPL_TC : MLORA_IMPL_SIMT;
 }
 
+// Checks of the 8-bit operands of a call (alignment: rows of an 8-bit matrix
+// start on 16-byte boundaries, which its leading dimension keeps).
+int check_q8(std::initializer_list<const void*> mats, std::initializer_list<const void*> scales) {
+  for (const void* q : mats)
+    if (!aligned(q, 16)) return MLORA_ERR_UNSUPPORTED;
+  for (const void* s : scales)
+    if (!aligned(s, 4)) return MLORA_ERR_UNSUPPORTED;
+  return MLORA_OK;
+}
+
+// One 8-bit product.
+int q8_main(const Q8Main& a, cudaStream_t st) { return q8_main_simt(a, st); }
+
 }  // namespace
 }  // namespace mlora
 
@@ -149,12 +163,30 @@ extern "C" int32_t mlora_num_tiles(int64_t rows) {
 
 namespace {
 
+// The 8-bit backbone product of mlora_forward_q8, with the LoRA expand of the
+// intermediate that the shrink before it left in zsave.
+int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8, const PlanDev& dev,
+                    const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
+                    cudaStream_t s) {
+  Q8Main m;
+  m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
+  m.Aq = q8->Xq; m.a_scale = q8->x_scale;
+  m.Wq = q8->Wq; m.w_scale = q8->w_scale;
+  m.bias = bias; m.out = Y; m.out_rows = route->out_rows;
+  m.expand = dev.n_chunks > 0 && !(stages & MLORA_STAGE_NO_EXPAND);
+  m.plan = dev; m.zt = zsave; m.pack = B_pack;
+  m.max_ctas = prob->max_ctas;
+  m.err = prob->err_word;
+  return q8_main(m, s);
+}
+
 // mlora_forward_staged, or with `ar` mlora_forward_push (MAIN pushes the
-// partial tiles to their owner ranks instead of writing Y).
+// partial tiles to their owner ranks instead of writing Y), or with `q8`
+// mlora_forward_q8 over all tiles.
 int forward_staged(const mlora_problem* prob, const mlora_routing* route, const void* X, const void* W,
                    const void* bias, const void* A_pack, const void* B_pack, void* Y, void* zsave,
                    void* workspace, size_t workspace_bytes, int32_t stages, int32_t tile_begin,
-                   int32_t tile_end, const mlora_peer_ar* ar, void* stream) {
+                   int32_t tile_end, const mlora_peer_ar* ar, const mlora_q8* q8, void* stream) {
   thread_local Plan p;
   int st = build_plan(prob, route, &p);
   if (st != MLORA_OK) return st;
@@ -178,6 +210,14 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   PlanDev dev;
   st = stage_plan(prob, p, workspace, s, &dev);
   if (st != MLORA_OK) return st;
+  if (q8 && q8->Xq) {  // operand of the 8-bit product, the saved form of X, or both
+    st = q8_quantize(X, prob->rows, prob->d_in, prob->d_in, prob->dtype, nullptr, (int8_t*)q8->Xq,
+                     q8->x_scale, s);
+    if (st != MLORA_OK) return st;
+  }
+  const bool q8_base = q8 && q8->Wq;
+  const int32_t all_stages = stages;
+  if (q8_base) stages &= ~MLORA_STAGE_MAIN;  // the kernels below run the shrink only
   if (impl == MLORA_IMPL_TC) {
     TcCall a;
     a.ar = ar;
@@ -194,7 +234,9 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     a.pair_fwd = prob->impl == MLORA_IMPL_TC_2SM || prob->impl == MLORA_IMPL_TC_WIDE ||
                  (prob->impl != MLORA_IMPL_TC_1SM && prob->d_in >= 2048);
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
-    return tc_forward(a, s);
+    st = tc_forward(a, s);
+    if (st != MLORA_OK || !q8_base) return st;
+    return q8_forward_main(prob, route, q8, dev, bias, B_pack, Y, zsave, all_stages, s);
   }
   SimtCall a;
   a.plan = dev;
@@ -207,7 +249,9 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   a.stages = stages; a.t0 = tile_begin; a.t1 = tile_end;
   a.c_begin = p.tile_chunk_begin[tile_begin];
   a.c_end = p.tile_chunk_begin[tile_end];
-  return simt_forward(a, s);
+  st = simt_forward(a, s);
+  if (st != MLORA_OK || !q8_base) return st;
+  return q8_forward_main(prob, route, q8, dev, bias, B_pack, Y, zsave, all_stages, s);
 }
 
 }  // namespace
@@ -218,7 +262,7 @@ extern "C" int mlora_forward_staged(const mlora_problem* prob, const mlora_routi
                                     void* workspace, size_t workspace_bytes, int32_t stages,
                                     int32_t tile_begin, int32_t tile_end, void* stream) {
   return forward_staged(prob, route, X, W, bias, A_pack, B_pack, Y, zsave, workspace, workspace_bytes, stages,
-                        tile_begin, tile_end, nullptr, stream);
+                        tile_begin, tile_end, nullptr, nullptr, stream);
 }
 
 extern "C" int mlora_forward_push(const mlora_problem* prob, const mlora_routing* route,
@@ -235,7 +279,7 @@ extern "C" int mlora_forward_push(const mlora_problem* prob, const mlora_routing
     if (!ar->recv[r] || !ar->arrive[r]) return MLORA_ERR_INVALID_ARG;
   if (prob->dtype != MLORA_BF16 && prob->dtype != MLORA_F16) return MLORA_ERR_UNSUPPORTED;
   return forward_staged(prob, route, X, W, bias, A_pack, B_pack, nullptr, zsave, workspace, workspace_bytes,
-                        stages, tile_begin, tile_end, ar, stream);
+                        stages, tile_begin, tile_end, ar, nullptr, stream);
 }
 
 extern "C" int mlora_forward(const mlora_problem* prob, const mlora_routing* route, const void* X,
@@ -248,41 +292,15 @@ extern "C" int mlora_forward(const mlora_problem* prob, const mlora_routing* rou
                               mlora_num_tiles(prob->rows), stream);
 }
 
-extern "C" int mlora_backward_staged(const mlora_problem* prob, const mlora_routing* route,
-                                     const void* dY, const void* X, const void* W, const void* A_pack,
-                                     const void* B_pack, const void* zsave, void* dzsave, void* dX,
-                                     void* dA_pack, void* dB_pack, void* workspace, size_t workspace_bytes,
-                                     int32_t stages, int32_t tile_begin, int32_t tile_end, int32_t db_begin,
-                                     int32_t db_end, void* stream) {
-  thread_local Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
-  if (stages & ~(MLORA_BWD_DZ | MLORA_BWD_DX | MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B))
-    return MLORA_ERR_INVALID_ARG;
-  // the fused SGD step updates the weights whose gradients the call writes
-  if ((stages & MLORA_BWD_SGD_A) && (!(stages & MLORA_BWD_DA) || !dA_pack || !A_pack)) return MLORA_ERR_INVALID_ARG;
-  if ((stages & MLORA_BWD_SGD_B) && (!(stages & MLORA_BWD_DB) || !dB_pack || !B_pack)) return MLORA_ERR_INVALID_ARG;
-  const int nb_out = (prob->d_out + 127) / 128;
-  if (tile_begin < 0 || tile_end < tile_begin || tile_end > p.n_tiles) return MLORA_ERR_INVALID_ARG;
-  if (db_begin < 0 || db_end < db_begin || db_end > nb_out) return MLORA_ERR_INVALID_ARG;
-  if (prob->rows == 0) return MLORA_OK;
-  if (!dY || !workspace) return MLORA_ERR_INVALID_ARG;
-  const bool lora = !p.chunks.empty();
-  const bool need_dz = lora && ((stages & MLORA_BWD_DZ) || (dX && (stages & MLORA_BWD_DX)) ||
-                                (dA_pack && (stages & MLORA_BWD_DA)));
-  if (need_dz && (!dzsave || !B_pack)) return MLORA_ERR_INVALID_ARG;
-  if (lora && dX && (stages & MLORA_BWD_DX) && !A_pack) return MLORA_ERR_INVALID_ARG;
-  if (lora && dB_pack && (stages & MLORA_BWD_DB) && !zsave) return MLORA_ERR_INVALID_ARG;
-  if (((dA_pack && (stages & MLORA_BWD_DA)) || (dB_pack && (stages & MLORA_BWD_DB))) && !X)
-    return MLORA_ERR_INVALID_ARG;
-  if (workspace_bytes < ws_bytes(p, prob->dtype)) return MLORA_ERR_WORKSPACE;
-  if (!aligned(workspace, 16)) return MLORA_ERR_UNSUPPORTED;  // plan tables hold 16-byte entries
-  const int impl = choose_impl(prob, {dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack});
-  if (impl < 0) return MLORA_ERR_UNSUPPORTED;
-  cudaStream_t s = (cudaStream_t)stream;
-  PlanDev dev;
-  st = stage_plan(prob, p, workspace, s, &dev);
-  if (st != MLORA_OK) return st;
+namespace {
+
+// The kernels of a backward call on a staged plan; with `q8`, dA reads the
+// saved 8-bit rows of X.
+int backward_kernels(const mlora_problem* prob, const mlora_routing* route, const Plan& p, const PlanDev& dev,
+                     int impl, const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
+                     const void* zsave, void* dzsave, void* dX, void* dA_pack, void* dB_pack, int32_t stages,
+                     int32_t tile_begin, int32_t tile_end, int32_t db_begin, int32_t db_end, const mlora_q8* q8,
+                     cudaStream_t s) {
   if (impl == MLORA_IMPL_TC) {
     TcCall a;
     a.plan = dev;
@@ -310,15 +328,126 @@ extern "C" int mlora_backward_staged(const mlora_problem* prob, const mlora_rout
   a.out_rows = route->out_rows;
   a.bwd_stages = stages; a.db0 = db_begin; a.db1 = db_end;
   a.lr = prob->lr;
+  if (q8) { a.Xq = q8->Xq; a.x_scale = q8->x_scale; }
   a.c_begin = p.tile_chunk_begin[tile_begin];
   a.c_end = p.tile_chunk_begin[tile_end];
   return simt_backward(a, s);
 }
 
-extern "C" int mlora_backward(const mlora_problem* prob, const mlora_routing* route, const void* dY,
-                              const void* X, const void* W, const void* A_pack, const void* B_pack,
-                              const void* zsave, void* dX, void* dA_pack, void* dB_pack,
-                              void* workspace, size_t workspace_bytes, void* stream) {
+// mlora_backward_q8 on a staged plan: the 8-bit product takes the place of
+// the dX mainloop, the saved 8-bit rows that of X in dA.
+int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Plan& p, const PlanDev& dev, int impl,
+                const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
+                const void* zsave, void* dzsave, void* dX, void* dA_pack, void* dB_pack, int32_t stages,
+                const mlora_q8* q8, cudaStream_t s) {
+  const int nb_out = (prob->d_out + 127) / 128;
+  const bool q8_dx = dX && q8->Wq && (stages & MLORA_BWD_DX);
+  const bool saved8 = q8->Xq != nullptr;
+  const int32_t reduce = MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B;
+  if (!q8_dx && !saved8)
+    return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack,
+                            dB_pack, stages, 0, p.n_tiles, 0, nb_out, nullptr, s);
+  // dZ (and the 16-bit dX), then the 8-bit dX, then the reductions
+  int st = backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave,
+                            q8_dx ? nullptr : dX, dA_pack, dB_pack, stages & ~reduce, 0, p.n_tiles, 0, nb_out,
+                            nullptr, s);
+  if (st != MLORA_OK) return st;
+  if (q8_dx) {
+    st = q8_quantize(dY, prob->rows, prob->d_out, prob->d_out, prob->dtype, q8->w_scale, q8->Gq, q8->g_scale, s);
+    if (st != MLORA_OK) return st;
+    Q8Main m;
+    m.bwd = true;
+    m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
+    m.Aq = q8->Gq; m.a_scale = q8->g_scale;
+    m.Wq = q8->Wq;
+    m.out = dX; m.out_rows = route->out_rows;
+    m.expand = dev.n_chunks > 0;
+    m.plan = dev; m.zt = dzsave; m.pack = A_pack;
+    m.max_ctas = prob->max_ctas;
+    m.err = prob->err_word;
+    st = q8_main(m, s);
+    if (st != MLORA_OK) return st;
+  }
+  if (!saved8)
+    return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, nullptr, dA_pack,
+                            dB_pack, stages & reduce, 0, p.n_tiles, 0, nb_out, nullptr, s);
+  // dA from the saved 8-bit rows, dB as ever
+  const int32_t of_a = MLORA_BWD_DA | MLORA_BWD_SGD_A, of_b = MLORA_BWD_DB | MLORA_BWD_SGD_B;
+  if (dA_pack && (stages & MLORA_BWD_DA)) {
+    st = backward_kernels(prob, route, p, dev, MLORA_IMPL_SIMT, dY, nullptr, W, A_pack, B_pack, zsave, dzsave,
+                          nullptr, dA_pack, nullptr, stages & of_a, 0, p.n_tiles, 0, nb_out, q8, s);
+    if (st != MLORA_OK) return st;
+  }
+  if (!dB_pack || !(stages & MLORA_BWD_DB)) return MLORA_OK;
+  return backward_kernels(prob, route, p, dev, impl, dY, nullptr, W, A_pack, B_pack, zsave, dzsave, nullptr, nullptr,
+                          dB_pack, stages & of_b, 0, p.n_tiles, 0, nb_out, nullptr, s);
+}
+
+}  // namespace
+
+namespace {
+
+// mlora_backward_staged, or with `q8` mlora_backward_q8 over all ranges.
+int backward_staged(const mlora_problem* prob, const mlora_routing* route, const void* dY, const void* X,
+                    const void* W, const void* A_pack, const void* B_pack, const void* zsave, void* dzsave, void* dX,
+                    void* dA_pack, void* dB_pack, void* workspace, size_t workspace_bytes, int32_t stages,
+                    int32_t tile_begin, int32_t tile_end, int32_t db_begin, int32_t db_end, const mlora_q8* q8,
+                    void* stream) {
+  thread_local Plan p;
+  int st = build_plan(prob, route, &p);
+  if (st != MLORA_OK) return st;
+  if (stages & ~(MLORA_BWD_DZ | MLORA_BWD_DX | MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B))
+    return MLORA_ERR_INVALID_ARG;
+  // the fused SGD step updates the weights whose gradients the call writes
+  if ((stages & MLORA_BWD_SGD_A) && (!(stages & MLORA_BWD_DA) || !dA_pack || !A_pack)) return MLORA_ERR_INVALID_ARG;
+  if ((stages & MLORA_BWD_SGD_B) && (!(stages & MLORA_BWD_DB) || !dB_pack || !B_pack)) return MLORA_ERR_INVALID_ARG;
+  const int nb_out = (prob->d_out + 127) / 128;
+  if (tile_begin < 0 || tile_end < tile_begin || tile_end > p.n_tiles) return MLORA_ERR_INVALID_ARG;
+  if (db_begin < 0 || db_end < db_begin || db_end > nb_out) return MLORA_ERR_INVALID_ARG;
+  if (prob->rows == 0) return MLORA_OK;
+  if (!dY || !workspace) return MLORA_ERR_INVALID_ARG;
+  const bool lora = !p.chunks.empty();
+  const bool need_dz = lora && ((stages & MLORA_BWD_DZ) || (dX && (stages & MLORA_BWD_DX)) ||
+                                (dA_pack && (stages & MLORA_BWD_DA)));
+  if (need_dz && (!dzsave || !B_pack)) return MLORA_ERR_INVALID_ARG;
+  if (lora && dX && (stages & MLORA_BWD_DX) && !A_pack) return MLORA_ERR_INVALID_ARG;
+  if (lora && dB_pack && (stages & MLORA_BWD_DB) && !zsave) return MLORA_ERR_INVALID_ARG;
+  const bool saved8 = q8 && q8->Xq;
+  // (the 8-bit call reads X for dA only, and not where its 8-bit rows are given)
+  if (q8 ? lora && dA_pack && (stages & MLORA_BWD_DA) && !X && !saved8
+         : ((dA_pack && (stages & MLORA_BWD_DA)) || (dB_pack && (stages & MLORA_BWD_DB))) && !X)
+    return MLORA_ERR_INVALID_ARG;
+  if (workspace_bytes < ws_bytes(p, prob->dtype)) return MLORA_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return MLORA_ERR_UNSUPPORTED;  // plan tables hold 16-byte entries
+  const int impl = choose_impl(prob, {dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack});
+  if (impl < 0) return MLORA_ERR_UNSUPPORTED;
+  cudaStream_t s = (cudaStream_t)stream;
+  PlanDev dev;
+  st = stage_plan(prob, p, workspace, s, &dev);
+  if (st != MLORA_OK) return st;
+  if (q8) return q8_backward(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack,
+                             dB_pack, stages, q8, s);
+  return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack,
+                          stages, tile_begin, tile_end, db_begin, db_end, nullptr, s);
+}
+
+}  // namespace
+
+extern "C" int mlora_backward_staged(const mlora_problem* prob, const mlora_routing* route,
+                                     const void* dY, const void* X, const void* W, const void* A_pack,
+                                     const void* B_pack, const void* zsave, void* dzsave, void* dX,
+                                     void* dA_pack, void* dB_pack, void* workspace, size_t workspace_bytes,
+                                     int32_t stages, int32_t tile_begin, int32_t tile_end, int32_t db_begin,
+                                     int32_t db_end, void* stream) {
+  return backward_staged(prob, route, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack, workspace,
+                         workspace_bytes, stages, tile_begin, tile_end, db_begin, db_end, nullptr, stream);
+}
+
+namespace {
+
+int backward_all(const mlora_problem* prob, const mlora_routing* route, const void* dY, const void* X, const void* W,
+                 const void* A_pack, const void* B_pack, const void* zsave, void* dX, void* dA_pack, void* dB_pack,
+                 void* workspace, size_t workspace_bytes, const mlora_q8* q8, void* stream) {
   if (!prob || !route) return MLORA_ERR_INVALID_ARG;
   size_t plan_bytes = 0;
   {
@@ -332,9 +461,132 @@ extern "C" int mlora_backward(const mlora_problem* prob, const mlora_routing* ro
   int32_t stages = ((dX || dA_pack) ? MLORA_BWD_DZ : 0) | MLORA_BWD_DX | MLORA_BWD_DA | MLORA_BWD_DB;
   if (prob->flags & MLORA_FUSED_SGD)
     stages |= (dA_pack ? MLORA_BWD_SGD_A : 0) | (dB_pack ? MLORA_BWD_SGD_B : 0);
-  return mlora_backward_staged(prob, route, dY, X, W, A_pack, B_pack, zsave, dzt, dX, dA_pack, dB_pack,
-                               workspace, workspace_bytes, stages, 0, mlora_num_tiles(prob->rows), 0,
-                               (prob->d_out + 127) / 128, stream);
+  return backward_staged(prob, route, dY, X, W, A_pack, B_pack, zsave, dzt, dX, dA_pack, dB_pack, workspace,
+                         workspace_bytes, stages, 0, mlora_num_tiles(prob->rows), 0, (prob->d_out + 127) / 128, q8,
+                         stream);
+}
+
+}  // namespace
+
+extern "C" int mlora_backward(const mlora_problem* prob, const mlora_routing* route, const void* dY,
+                              const void* X, const void* W, const void* A_pack, const void* B_pack,
+                              const void* zsave, void* dX, void* dA_pack, void* dB_pack,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return backward_all(prob, route, dY, X, W, A_pack, B_pack, zsave, dX, dA_pack, dB_pack, workspace,
+                      workspace_bytes, nullptr, stream);
+}
+
+// ---------------------------------------------------------------- 8-bit entry points
+
+extern "C" int64_t mlora_q8_ld(int64_t cols) { return cols <= 0 ? 0 : q8_ld(cols); }
+
+namespace {
+
+int check_rows_cols(int64_t rows, int64_t cols, int32_t dtype) {
+  if (rows < 0 || rows > (int64_t(1) << 31) - kTileRows || cols < 1 || cols > INT32_MAX - 64)
+    return MLORA_ERR_INVALID_ARG;
+  if (dtype != MLORA_F32 && dtype != MLORA_BF16 && dtype != MLORA_F16) return MLORA_ERR_UNSUPPORTED;
+  return MLORA_OK;
+}
+
+// shape of an 8-bit product
+int check_q8_problem(const mlora_problem* prob) {
+  if (!prob) return MLORA_ERR_INVALID_ARG;
+  int st = check_rows_cols(prob->rows, prob->d_in, prob->dtype);
+  if (st == MLORA_OK) st = check_rows_cols(prob->rows, prob->d_out, prob->dtype);
+  if (st != MLORA_OK) return st;
+  if (prob->max_ctas < 0) return MLORA_ERR_INVALID_ARG;
+  return prob->d_in > kQ8MaxK || prob->d_out > kQ8MaxK ? MLORA_ERR_UNSUPPORTED : MLORA_OK;
+}
+
+}  // namespace
+
+extern "C" int mlora_q8_quantize(const void* src, int64_t rows, int64_t cols, int64_t ld_src, int32_t dtype,
+                                 const float* col_scale, int8_t* q, float* scale, void* stream) {
+  int st = check_rows_cols(rows, cols, dtype);
+  if (st != MLORA_OK) return st;
+  if (ld_src < cols) return MLORA_ERR_INVALID_ARG;
+  if (rows == 0) return MLORA_OK;
+  if (!src || !q || !scale) return MLORA_ERR_INVALID_ARG;
+  if (!aligned(src, size_t(elem_bytes(dtype)))) return MLORA_ERR_UNSUPPORTED;
+  if ((st = check_q8({q}, {scale, col_scale})) != MLORA_OK) return st;
+  return q8_quantize(src, rows, cols, ld_src, dtype, col_scale, q, scale, (cudaStream_t)stream);
+}
+
+extern "C" int mlora_q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64_t cols, int32_t dtype,
+                                   void* dst, void* stream) {
+  int st = check_rows_cols(rows, cols, dtype);
+  if (st != MLORA_OK) return st;
+  if (rows == 0) return MLORA_OK;
+  if (!q || !scale || !dst) return MLORA_ERR_INVALID_ARG;
+  if (!aligned(dst, size_t(elem_bytes(dtype)))) return MLORA_ERR_UNSUPPORTED;
+  if ((st = check_q8({q}, {scale})) != MLORA_OK) return st;
+  return q8_dequantize(q, scale, rows, cols, dtype, dst, (cudaStream_t)stream);
+}
+
+extern "C" int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t ld_x, int8_t* Xq, float* x_scale,
+                               const int8_t* Wq, const float* w_scale, const void* bias, void* Y, void* stream) {
+  int st = check_q8_problem(prob);
+  if (st != MLORA_OK) return st;
+  if (X && ld_x < prob->d_in) return MLORA_ERR_INVALID_ARG;
+  if (prob->rows == 0) return MLORA_OK;
+  if (!Xq || !x_scale || !Wq || !w_scale || !Y) return MLORA_ERR_INVALID_ARG;
+  if (!pointers_aligned({X, bias, Y}, size_t(elem_bytes(prob->dtype)))) return MLORA_ERR_UNSUPPORTED;
+  if ((st = check_q8({Xq, Wq}, {x_scale, w_scale})) != MLORA_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (X && (st = q8_quantize(X, prob->rows, prob->d_in, ld_x, prob->dtype, nullptr, Xq, x_scale, s)) != MLORA_OK)
+    return st;
+  Q8Main m;
+  m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
+  m.Aq = Xq; m.a_scale = x_scale; m.Wq = Wq; m.w_scale = w_scale; m.bias = bias; m.out = Y;
+  m.max_ctas = prob->max_ctas; m.err = prob->err_word;
+  return q8_main(m, s);
+}
+
+extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale,
+                                  const int8_t* Wq, const float* w_scale, void* dX, void* stream) {
+  int st = check_q8_problem(prob);
+  if (st != MLORA_OK) return st;
+  if (prob->rows == 0) return MLORA_OK;
+  if (!dY || !Gq || !g_scale || !Wq || !w_scale || !dX) return MLORA_ERR_INVALID_ARG;
+  if (!pointers_aligned({dY, dX}, size_t(elem_bytes(prob->dtype)))) return MLORA_ERR_UNSUPPORTED;
+  if ((st = check_q8({Gq, Wq}, {g_scale, w_scale})) != MLORA_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  st = q8_quantize(dY, prob->rows, prob->d_out, prob->d_out, prob->dtype, w_scale, Gq, g_scale, s);
+  if (st != MLORA_OK) return st;
+  Q8Main m;
+  m.bwd = true;
+  m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
+  m.Aq = Gq; m.a_scale = g_scale; m.Wq = Wq; m.out = dX;
+  m.max_ctas = prob->max_ctas; m.err = prob->err_word;
+  return q8_main(m, s);
+}
+
+extern "C" int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
+                                const void* X, const void* W, const void* bias, const void* A_pack,
+                                const void* B_pack, void* Y, void* zsave, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (!prob || !route || !q8) return MLORA_ERR_INVALID_ARG;
+  if ((q8->Wq && (W || !q8->w_scale || !q8->Xq)) || (q8->Xq && !q8->x_scale)) return MLORA_ERR_INVALID_ARG;
+  if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
+  int st = check_q8({q8->Wq, q8->Xq}, {q8->w_scale, q8->x_scale});
+  if (st != MLORA_OK) return st;
+  return forward_staged(prob, route, X, W, bias, A_pack, B_pack, Y, zsave, workspace, workspace_bytes,
+                        MLORA_STAGE_SHRINK | MLORA_STAGE_MAIN, 0, mlora_num_tiles(prob->rows), nullptr, q8, stream);
+}
+
+extern "C" int mlora_backward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
+                                 const void* dY, const void* X, const void* W, const void* A_pack,
+                                 const void* B_pack, const void* zsave, void* dX, void* dA_pack, void* dB_pack,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  if (!prob || !route || !q8) return MLORA_ERR_INVALID_ARG;
+  if ((q8->Wq && (W || !q8->w_scale || (dX && (!q8->Gq || !q8->g_scale)))) || (q8->Xq && !q8->x_scale))
+    return MLORA_ERR_INVALID_ARG;
+  if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
+  int st = check_q8({q8->Wq, q8->Xq, q8->Gq}, {q8->w_scale, q8->x_scale, q8->g_scale});
+  if (st != MLORA_OK) return st;
+  return backward_all(prob, route, dY, X, W, A_pack, B_pack, zsave, dX, dA_pack, dB_pack, workspace,
+                      workspace_bytes, q8, stream);
 }
 
 extern "C" int mlora_sgd(const mlora_sgd_item* items, int32_t n_items, float lr, int32_t dtype,

@@ -4,6 +4,7 @@
 #include "plan.cu"
 #include "timing.cu"
 #include "simt.cu"
+#include "q8.cu"
 #include "route.cu"
 #include "tc.cu"
 #include "allreduce.cu"

@@ -1,0 +1,48 @@
+// 8-bit integer matrices: rows of int8 with one float scale per row, the
+// quantizer that makes them and the matrix products that read them.
+#pragma once
+
+#include "common.cuh"
+
+namespace mlora {
+
+// Leading dimension (bytes) of an 8-bit matrix of `cols` columns: rows start
+// on 16-byte boundaries, which TMA and 16-byte loads need; the bytes past
+// `cols` are zero.
+inline __host__ __device__ int64_t q8_ld(int64_t cols) { return (cols + 15) / 16 * 16; }
+
+// Longest contraction of one product: |q| <= 127, so 127^2 * 131072 is still
+// below 2^31 and a 32-bit accumulator cannot overflow.
+constexpr int kQ8MaxK = 131072;
+
+int q8_quantize(const void* src, int64_t rows, int64_t cols, int64_t ld_src, int dtype, const float* col_scale,
+                int8_t* q, float* scale, cudaStream_t st);
+int q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64_t cols, int dtype, void* dst,
+                  cudaStream_t st);
+
+// One 8-bit product with its epilogue.
+//   forward   out = s_a[i] s_w[j] sum_k Aq[i, k] Wq[j, k] + bias[j] + sum_c Zt[c] B_pack[j, chunk c]   (N = d_out)
+//   backward  out = s_a[i] sum_k Aq[i, k] Wq[k, j] + sum_c dZt[c] A_pack[chunk c, j]                    (N = d_in)
+struct Q8Main {
+  bool bwd = false;
+  int64_t M = 0;
+  int d_in = 0, d_out = 0, R = 0, dtype = MLORA_F32;
+  const int8_t* Aq = nullptr;      // Xq [M, q8_ld(d_in)] or Gq [M, q8_ld(d_out)]
+  const float* a_scale = nullptr;  // [M]
+  const int8_t* Wq = nullptr;      // [d_out, q8_ld(d_in)]
+  const float* w_scale = nullptr;  // [d_out], forward only (the backward's Gq already holds it)
+  const void* bias = nullptr;      // forward only
+  void* out = nullptr;
+  const int32_t* out_rows = nullptr;
+  // LoRA expand: the routing plan and its low-rank blocks (none without chunks)
+  bool expand = false;
+  PlanDev plan = {};
+  const void* zt = nullptr;
+  const void* pack = nullptr;  // B_pack or A_pack
+  int max_ctas = 0;
+  int* err = nullptr;
+};
+
+int q8_main_simt(const Q8Main& a, cudaStream_t st);
+
+}  // namespace mlora

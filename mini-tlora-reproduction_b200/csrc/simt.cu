@@ -12,6 +12,7 @@
 //   reduce   dA_chunk = sum_tiles dZt[c]^T X_tile, dB_chunk = sum_tiles dY_tile^T Zt[c]
 //   sgd      P <- P - lr dP on the listed adapter tensors
 #include "common.cuh"
+#include "q8.cuh"
 #include "simt.cuh"
 
 namespace mlora {
@@ -172,7 +173,8 @@ __global__ void __launch_bounds__(NT) k_reduce(PlanDev plan, const T* __restrict
                                                 const T* __restrict__ dY, const T* __restrict__ zt,
                                                 const T* __restrict__ dzt, T* __restrict__ dA,
                                                 T* __restrict__ dB, int64_t M, int d_in, int d_out,
-                                                int R, int db0, int db1, T* A_upd, T* B_upd, float lr) {
+                                                int R, int db0, int db1, T* A_upd, T* B_upd, float lr,
+                                                const int8_t* __restrict__ Xq, const float* __restrict__ x_scale) {
   __shared__ float As[BK][LD], Bs[BK][LD];
   const ReduceItem it = plan.reduce[blockIdx.x];
   const int jc = blockIdx.y;
@@ -189,6 +191,12 @@ __global__ void __launch_bounds__(NT) k_reduce(PlanDev plan, const T* __restrict
   auto fa = [&](int i, int tok) -> float {
     const int c = plan.list[it.lb + tok / kTileRows] + j;
     const int64_t row = int64_t(plan.chunks[c].tile) * kTileRows + tok % kTileRows;
+    if (!is_dB && Xq) {
+      // a row of another segment of the tile counts as zero: its scale may be NaN
+      const int rt = tok % kTileRows;
+      if (row >= M || b0 + i >= D || rt < plan.chunks[c].lo || rt >= plan.chunks[c].hi) return 0.f;
+      return float(Xq[row * q8_ld(d_in) + b0 + i]) * x_scale[row];
+    }
     return (row < M && b0 + i < D) ? to_f(mat[row * D + b0 + i]) : 0.f;
   };
   auto fb = [&](int jj, int tok) -> float {
@@ -282,7 +290,7 @@ int launch_backward(const SimtCall& a, cudaStream_t st) {
     T* B_upd = dB && (a.bwd_stages & MLORA_BWD_SGD_B) ? (T*)a.B_pack : nullptr;
     k_reduce<T><<<dim3(a.n_reduce, kMaxChunksPerItem, 2), NT, 0, st>>>(
         a.plan, (const T*)a.X, (const T*)a.dY, (const T*)a.zsave, (const T*)a.dzt, (T*)dA,
-        (T*)dB, a.M, a.d_in, a.d_out, a.R, a.db0, a.db1, A_upd, B_upd, a.lr);
+        (T*)dB, a.M, a.d_in, a.d_out, a.R, a.db0, a.db1, A_upd, B_upd, a.lr, a.Xq, a.x_scale);
     count_launch();
   }
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;

@@ -1941,8 +1941,10 @@ int tc_backward(const TcCall& a, cudaStream_t st) {
   const bool db = a.dB && (a.bwd_stages & MLORA_BWD_DB) && a.db1 > a.db0;
   if (n_chunks > 0 && (da || db)) {
     TcParams prm = base_params(a);
-    if (!make_map(&prm.mA0, a.X, a.M, a.d_in, 64) || !make_map(&prm.mB0, a.dzt, zrows, 64, 64) ||
-        !make_map(&prm.mA1, a.dY, a.M, a.d_out, 64) || !make_map(&prm.mB1, a.zsave, zrows, 64, 64))
+    // the operands of the gradients asked for (X may be absent from a call for dB alone)
+    if (da && (!make_map(&prm.mA0, a.X, a.M, a.d_in, 64) || !make_map(&prm.mB0, a.dzt, zrows, 64, 64)))
+      return MLORA_ERR_UNSUPPORTED;
+    if (db && (!make_map(&prm.mA1, a.dY, a.M, a.d_out, 64) || !make_map(&prm.mB1, a.zsave, zrows, 64, 64)))
       return MLORA_ERR_UNSUPPORTED;
     prm.n_items = a.plan.n_reduce;
     prm.dA = reinterpret_cast<__nv_bfloat16*>(a.dA);

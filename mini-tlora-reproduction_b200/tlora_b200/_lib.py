@@ -134,6 +134,21 @@ class SgdItem(ctypes.Structure):
     ]
 
 
+class Q8(ctypes.Structure):
+    """mlora_q8: the 8-bit operands of mlora_forward_q8 / mlora_backward_q8."""
+    _fields_ = [
+        ("Wq", ctypes.c_void_p),
+        ("w_scale", ctypes.c_void_p),
+        ("Xq", ctypes.c_void_p),
+        ("x_scale", ctypes.c_void_p),
+        ("Gq", ctypes.c_void_p),
+        ("g_scale", ctypes.c_void_p),
+    ]
+
+
+Q8_MAX_K = 131072  # longest contraction of an 8-bit product
+
+
 # every symbol include/mlora.h declares, with its ctypes signature
 _VP = ctypes.c_void_p
 SIGNATURES = {
@@ -170,6 +185,17 @@ SIGNATURES = {
     "mlora_backward_staged": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Routing), _VP, _VP, _VP, _VP,
                                              _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, ctypes.c_int32,
                                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _VP]),
+    "mlora_q8_ld": (ctypes.c_int64, [ctypes.c_int64]),
+    "mlora_q8_quantize": (ctypes.c_int, [_VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _VP,
+                                         _VP, _VP, _VP]),
+    "mlora_q8_dequantize": (ctypes.c_int, [_VP, _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _VP, _VP]),
+    "mlora_q8_linear": (ctypes.c_int, [ctypes.POINTER(Problem), _VP, ctypes.c_int64, _VP, _VP, _VP, _VP, _VP, _VP,
+                                       _VP]),
+    "mlora_q8_linear_dx": (ctypes.c_int, [ctypes.POINTER(Problem), _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "mlora_forward_q8": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Routing), ctypes.POINTER(Q8), _VP,
+                                        _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP]),
+    "mlora_backward_q8": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Routing), ctypes.POINTER(Q8), _VP,
+                                         _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP]),
     "mlora_sgd": (ctypes.c_int, [ctypes.POINTER(SgdItem), ctypes.c_int32, ctypes.c_float, ctypes.c_int32, _VP]),
     "mlora_route_runs": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, ctypes.c_int32, ctypes.c_int32, _VP, _VP]),
     "mlora_route_sort_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),

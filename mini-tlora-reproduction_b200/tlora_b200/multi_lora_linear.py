@@ -60,7 +60,90 @@ class LoRAAdapter(nn.Module):
         return y.reshape(*lead, self.out_features)
 
 
-class IndependentLoRALinear(nn.Module):
+class Int8Base(nn.Module):
+    """A frozen backbone held in 8 bits: ``weight_q8`` int8 [out, ld] and
+    ``weight_scale`` float32 [out] (an ``ops.Int8Rows`` of W's rows, the output
+    channels) and the bias as it was.  The scales stay float32 whatever type
+    the module is cast to."""
+
+    def __init__(self, rows8: ops.Int8Rows, bias: Optional[torch.Tensor]):
+        super().__init__()
+        self.in_features, self.out_features = rows8.cols, rows8.rows
+        self.register_buffer("weight_q8", rows8.q)
+        self.register_buffer("weight_scale", rows8.scale)
+        self.bias = nn.Parameter(bias.detach().clone(), requires_grad=False) if bias is not None else None
+
+    @classmethod
+    def from_linear(cls, base: nn.Linear) -> "Int8Base":
+        return cls(ops.quantize_rows(base.weight.detach()), base.bias)
+
+    @property
+    def rows8(self) -> ops.Int8Rows:
+        return ops.Int8Rows(self.weight_q8, self.weight_scale, self.in_features)
+
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:  # .half() and the like: moved, not cast
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        lead = x.shape[:-1]
+        y = ops.int8_linear(x.reshape(-1, x.shape[-1]), self.rows8, self.bias)
+        return y.reshape(*lead, self.out_features)
+
+    def to_linear(self, dtype: torch.dtype) -> nn.Linear:
+        base = nn.Linear(self.in_features, self.out_features, bias=self.bias is not None, device=self.weight_q8.device,
+                         dtype=dtype)
+        with torch.no_grad():
+            base.weight.copy_(ops.dequantize_rows(self.rows8, dtype))
+            if self.bias is not None:
+                base.bias.copy_(self.bias)
+        for p in base.parameters():
+            p.requires_grad_(False)
+        return base
+
+
+class _Int8BaseMixin:
+    """Switching a module's ``base`` between its own type and 8 bits, and how
+    its input is kept for the backward."""
+
+    save_input = "full"  # or "int8"
+
+    def quantize_base(self):
+        """Hold the frozen backbone in 8 bits (one scale per output channel)
+        from now on: forward and dX run the 8-bit product (``ops.int8_linear``)
+        with the LoRA terms added as before.  The adapters are untouched.
+        ``state_dict`` then has ``base.weight_q8`` and ``base.weight_scale`` in
+        place of ``base.weight``.  Returns the module."""
+        if not isinstance(self.base, Int8Base):
+            self.base = Int8Base.from_linear(self.base)
+        return self
+
+    def dequantize_base(self):
+        """Back to an ``nn.Linear`` of the adapters' type, with the values the
+        8-bit weights stand for.  Returns the module."""
+        if isinstance(self.base, Int8Base):
+            self.base = self.base.to_linear(next(self._adapter_modules()).A.dtype)
+        return self
+
+    def _base_operands(self):
+        """(W or None, 8-bit rows or None, bias)."""
+        b = self.base
+        return (None, b.rows8, b.bias) if isinstance(b, Int8Base) else (b.weight, None, b.bias)
+
+
+_SAVE_INPUT = ("full", "int8")
+
+
+def _save8(value: str) -> bool:
+    if value not in _SAVE_INPUT:
+        raise ValueError(f"save_input must be one of {_SAVE_INPUT}, not {value!r}")
+    return value == "int8"
+
+
+class IndependentLoRALinear(_Int8BaseMixin, nn.Module):
     """One LoRA job on its own frozen backbone (tlora/multi_lora_linear.py:34-56)."""
 
     def __init__(self, in_features: int, out_features: int, rank: int, bias: bool = True,
@@ -72,13 +155,17 @@ class IndependentLoRALinear(nn.Module):
         self.adapter = LoRAAdapter(in_features, out_features, rank, alpha)
         self._packed = None
 
+    def _adapter_modules(self):
+        yield self.adapter
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1])
         ids = torch.zeros(x2.shape[0], dtype=torch.int64)
         if self._packed is None or not self._packed.owns({"0": self.adapter}):
             self._packed = _PackedAdapters({"0": self.adapter})
-        y = self._packed.apply(x2, ids, self.base.weight, self.base.bias, impl="auto")
+        W, base8, bias = self._base_operands()
+        y = self._packed.apply(x2, ids, W, bias, impl="auto", base8=base8, save8=_save8(self.save_input))
         return y.reshape(*lead, self.base.out_features)
 
 
@@ -139,7 +226,8 @@ class _PackedAdapters:
     def scaling(self) -> np.ndarray:
         return np.array([float(a.scaling) for a in self.adapters], dtype=np.float32)
 
-    def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None):
+    def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
+              base8: Optional[ops.Int8Rows] = None, save8: bool = False):
         if x.device.type != "cuda":
             raise RuntimeError(
                 "tlora_b200 computes on CUDA devices only (sm_100a); move the module and inputs to a "
@@ -149,12 +237,19 @@ class _PackedAdapters:
             raise RuntimeError(f"input on {x.device} but adapters on {self.A_pack.device}")
         if x.dtype != self.A_pack.dtype or (W is not None and W.dtype != x.dtype):
             raise RuntimeError(f"dtype mismatch: input {x.dtype}, weights {self.A_pack.dtype}")
+        if base8 is not None and base8.device != x.device:
+            raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
+        if base8 is not None and bias is not None and (bias.dtype != x.dtype or bias.device != x.device):
+            raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
         if W is not None and W.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the backbone is frozen: no dW (tlora/multi_lora_linear.py:78-80)")
         x = x.contiguous()
         if plan is None:
             plan = ops.route(ids, self.table, x.device)
-        st = ops.LayerState(self.table, self.scaling(), plan, self.A_pack, self.B_pack, impl)
+        # nothing is kept for a backward that cannot follow
+        save8 = save8 and torch.is_grad_enabled()
+        st = ops.LayerState(self.table, self.scaling(), plan, self.A_pack, self.B_pack, impl, base8=base8,
+                            save8=save8)
         params = []
         for ad in self.adapters:
             params += [ad.A, ad.B]
@@ -164,14 +259,19 @@ class _PackedAdapters:
             return ops.MultiLoRAFunction.apply(x, Wc, bc, st, *params)
 
 
-class MultiLoRALinear(nn.Module):
+class MultiLoRALinear(_Int8BaseMixin, nn.Module):
     """Shared frozen backbone + heterogeneous-rank adapters, one per job.
 
     tlora/multi_lora_linear.py:59-118.  ``forward(x, adapter_ids)`` takes
     ``x`` [batch, in_features] and per-row adapter ids [batch] in any order;
     rows whose id names no adapter get the backbone output only.  ``impl``
     selects the kernel family: "auto" (tcgen05 for bf16, SIMT otherwise),
-    "tc" or "simt"."""
+    "tc" or "simt".
+
+    ``quantize_base()`` holds the backbone in 8 bits.  ``save_input = "int8"``
+    keeps x in 8 bits (one scale per row) between forward and backward instead
+    of as it is ("full"): half the saved bytes of a 16-bit layer, and dA is
+    computed from the 8-bit rows."""
 
     def __init__(self, in_features: int, out_features: int, adapter_ranks: Dict[int, int], bias: bool = True):
         super().__init__()
@@ -185,6 +285,9 @@ class MultiLoRALinear(nn.Module):
              for adapter_id, rank in adapter_ranks.items()})
         self.impl = "auto"
         self._packed: Optional[_PackedAdapters] = None
+
+    def _adapter_modules(self):
+        return iter(self.adapters.values())
 
     def adapter_parameters(self, adapter_id: int) -> Iterable[nn.Parameter]:
         return self.adapters[str(adapter_id)].parameters()
@@ -202,7 +305,7 @@ class MultiLoRALinear(nn.Module):
     def route(self, adapter_ids: torch.Tensor, device=None) -> ops.RoutePlan:
         """Routing plan of ``adapter_ids``; pass it back as ``plan=`` to reuse
         it across calls with the same ids."""
-        dev = torch.device(device) if device is not None else self.base.weight.device
+        dev = torch.device(device) if device is not None else next(self._adapter_modules()).A.device
         return ops.route(adapter_ids, self._pack().table, dev)
 
     def make_resident(self, plan: ops.RoutePlan) -> None:
@@ -214,8 +317,8 @@ class MultiLoRALinear(nn.Module):
         pk = self._pack()
         pk.sync()
         st = ops.LayerState(pk.table, pk.scaling(), plan, pk.A_pack, pk.B_pack, self.impl)
-        w = self.base.weight
-        ops.make_resident(st, plan.rows, self.base.in_features, self.base.out_features, w.dtype, w.device)
+        ops.make_resident(st, plan.rows, self.base.in_features, self.base.out_features, pk.A_pack.dtype,
+                          pk.A_pack.device)
 
     def packed(self):
         """(A_pack, B_pack, AdapterTable): the packed adapter storage."""
@@ -229,9 +332,9 @@ class MultiLoRALinear(nn.Module):
             raise ValueError("Phase 1 expects x shaped [batch, in_features]")
         if adapter_ids.ndim != 1 or adapter_ids.shape[0] != x.shape[0]:
             raise ValueError("adapter_ids must be [batch] and match x.shape[0]")
-        W = self.base.weight if add_base else None
-        b = self.base.bias if add_base else None
-        return self._pack().apply(x, adapter_ids, W, b, impl=self.impl, plan=plan)
+        W, base8, b = self._base_operands() if add_base else (None, None, None)
+        return self._pack().apply(x, adapter_ids, W, b, impl=self.impl, plan=plan, base8=base8,
+                                  save8=_save8(self.save_input))
 
     @torch.no_grad()
     def sgd_step(self, lr: float, adapter_ids: Optional[Iterable[int]] = None) -> int:

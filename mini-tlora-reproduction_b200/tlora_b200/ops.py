@@ -201,6 +201,192 @@ def scatter_rows(src: torch.Tensor, perm: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------
+# 8-bit rows
+# ---------------------------------------------------------------------------
+
+@dataclass
+class Int8Rows:
+    """A matrix [rows, cols] in 8 bits: int8 ``q`` [rows, ld] and one float
+    ``scale`` [rows]; element (i, k) stands for ``scale[i] * q[i, k]``.  ``ld``
+    is ``cols`` rounded up to 16 and the bytes past ``cols`` are zero.  Rows are
+    tokens of an activation, or output channels of a weight."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+
+    def __post_init__(self):
+        q, s = self.q, self.scale
+        if q.dim() != 2 or q.dtype != torch.int8 or q.shape[1] != q8_ld(self.cols) or not q.is_contiguous():
+            raise ValueError(f"Int8Rows.q must be a contiguous int8 matrix [rows, {q8_ld(self.cols)}]")
+        if s.dim() != 1 or s.dtype != torch.float32 or s.shape[0] != q.shape[0] or not s.is_contiguous():
+            raise ValueError("Int8Rows.scale must be a contiguous float32 vector, one element per row")
+        if s.device != q.device:
+            raise ValueError(f"Int8Rows: q on {q.device} but scale on {s.device}")
+
+    @property
+    def rows(self) -> int:
+        return self.q.shape[0]
+
+    @property
+    def shape(self):
+        return torch.Size((self.q.shape[0], self.cols))
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+
+def q8_ld(cols: int) -> int:
+    """Bytes between the rows of an 8-bit matrix of ``cols`` columns."""
+    return (int(cols) + 15) // 16 * 16
+
+
+def _new_rows8(rows: int, cols: int, device) -> Int8Rows:
+    return Int8Rows(torch.empty(rows, q8_ld(cols), dtype=torch.int8, device=device),
+                    torch.empty(rows, dtype=torch.float32, device=device), cols)
+
+
+def _q8_struct(base8: Optional[Int8Rows], rows8: Optional[Int8Rows], grad8: Optional[Int8Rows] = None):
+    def pair(m):
+        return (m.q.data_ptr(), m.scale.data_ptr()) if m is not None else (None, None)
+
+    return _lib.Q8(*pair(base8), *pair(rows8), *pair(grad8))
+
+
+def _check_cuda(t: torch.Tensor, what: str) -> None:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} computes on CUDA devices only (sm_100a); there is no CPU path")
+
+
+def _row_major(x: torch.Tensor):
+    """(x, elements between rows): rows with unit column stride are read in
+    place, anything else is copied."""
+    if x.shape[0] <= 1 or x.shape[1] <= 1 or x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+        return x, x.shape[1]
+    return x, x.stride(0)
+
+
+@torch.no_grad()
+def quantize_rows(x: torch.Tensor, col_scale: Optional[torch.Tensor] = None) -> Int8Rows:
+    """8-bit rows of ``x`` [rows, cols] (float32, bfloat16 or float16):
+    ``scale[i] = float32(max_k |x[i, k]| / 127)`` and
+    ``q[i, k] = round(x[i, k] / scale[i])``, ties to even, the quotient rounded
+    exactly.  With ``col_scale`` (float32 [cols]) ``x`` is multiplied by it
+    first, in float32.  A row of zeros has scale 0; a row with an infinity or a
+    NaN has scale NaN and zeros.  Differentiable use goes through
+    :func:`int8_linear` and ``MultiLoRALinear``."""
+    _check_cuda(x, "quantize_rows")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("quantize_rows expects x shaped [rows, cols] with at least one column")
+    dt = mlora_dtype(x.dtype)
+    if col_scale is not None and (col_scale.dtype != torch.float32 or col_scale.shape != (x.shape[1],) or
+                                  col_scale.device != x.device):
+        raise ValueError("col_scale must be a float32 vector on x's device, one element per column")
+    with torch.cuda.device(x.device):
+        x, ld = _row_major(x)
+        cs = col_scale.contiguous() if col_scale is not None else None
+        out = _new_rows8(x.shape[0], x.shape[1], x.device)
+        _lib.call("mlora_q8_quantize", _ptr(x), x.shape[0], x.shape[1], ld, dt, _ptr(cs), _ptr(out.q),
+                  _ptr(out.scale), _stream(x.device))
+    return out
+
+
+@torch.no_grad()
+def dequantize_rows(rows8: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The matrix [rows, cols] that 8-bit rows stand for, rounded once to ``dtype``."""
+    _check_cuda(rows8.q, "dequantize_rows")
+    dt = mlora_dtype(dtype)
+    with torch.cuda.device(rows8.device):
+        out = torch.empty(rows8.rows, rows8.cols, dtype=dtype, device=rows8.device)
+        _lib.call("mlora_q8_dequantize", _ptr(rows8.q), _ptr(rows8.scale), rows8.rows, rows8.cols, dt, _ptr(out),
+                  _stream(rows8.device))
+    return out
+
+
+class Int8LinearFunction(torch.autograd.Function):
+    """y = x W^T + b with x and W in 8 bits; dx through the 8-bit rows of
+    dy * (W's scales), no gradient of W or b (both frozen)."""
+
+    @staticmethod
+    def forward(ctx, x, wq, w_scale, bias, d_in):
+        ctx.save_for_backward(wq, w_scale)
+        ctx.d_in = d_in
+        return _int8_product(x, Int8Rows(wq, w_scale, d_in), bias, x.dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        wq, w_scale = ctx.saved_tensors
+        rows, d_out, d_in = dy.shape[0], wq.shape[0], ctx.d_in
+        dev = dy.device
+        with torch.cuda.device(dev):
+            dy = dy.contiguous()
+            g8 = _new_rows8(rows, d_out, dev)
+            dx = torch.empty(rows, d_in, dtype=dy.dtype, device=dev)
+            prob = _lib.Problem(rows, d_in, d_out, mlora_dtype(dy.dtype), _lib.IMPL_AUTO)
+            _lib.call("mlora_q8_linear_dx", ctypes.byref(prob), _ptr(dy), _ptr(g8.q), _ptr(g8.scale), _ptr(wq),
+                      _ptr(w_scale), _ptr(dx), _stream(dev))
+        return dx, None, None, None, None
+
+
+def _int8_product(x, weight: Int8Rows, bias, dtype):
+    dev = weight.device
+    with torch.cuda.device(dev):
+        if isinstance(x, Int8Rows):
+            x8, src, ld = x, None, 0
+        else:
+            src, ld = _row_major(x)
+            x8 = _new_rows8(x.shape[0], x.shape[1], dev)
+        y = torch.empty(x8.rows, weight.rows, dtype=dtype, device=dev)
+        prob = _lib.Problem(x8.rows, weight.cols, weight.rows, mlora_dtype(dtype), _lib.IMPL_AUTO)
+        _lib.call("mlora_q8_linear", ctypes.byref(prob), _ptr(src), ld, _ptr(x8.q), _ptr(x8.scale), _ptr(weight.q),
+                  _ptr(weight.scale), _ptr(bias), _ptr(y), _stream(dev))
+    return y
+
+
+def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
+                dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Matrix product in 8-bit integers with a scale per token and per output
+    channel: ``y[i, j] = s_x[i] s_w[j] sum_k q_x[i, k] q_w[j, k] + bias[j]``.
+
+    ``x`` is a tensor [rows, in_features] (float32, bfloat16 or float16; its
+    rows are quantized as by :func:`quantize_rows`, and the gradient flows back
+    to it) or an :class:`Int8Rows` (rows quantized once for several products;
+    then ``dtype``, or the bias's type, is the type of ``y``).  ``weight`` holds the
+    8-bit rows of W [out_features, in_features] (``quantize_rows(W)``) and is
+    frozen, like the backbone of ``MultiLoRALinear``."""
+    if not isinstance(weight, Int8Rows):
+        raise TypeError("int8_linear expects weight as Int8Rows (quantize_rows(W))")
+    eight = isinstance(x, Int8Rows)
+    _check_cuda(weight.q, "int8_linear")
+    if not eight and x.dim() != 2:
+        raise ValueError("int8_linear expects x shaped [rows, in_features]")
+    if x.shape[1] != weight.cols:
+        raise ValueError(f"x has {x.shape[1]} features, the weight {weight.cols}")
+    if x.device != weight.device:
+        raise RuntimeError(f"input on {x.device} but weight on {weight.device}")
+    if not eight:
+        if dtype is not None and dtype != x.dtype:
+            raise ValueError("dtype applies to 8-bit input; a tensor's product has its own type")
+        dtype = x.dtype
+    elif dtype is None:
+        if bias is None:
+            raise ValueError("int8_linear of 8-bit rows needs the type of y (dtype or bias)")
+        dtype = bias.dtype
+    mlora_dtype(dtype)
+    if bias is not None:
+        if bias.shape != (weight.rows,) or bias.dtype != dtype or bias.device != weight.device:
+            raise ValueError("bias must be a vector of y's type on the weight's device, one element per output")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("the 8-bit linear is frozen: no gradient of its bias")
+        bias = bias.contiguous()
+    if eight:
+        return _int8_product(x, weight, bias, dtype)
+    return Int8LinearFunction.apply(x, weight.q, weight.scale, bias, weight.cols)
+
+
+# ---------------------------------------------------------------------------
 # C structs for one call
 # ---------------------------------------------------------------------------
 
@@ -250,6 +436,10 @@ class LayerState:
     # device int32 tensor that receives the device-side flags of the calls made
     # with this state (bounds bit 0, timeout bit 1); None = the library-wide word
     err_word: Optional[torch.Tensor] = None
+    # the backbone in 8 bits (then W is None), and whether the input is kept
+    # in 8 bits for the backward
+    base8: Optional["Int8Rows"] = None
+    save8: bool = False
 
 
 def _resident_key(rows, d_in, d_out, dtype, st: LayerState):
@@ -285,11 +475,13 @@ def _workspace(st: LayerState, args, wb, device):
     return torch.empty(max(wb, 1), dtype=torch.uint8, device=device), 0
 
 
-def forward_raw(x, W, bias, st: LayerState, x_sorted=None):
+def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8Rows"] = None):
     """Run mlora_forward; returns (Y in the caller's row order, zsave, x in
     sorted order, call args).  With interleaved ids the rows of X are
     gathered into adapter order and the kernels write each row of Y straight
-    to its original position (mlora_routing.out_rows), with no scatter pass."""
+    to its original position (mlora_routing.out_rows), with no scatter pass.
+    With an 8-bit backbone (st.base8) or ``rows8`` the call is
+    mlora_forward_q8; ``rows8`` receives the 8-bit rows of the sorted x."""
     rows, d_in = x.shape
     d_out = st.B_pack.shape[0]
     xs = x_sorted if x_sorted is not None else (gather_rows(x, st.plan.perm) if st.plan.perm is not None else x)
@@ -300,8 +492,15 @@ def forward_raw(x, W, bias, st: LayerState, x_sorted=None):
     y = torch.empty(rows, d_out, dtype=x.dtype, device=dev)
     z = torch.empty(max(zb, 1), dtype=torch.uint8, device=dev)
     ws, args.prob.flags = _workspace(st, args, wb, dev)
-    _lib.call("mlora_forward", ctypes.byref(args.prob), ctypes.byref(args.route), _ptr(xs), _ptr(W), _ptr(bias),
-              _ptr(st.A_pack), _ptr(st.B_pack), _ptr(y), _ptr(z), _ptr(ws), wb, _stream(dev))
+    if st.base8 is None and rows8 is None:
+        _lib.call("mlora_forward", ctypes.byref(args.prob), ctypes.byref(args.route), _ptr(xs), _ptr(W), _ptr(bias),
+                  _ptr(st.A_pack), _ptr(st.B_pack), _ptr(y), _ptr(z), _ptr(ws), wb, _stream(dev))
+        return y, z, xs, args
+    if rows8 is None:
+        rows8 = _new_rows8(rows, d_in, dev)
+    q8 = _q8_struct(st.base8, rows8)
+    _lib.call("mlora_forward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8), _ptr(xs),
+              _ptr(W), _ptr(bias), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(y), _ptr(z), _ptr(ws), wb, _stream(dev))
     return y, z, xs, args
 
 
@@ -370,10 +569,13 @@ class StagedForward:
                   self.n_tiles if t1 is None else t1, ctypes.byref(ar.ar), _stream(self.x.device))
 
 
-def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, want_dB: bool):
+def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, want_dB: bool,
+                 rows8: Optional["Int8Rows"] = None):
     """Run mlora_backward; returns (dX in the caller's row order or None,
     dA_pack or None, dB_pack or None).  dY is gathered into adapter order;
-    dX rows are written straight to their original positions."""
+    dX rows are written straight to their original positions.  With an 8-bit
+    backbone or ``rows8`` (the 8-bit rows of the sorted input, in place of
+    ``xs``) the call is mlora_backward_q8."""
     rows = dy.shape[0]
     d_in = st.A_pack.shape[1]
     d_out = st.B_pack.shape[0]
@@ -388,6 +590,13 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     # rest is never exposed (inactive adapters get None gradients)
     dA = torch.empty_like(st.A_pack) if want_dA else None
     dB = torch.empty_like(st.B_pack) if want_dB else None
+    if st.base8 is not None or rows8 is not None:
+        grad8 = _new_rows8(rows, d_out, dev) if st.base8 is not None and want_dx else None
+        q8 = _q8_struct(st.base8, rows8, grad8)
+        _lib.call("mlora_backward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8),
+                  _ptr(dys), _ptr(xs), _ptr(W), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA),
+                  _ptr(dB), _ptr(ws), wb, _stream(dev))
+        return dx, dA, dB
     _lib.call("mlora_backward", ctypes.byref(args.prob), ctypes.byref(args.route), _ptr(dys), _ptr(xs), _ptr(W),
               _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA), _ptr(dB), _ptr(ws), wb,
               _stream(dev))
@@ -493,21 +702,33 @@ class MultiLoRAFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, W, bias, st: LayerState, *adapter_params):
-        y, z, xs, _ = forward_raw(x, W, bias, st)
         ctx.st = st
-        ctx.save_for_backward(xs, z, W, st.A_pack, st.B_pack)
+        if st.base8 is None and not st.save8:
+            y, z, xs, _ = forward_raw(x, W, bias, st)
+            ctx.save_for_backward(xs, z, W, st.A_pack, st.B_pack)
+            return y
+        # dA alone reads the input in the backward: kept as it is, or in 8 bits
+        keep = any(ctx.needs_input_grad[4::2])
+        rows8 = _new_rows8(x.shape[0], x.shape[1], x.device) if keep and st.save8 else None
+        y, z, xs, _ = forward_raw(x, W, bias, st, rows8=rows8)
+        b8, r8 = st.base8, rows8
+        ctx.save_for_backward(xs if keep and not st.save8 else None, z, W, st.A_pack, st.B_pack,
+                              *((b8.q, b8.scale) if b8 is not None else (None, None)),
+                              *((r8.q, r8.scale) if r8 is not None else (None, None)))
+        ctx.d_in = x.shape[1]
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        xs, z, W, _, _ = ctx.saved_tensors
+        xs, z, W, _, _, *kept = ctx.saved_tensors
         st: LayerState = ctx.st
+        rows8 = Int8Rows(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
         n = st.table.n
         need = ctx.needs_input_grad
         want_dx = need[0]
         want_A = any(need[4 + 2 * i] for i in range(n))
         want_B = any(need[5 + 2 * i] for i in range(n))
-        dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, want_dx, want_A, want_B)
+        dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, want_dx, want_A, want_B, rows8)
         grads = []
         for i in range(n):
             o, r = int(st.table.pack_off[i]), int(st.table.rank[i])

@@ -243,6 +243,8 @@ class ShardedLayer:
             raise ValueError(f"comm must be one of {COMMS}, not {comm!r}")
         if dz not in ("split", "replicated"):
             raise ValueError(f"dz must be 'split' or 'replicated', not {dz!r}")
+        if not hasattr(model.base, "weight"):
+            raise NotImplementedError("a backbone in 8 bits is not sharded: call model.dequantize_base() first")
         self.dz = dz
         # nano-batch ranges over the plan tiles: "even" (the reference's
         # split_ranges) or "ramp" (the first nano-batch half as long, so that
