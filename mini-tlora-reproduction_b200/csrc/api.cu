@@ -119,8 +119,12 @@ int check_q8(std::initializer_list<const void*> mats, std::initializer_list<cons
   return MLORA_OK;
 }
 
-// One 8-bit product.
-int q8_main(const Q8Main& a, cudaStream_t st) { return q8_main_simt(a, st); }
+// One 8-bit product: on the tensor cores where they can run it, whatever its
+// size, unless the call asks for the CUDA cores.
+int q8_main(const Q8Main& a, int impl, cudaStream_t st) {
+  const bool tc = impl != MLORA_IMPL_SIMT && q8_tc_ok(a);
+  return tc ? q8_main_tc(a, st) : q8_main_simt(a, st);
+}
 
 }  // namespace
 }  // namespace mlora
@@ -163,10 +167,17 @@ extern "C" int32_t mlora_num_tiles(int64_t rows) {
 
 namespace {
 
+// Kernel family of the 8-bit product of a layer call whose 16-bit kernels run
+// as `impl`: a call without LoRA rows has no operand that needs the 16-bit
+// family's alignment.
+int q8_impl(const mlora_problem* prob, int impl) {
+  return prob->impl == MLORA_IMPL_AUTO ? MLORA_IMPL_AUTO : impl;
+}
+
 // The 8-bit backbone product of mlora_forward_q8, with the LoRA expand of the
 // intermediate that the shrink before it left in zsave.
 int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8, const PlanDev& dev,
-                    const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
+                    int impl, const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
                     cudaStream_t s) {
   Q8Main m;
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
@@ -177,7 +188,7 @@ int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const
   m.plan = dev; m.zt = zsave; m.pack = B_pack;
   m.max_ctas = prob->max_ctas;
   m.err = prob->err_word;
-  return q8_main(m, s);
+  return q8_main(m, impl, s);
 }
 
 // mlora_forward_staged, or with `ar` mlora_forward_push (MAIN pushes the
@@ -236,7 +247,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     st = tc_forward(a, s);
     if (st != MLORA_OK || !q8_base) return st;
-    return q8_forward_main(prob, route, q8, dev, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), bias, B_pack, Y, zsave, all_stages, s);
   }
   SimtCall a;
   a.plan = dev;
@@ -251,7 +262,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   a.c_end = p.tile_chunk_begin[tile_end];
   st = simt_forward(a, s);
   if (st != MLORA_OK || !q8_base) return st;
-  return q8_forward_main(prob, route, q8, dev, bias, B_pack, Y, zsave, all_stages, s);
+  return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), bias, B_pack, Y, zsave, all_stages, s);
 }
 
 }  // namespace
@@ -365,7 +376,7 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     m.plan = dev; m.zt = dzsave; m.pack = A_pack;
     m.max_ctas = prob->max_ctas;
     m.err = prob->err_word;
-    st = q8_main(m, s);
+    st = q8_main(m, q8_impl(prob, impl), s);
     if (st != MLORA_OK) return st;
   }
   if (!saved8)
@@ -540,7 +551,7 @@ extern "C" int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
   m.Aq = Xq; m.a_scale = x_scale; m.Wq = Wq; m.w_scale = w_scale; m.bias = bias; m.out = Y;
   m.max_ctas = prob->max_ctas; m.err = prob->err_word;
-  return q8_main(m, s);
+  return q8_main(m, prob->impl, s);
 }
 
 extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale,
@@ -559,7 +570,7 @@ extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
   m.Aq = Gq; m.a_scale = g_scale; m.Wq = Wq; m.out = dX;
   m.max_ctas = prob->max_ctas; m.err = prob->err_word;
-  return q8_main(m, s);
+  return q8_main(m, prob->impl, s);
 }
 
 extern "C" int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,

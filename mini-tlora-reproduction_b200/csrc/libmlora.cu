@@ -7,6 +7,7 @@
 #include "q8.cu"
 #include "route.cu"
 #include "tc.cu"
+#include "q8_tc.cu"
 #include "allreduce.cu"
 #include "multimem.cu"
 #include "api.cu"

@@ -44,5 +44,7 @@ struct Q8Main {
 };
 
 int q8_main_simt(const Q8Main& a, cudaStream_t st);
+bool q8_tc_ok(const Q8Main& a);
+int q8_main_tc(const Q8Main& a, cudaStream_t st);
 
 }  // namespace mlora

@@ -1,0 +1,545 @@
+// Tensor-core form of the 8-bit products (tcgen05 kind::i8, s32 accumulators
+// in TMEM, operands staged by TMA).
+//
+//   forward   Y[i, j]  = s_x[i] s_w[j] acc + bias[j] + sum_c Zt[c] Bpack[:, chunk c]^T
+//   backward  dX[i, k] = s_g[i] acc + sum_c dZt[c] Apack[chunk c, :]
+//
+// k_q8: a cluster of two CTAs per 256 x 256 output tile, one
+// tcgen05.mma.cta_group::2 (M = 256, N = 256, K = 32) per 32 bytes of K.  A
+// k-block is 128 bytes of K per row (128-byte swizzle): 16 KB of A and 16 KB
+// of B per CTA, as many bytes as 64 16-bit columns, for twice the products.
+// The weight is stored once, [d_out, d_in]: K-major for the forward, MN-major
+// for dX.
+//
+// The LoRA terms are 16-bit products with fp32 sums and the backbone's sums
+// are integers, so they cannot share an accumulator from the start.  The
+// epilogue warps rewrite a tile's integers in TMEM as the scaled fp32 values
+// (tcgen05.ld, multiply, tcgen05.st), the MMA issuer then adds the tile's
+// expand k-blocks onto them (kind::f16), and the epilogue drains the sum.
+// All of that happens while the next tile's integer mainloop fills the other
+// accumulator: its expand k-blocks sit in the ring after the first kDefer
+// k-blocks of the next tile, by which time the rewrite has finished.
+//
+// Bound by the integer tensor rate for large tiles; the tile order keeps a
+// group of weight blocks in L2 while the rows stream, as in the 16-bit
+// mainloops.  Tiles are dealt round-robin to the resident pairs: all tiles of
+// a launch are equal up to a few expand k-blocks.
+#include "q8.cuh"
+
+namespace mlora {
+namespace {
+
+constexpr int kDefer = 8;       // k-blocks of the next tile before a tile's expand
+constexpr int kQ8K = 128;       // bytes of K per k-block
+constexpr int kQ8Stages = 6;    // 32 KB per CTA each
+constexpr int kQ8StageBytes = 32 * 1024;
+constexpr int kQ8Smem = kQ8Stages * kQ8StageBytes + kStageOut2Bytes + 1024 + 512;
+static_assert(kQ8Smem <= 232448, "dynamic shared memory above 227 KB");
+
+struct Q8Params {
+  CUtensorMap mA, mB;  // 8-bit operands, 128 x 128 byte boxes
+  CUtensorMap mZ, mP;  // 16-bit low-rank blocks and pack of the expand
+  CUtensorMap mY;      // output store map (tma_out)
+  PlanDev plan;
+  int64_t M;
+  int N;
+  int n_tiles, n_nblk, group, n_items;
+  int nk;              // 128-byte k-blocks of the integer product
+  int expand;
+  int dtype;
+  int tma_out;         // 16-bit output rows that TMA can describe, in place
+  const float* a_scale;
+  const float* w_scale;  // forward
+  const void* bias;
+  void* out;
+  const int32_t* out_rows;
+  int* err;
+};
+
+__device__ __forceinline__ void tc_mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// Instruction descriptor of kind::i8: signed 8-bit A and B, s32 accumulator
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n, bool b_mn) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(m >> 4) << 24);
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const float (&f)[32]) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(f[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+struct Q8Item {
+  int t, nb;   // plan tile, 256-wide N block
+  int c0, nc;  // its expand chunks
+};
+
+// Item `i` of the launch: groups of `group` N blocks sweep all tiles.
+__device__ __forceinline__ Q8Item q8_item(const Q8Params& p, int i) {
+  Q8Item it;
+  const int per = p.group * p.n_tiles, g = i / per, r = i % per;
+  const int n0 = g * p.group, gs = min(p.group, p.n_nblk - n0);
+  it.t = r / gs;
+  it.nb = n0 + r % gs;
+  it.c0 = it.nc = 0;
+  if (p.expand) {
+    it.c0 = p.plan.tile_chunk_begin[it.t];
+    it.nc = p.plan.tile_chunk_begin[it.t + 1] - it.c0;
+    if (it.c0 < 0 || it.nc < 0 || it.c0 + it.nc > p.plan.n_chunks) {  // a corrupted plan
+      flag_error(p.err, kErrBounds);
+      it.c0 = it.nc = 0;
+    }
+  }
+  return it;
+}
+
+// 32 fp32 values of columns n0.. of N: multiplied / added elementwise
+template <bool VECTOR_OK = true>
+__device__ __forceinline__ void q8_scale_cols(float (&f)[32], const float* s, int n, int N) {
+  if (n + 32 <= N && VECTOR_OK) {
+    const bool a16 = (reinterpret_cast<uintptr_t>(s + n) & 15) == 0;
+    if (a16) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(s + n) + q);
+        f[4 * q] *= v.x; f[4 * q + 1] *= v.y; f[4 * q + 2] *= v.z; f[4 * q + 3] *= v.w;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 32; ++q)
+    if (n + q < N) f[q] *= __ldg(s + n + q);
+}
+
+template <class T>
+__device__ __forceinline__ void q8_add_bias(float (&f)[32], const T* b, int n, int N) {
+  if (n + 32 <= N && (reinterpret_cast<uintptr_t>(b + n) & 15) == 0) {
+    constexpr int PER = 16 / int(sizeof(T));
+#pragma unroll
+    for (int q = 0; q < 32 / PER; ++q) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + n) + q);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) f[q * PER + k] += to_f(e[k]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 32; ++q)
+    if (n + q < N) f[q] += to_f(b[n + q]);
+}
+
+// One 32 x 32 slice of finished values (lane = row row_w0 + lane, columns n..)
+// to the output.  Warp-collective.
+__device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&f)[32], int64_t row_w0, int n,
+                                               uint32_t buf, int lane) {
+  const bool f16 = p.dtype == MLORA_F16;
+  if (p.tma_out) {
+    if (lane == 0) bulk_wait_read_1();  // the store issued from this buffer two slices ago
+    __syncwarp();
+    const uint32_t rowb = buf + uint32_t(lane) * 64u, sw = uint32_t(lane >> 1) & 3u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      sts128(rowb + ((uint32_t(q) ^ sw) << 4), pack2(f[8 * q], f[8 * q + 1], f16),
+             pack2(f[8 * q + 2], f[8 * q + 3], f16), pack2(f[8 * q + 4], f[8 * q + 5], f16),
+             pack2(f[8 * q + 6], f[8 * q + 7], f16));
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (row_w0 < p.M) tma_store(&p.mY, buf, n, int(row_w0));
+      bulk_commit();
+    }
+    return;
+  }
+  const int64_t row = row_w0 + lane;
+  int64_t orow = row < p.M ? (p.out_rows ? int64_t(p.out_rows[row]) : row) : -1;
+  if (row < p.M && (orow < 0 || orow >= p.M)) {  // out_rows is not a permutation
+    flag_error(p.err, kErrBounds);
+    orow = -1;
+  }
+  if (p.dtype == MLORA_F32) {
+    if (orow < 0) return;
+    float* dst = static_cast<float*>(p.out) + orow * p.N + n;
+    if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        reinterpret_cast<float4*>(dst)[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 32; ++q)
+        if (n + q < p.N) dst[q] = f[q];
+    }
+    return;
+  }
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
+  if (n + 32 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    if (orow >= 0) store32(out + orow * p.N + n, f, f16);
+    return;
+  }
+  // rows that start anywhere: through shared memory, so that a warp writes 32
+  // neighbouring elements of one row at a time
+  __syncwarp();
+  const uint32_t rowb = buf + uint32_t(lane) * 64u, sw = uint32_t(lane >> 1) & 3u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    sts128(rowb + ((uint32_t(q) ^ sw) << 4), pack2(f[8 * q], f[8 * q + 1], f16),
+           pack2(f[8 * q + 2], f[8 * q + 3], f16), pack2(f[8 * q + 4], f[8 * q + 5], f16),
+           pack2(f[8 * q + 6], f[8 * q + 7], f16));
+  __syncwarp();
+  for (int r = 0; r < 32; ++r) {
+    const int64_t o = __shfl_sync(0xffffffffu, orow, r);
+    const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
+                       (uint32_t(lane) & 7u) * 2u;
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+    if (o >= 0 && n + lane < p.N) reinterpret_cast<uint16_t*>(out)[o * p.N + n + lane] = v;
+  }
+}
+
+template <bool BWD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(const __grid_constant__ Q8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* stage_out = smem + kQ8Stages * kQ8StageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kStageOut2Bytes);
+  uint64_t* empty = full + kQ8Stages;
+  uint64_t* ifull = empty + kQ8Stages;  // [2] integer sums of the accumulator complete
+  uint64_t* conv = ifull + 2;           // [2] rewritten as fp32 in both CTAs (used in the even CTA)
+  uint64_t* xfull = conv + 2;           // [2] expand added
+  uint64_t* tempty = xfull + 2;         // [2] drained in both CTAs (used in the even CTA)
+  uint64_t* drain = tempty + 2;         // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t crank = cluster_rank();
+  const bool leader = crank == 0;
+  const int pair = blockIdx.x / 2, n_pairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kQ8Stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&ifull[a], 1);
+      mbar_init(&conv[a], 8);  // one arrival per epilogue warp of both CTAs
+      mbar_init(&xfull[a], 1);
+      mbar_init(&tempty[a], 8);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if ((warp == 0 || warp >= 6) && lane == 0) {
+    // ---------------------------------------------------------------- TMA producers (both CTAs)
+    const uint32_t pid = warp == 0 ? 0u : uint32_t(warp - 5);
+    uint32_t gk = 0;
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued = 0, issued_par = 0;
+    bool ok = true;
+    const uint64_t pol_keep = policy_evict_last(), pol_norm = policy_evict_normal();
+    // the ring slot of the next k-block, when it is this warp's
+    auto claim = [&]() -> int {
+      const int s = (gk++ % kProducers) == pid ? stage : -1;
+      if (s >= 0) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.err)) {
+          ok = false;
+          return -1;
+        }
+        if (leader) mbar_expect_tx(&full[stage], 2 * kQ8StageBytes);
+        issued |= 1u << stage;
+        issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+      }
+      if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+      return s;
+    };
+    auto expand = [&](const Q8Item& it) {
+      for (int i = 0; i < it.nc && ok; ++i) {
+        const int s = claim();
+        if (s < 0) continue;
+        uint8_t* sA = smem + s * kQ8StageBytes;
+        uint8_t* sB = sA + kA2Bytes;
+        const uint32_t bar = mapa(su32(&full[s]), 0);
+        const int c = it.c0 + i, pcol = p.plan.chunks[c].pcol, nh = it.nb * 256 + int(crank) * 128;
+        tma_load_pair(sA, &p.mZ, bar, 0, c * kTileRows + int(crank) * kHalfRows, pol_norm);
+        if (!BWD) {
+          tma_load_pair(sB, &p.mP, bar, pcol, nh, pol_keep);
+        } else {
+          for (int h = 0; h < 2; ++h) tma_load_pair(sB + h * kBox64, &p.mP, bar, nh + 64 * h, pcol, pol_keep);
+        }
+      }
+    };
+    Q8Item last;
+    last.nc = 0;
+    for (int item = pair; item < p.n_items && ok; item += n_pairs) {
+      const Q8Item it = q8_item(p, item);
+      const int row0 = it.t * kTileRows + int(crank) * kHalfRows;
+      const int nh = it.nb * 256 + int(crank) * 128;
+      const int defer = min(kDefer, p.nk);
+      for (int kb = 0; kb < p.nk && ok; ++kb) {
+        if (kb == defer) expand(last);
+        if (!ok) break;
+        const int s = claim();
+        if (s < 0) continue;
+        uint8_t* sA = smem + s * kQ8StageBytes;
+        uint8_t* sB = sA + kA2Bytes;
+        const uint32_t bar = mapa(su32(&full[s]), 0);
+        tma_load_pair(sA, &p.mA, bar, kb * kQ8K, row0, pol_norm);
+        if (!BWD) tma_load_pair(sB, &p.mB, bar, kb * kQ8K, nh, pol_keep);
+        else tma_load_pair(sB, &p.mB, bar, nh, kb * kQ8K, pol_keep);
+      }
+      if (ok && defer == p.nk) expand(last);
+      last = it;
+    }
+    if (ok) expand(last);
+    if (!ok && leader) {
+      // let copies already in flight land before the CTAs exit
+      const unsigned long long t0 = now_ns();
+      for (int s = 0; s < kQ8Stages; ++s) {
+        if (!((issued >> s) & 1u)) continue;
+        while (!mbar_try(su32(&full[s]), (issued_par >> s) & 1u)) {
+          if (now_ns() - t0 > kTimeoutNs) break;
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0 && leader) {
+    // ---------------------------------------------------------------- MMA issuer (even CTA)
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t id_i8 = idesc_i8(256, 256, BWD), id_16 = idesc_16(256, 256, false, BWD, p.dtype == MLORA_F16);
+    const uint32_t i8_step = BWD ? (32 * 128) >> 4 : 32 >> 4;   // 32 rows, or 32 bytes, of K
+    const uint32_t x_step = BWD ? (16 * 128) >> 4 : 32 >> 4;    // 16 rows, or 16 columns, of K
+    const uint32_t x_lbo = BWD ? uint32_t(kBox64) : 16u;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    uint32_t conv_phase[2] = {0, 0};
+    int last_nc = 0;
+    // next filled stage -> its A address
+    auto take = [&](uint32_t& sA) {
+      if (!mbar_wait(&full[stage], phase, abort_flag, p.err)) return ok = false;
+      tc_fence_after();
+      sA = su32(smem + stage * kQ8StageBytes);
+      return true;
+    };
+    auto release = [&]() {
+      tc_commit_pair_both(&empty[stage]);
+      if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+    };
+    // expand of the previous item, on accumulator b
+    auto expand = [&](int b) {
+      if (last_nc == 0) return;
+      if (!mbar_wait_cluster(&conv[b], conv_phase[b], abort_flag, p.err)) { ok = false; return; }
+      conv_phase[b] ^= 1;
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(b * kAccCols);
+      for (int i = 0; i < last_nc; ++i) {
+        uint32_t sA;
+        if (!take(sA)) return;
+        const uint64_t ad = sdesc(sA, 16u, 1024), bd = sdesc(sA + kA2Bytes, x_lbo, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_pair(d, ad + uint64_t(k * 2), bd + uint64_t(k * x_step), id_16, 1);
+        release();
+      }
+      tc_commit_pair_both(&xfull[b]);
+    };
+    for (int item = pair; item < p.n_items && ok; item += n_pairs) {
+      const Q8Item it = q8_item(p, item);
+      if (!mbar_wait_cluster(&tempty[acc], acc_phase ^ 1, abort_flag, p.err)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(acc * kAccCols);
+      const int defer = min(kDefer, p.nk);
+      for (int kb = 0; kb < p.nk && ok; ++kb) {
+        if (kb == defer) expand(acc ^ 1);
+        uint32_t sA;
+        if (!ok || !take(sA)) break;
+        const uint64_t ad = sdesc(sA, 16u, 1024), bd = sdesc(sA + kA2Bytes, 16u, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma_i8_pair(d, ad + uint64_t(k * 2), bd + uint64_t(k * i8_step), id_i8, (kb | k) != 0);
+        release();
+      }
+      if (ok && defer == p.nk) expand(acc ^ 1);
+      if (!ok) break;
+      tc_commit_pair_both(&ifull[acc]);
+      last_nc = it.nc;
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (ok) expand(acc ^ 1);
+    tc_commit_pair_local(drain);
+    const unsigned long long t0 = now_ns();
+    while (!mbar_try(su32(drain), 0)) {
+      if (now_ns() - t0 > kTimeoutNs) { flag_error(p.err, kErrTimeout); break; }
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ---------------------------------------------------------------- epilogue (both CTAs)
+    const int quad = warp % 4;
+    const uint32_t tempty0 = mapa(su32(&tempty[0]), 0), conv0 = mapa(su32(&conv[0]), 0);
+    const uint32_t obuf = su32(stage_out) + uint32_t(warp - 2) * 4096u;
+    uint32_t slices = 0;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    uint32_t x_phase[2] = {0, 0};
+    for (int item = pair; item < p.n_items; item += n_pairs) {
+      const Q8Item it = q8_item(p, item);
+      const int64_t row_w0 = int64_t(it.t) * kTileRows + int(crank) * kHalfRows + quad * 32;
+      const int n0 = it.nb * 256;
+      const float sa = row_w0 + lane < p.M ? __ldg(p.a_scale + row_w0 + lane) : 0.f;
+      const uint32_t tbase = tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kAccCols);
+      if (!mbar_wait(&ifull[acc], acc_phase, abort_flag, p.err)) break;
+      tc_fence_after();
+      auto scaled = [&](int col, float (&f)[32]) {
+        uint32_t v[32];
+        tc_ld32(tbase + col, v);
+#pragma unroll
+        for (int q = 0; q < 32; ++q) f[q] = __int2float_rn(int(v[q])) * sa;
+        if (!BWD) q8_scale_cols(f, p.w_scale, n0 + col, p.N);
+      };
+      const bool expanded = it.nc > 0;
+      if (expanded) {
+        for (int col = 0; col < kAccCols && n0 + col < p.N; col += 32) {
+          float f[32];
+          scaled(col, f);
+          tc_st32(tbase + col, f);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(conv0 + 8u * uint32_t(acc));
+        if (!mbar_wait(&xfull[acc], x_phase[acc], abort_flag, p.err)) break;
+        x_phase[acc] ^= 1;
+        tc_fence_after();
+      }
+      for (int col = 0; col < kAccCols && n0 + col < p.N; col += 32) {
+        float f[32];
+        if (expanded) {
+          uint32_t v[32];
+          tc_ld32(tbase + col, v);
+#pragma unroll
+          for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(v[q]);
+        } else {
+          scaled(col, f);
+        }
+        if (!BWD && p.bias) {
+          if (p.dtype == MLORA_BF16) q8_add_bias(f, static_cast<const __nv_bfloat16*>(p.bias), n0 + col, p.N);
+          else if (p.dtype == MLORA_F16) q8_add_bias(f, static_cast<const __half*>(p.bias), n0 + col, p.N);
+          else q8_add_bias(f, static_cast<const float*>(p.bias), n0 + col, p.N);
+        }
+        q8_store_slice(p, f, row_w0, n0 + col, obuf + (slices & 1u) * 2048u, lane);
+        ++slices;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * uint32_t(acc));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// 2-D map over an 8-bit matrix [rows, cols] with rows ld bytes apart; 128 x
+// 128 byte boxes, 128-byte swizzle.  The extent is q8_ld(cols): its last
+// bytes are zero.
+bool make_map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t ld) {
+  EncodeFn enc = get_encode();
+  if (!enc || rows < 1 || ld < 16 || ld % 16 || reinterpret_cast<uintptr_t>(base) % 16) return false;
+  cuuint64_t dims[2] = {cuuint64_t(ld), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(ld)};
+  cuuint32_t box[2] = {128u, 128u}, estr[2] = {1u, 1u};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+// Any sizes, alignments and types, except that the expand reads 16-bit
+// operands by TMA (a LoRA call of the tensor-core family).
+bool q8_tc_ok(const Q8Main& a) {
+  if (a.expand && (a.dtype == MLORA_F32 || (a.bwd && a.d_in % 8) || !aligned(a.pack, 16) || !aligned(a.zt, 16)))
+    return false;
+  return tc_available();
+}
+
+int q8_main_tc(const Q8Main& a, cudaStream_t st) {
+  Q8Params prm;
+  memset(&prm, 0, sizeof(prm));
+  const int K = a.bwd ? a.d_out : a.d_in, N = a.bwd ? a.d_in : a.d_out;
+  if (!make_map8(&prm.mA, a.Aq, a.M, q8_ld(K)) || !make_map8(&prm.mB, a.Wq, a.d_out, q8_ld(a.d_in)))
+    return MLORA_ERR_UNSUPPORTED;
+  if (a.expand) {
+    const int64_t zrows = int64_t(a.plan.n_chunks) * kTileRows;
+    if (!make_map(&prm.mZ, a.zt, zrows, 64, 128) ||
+        !(a.bwd ? make_map(&prm.mP, a.pack, a.R, a.d_in, 64) : make_map(&prm.mP, a.pack, a.d_out, a.R, 128)))
+      return MLORA_ERR_UNSUPPORTED;
+    prm.expand = 1;
+    prm.plan = a.plan;
+  }
+  prm.M = a.M;
+  prm.N = N;
+  prm.dtype = a.dtype;
+  prm.tma_out = a.dtype != MLORA_F32 && !a.out_rows && N % 8 == 0 && aligned(a.out, 16);
+  if (prm.tma_out && !make_out_map(&prm.mY, a.out, a.M, N)) return MLORA_ERR_UNSUPPORTED;
+  prm.n_tiles = mlora_num_tiles(a.M);
+  prm.n_nblk = (N + 255) / 256;
+  // as for the 16-bit mainloops: about 48 MB of weight blocks stay in L2
+  const double block = 256.0 * K;
+  prm.group = std::max(1, std::min(std::max(4, std::min(16, int(48.0 * (1 << 20) / block + 0.5))), prm.n_nblk));
+  prm.n_items = prm.n_tiles * prm.n_nblk;
+  prm.nk = (K + kQ8K - 1) / kQ8K;
+  prm.a_scale = a.a_scale;
+  prm.w_scale = a.w_scale;
+  prm.bias = a.bias;
+  prm.out = a.out;
+  prm.out_rows = a.out_rows;
+  prm.err = a.err;
+  const int sms = cta_budget(a.max_ctas);
+  if (sms < 2) return MLORA_ERR_UNSUPPORTED;
+  const void* fn = a.bwd ? reinterpret_cast<const void*>(&k_q8<true>) : reinterpret_cast<const void*>(&k_q8<false>);
+  MLORA_CUDA_TRY(set_smem_once(fn, kQ8Smem));
+  const unsigned grid = 2u * unsigned(std::min(prm.n_items, sms / 2));
+  if (a.bwd) k_q8<true><<<grid, kThreads, kQ8Smem, st>>>(prm);
+  else k_q8<false><<<grid, kThreads, kQ8Smem, st>>>(prm);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
+}
+
+}  // namespace mlora

@@ -257,6 +257,9 @@ LAYERS = {
     "tokens": (2048, 1536, {i: [8, 16, 32, 64][i % 4] for i in range(16)}, torch.arange(16)),
     "two_tokens_each": (768, 520, {i: 8 for i in range(8)}, torch.arange(8).repeat(2)),
     "unaligned": (100, 75, {0: 3, 1: 20}, grouped((0, 40), (1, 35))),
+    # several tiles per pair of SMs, with fewer and with more k-blocks than a tile's expand waits for
+    "many_tiles_short": (264, 2312, {0: 24, 1: 64, 2: 100}, grouped((0, 2100), (-1, 300), (1, 1200), (2, 1500))),
+    "many_tiles": (2048, 2312, {i: 16 for i in range(9)}, torch.arange(9).repeat_interleave(563)),
     "wide": (72, 2056, {0: 24, 1: 64}, grouped((0, 400), (1, 200))),
 }
 
