@@ -446,7 +446,11 @@ typedef struct mlora_q8 {
   float* x_scale;        /* [rows] */
   int8_t* Gq;            /* [rows, ld(d_out)] scratch of a backward with Wq that writes dX */
   float* g_scale;        /* [rows] */
+  void* scratch;         /* scratch of a backward of 16-bit tensors that reads Xq for dA:
+                            mlora_q8_scratch_bytes bytes, 16-byte aligned */
+  size_t scratch_bytes;
 } mlora_q8;
+int mlora_q8_scratch_bytes(const mlora_problem* prob, const mlora_routing* route, size_t* bytes);
 
 /* mlora_forward with the backbone product in 8 bits (q8->Wq), and / or with X
  * also written in 8 bits (q8->Xq) for the backward.  The LoRA term reads X as

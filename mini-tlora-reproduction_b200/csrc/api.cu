@@ -33,6 +33,7 @@ int upload_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
   put(p.off_reduce, p.reduce.data(), sizeof(ReduceItem) * p.reduce.size());
   put(p.off_list, p.list.data(), sizeof(int32_t) * p.list.size());
   put(p.off_list_desc, p.list_desc.data(), sizeof(int4) * p.list_desc.size());
+  put(p.off_saved, p.saved.data(), sizeof(SavedItem) * p.saved.size());
   MLORA_CUDA_TRY(cudaMemcpyAsync(ws, host.data(), p.bytes, cudaMemcpyHostToDevice, st));
   uint8_t* b = (uint8_t*)ws;
   std::memset(dev, 0, sizeof(*dev));
@@ -48,6 +49,9 @@ int upload_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
   dev->list = (const int32_t*)(b + p.off_list);
   dev->list_desc = (const int4*)(b + p.off_list_desc);
   dev->counters = (int32_t*)(b + p.off_counters);
+  dev->n_saved = int32_t(p.saved.size());
+  dev->saved = (const SavedItem*)(b + p.off_saved);
+  dev->saved_done = dev->counters + 16;
   return MLORA_OK;
 }
 
@@ -68,6 +72,9 @@ int view_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
   dev->list = (const int32_t*)(b + p.off_list);
   dev->list_desc = (const int4*)(b + p.off_list_desc);
   dev->counters = (int32_t*)(b + p.off_counters);
+  dev->n_saved = int32_t(p.saved.size());
+  dev->saved = (const SavedItem*)(b + p.off_saved);
+  dev->saved_done = dev->counters + 16;
   MLORA_CUDA_TRY(cudaMemsetAsync(dev->counters, 0, p.bytes - p.off_counters, st));
   return MLORA_OK;
 }
@@ -326,6 +333,7 @@ int backward_kernels(const mlora_problem* prob, const mlora_routing* route, cons
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     a.bwd_stages = stages; a.t0 = tile_begin; a.t1 = tile_end; a.db0 = db_begin; a.db1 = db_end;
     a.lr = prob->lr;
+    if (q8) { a.x_scale = q8->x_scale; a.dz8 = q8->scratch; }
     return tc_backward(a, s);
   }
   SimtCall a;
@@ -345,6 +353,20 @@ int backward_kernels(const mlora_problem* prob, const mlora_routing* route, cons
   return simt_backward(a, s);
 }
 
+Q8Saved saved_call(const mlora_problem* prob, const mlora_routing* route, const Plan& p, const PlanDev& dev,
+                   const void* A_pack, void* dA_pack, int32_t stages, const mlora_q8* q8) {
+  Q8Saved c;
+  c.M = prob->rows; c.d_in = prob->d_in; c.dtype = prob->dtype;
+  c.Xq = q8->Xq;
+  c.plan = dev;
+  c.scratch = q8->scratch;
+  c.dA = dA_pack;
+  c.A_upd = (stages & MLORA_BWD_SGD_A) ? const_cast<void*>(A_pack) : nullptr;
+  c.lr = prob->lr;
+  c.max_ctas = prob->max_ctas;
+  return c;
+}
+
 // mlora_backward_q8 on a staged plan: the 8-bit product takes the place of
 // the dX mainloop, the saved 8-bit rows that of X in dA.
 int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Plan& p, const PlanDev& dev, int impl,
@@ -361,7 +383,7 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
   // dZ (and the 16-bit dX), then the 8-bit dX, then the reductions
   int st = backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave,
                             q8_dx ? nullptr : dX, dA_pack, dB_pack, stages & ~reduce, 0, p.n_tiles, 0, nb_out,
-                            nullptr, s);
+                            saved8 && dA_pack ? q8 : nullptr, s);
   if (st != MLORA_OK) return st;
   if (q8_dx) {
     st = q8_quantize(dY, prob->rows, prob->d_out, prob->d_out, prob->dtype, q8->w_scale, q8->Gq, q8->g_scale, s);
@@ -384,7 +406,10 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
                             dB_pack, stages & reduce, 0, p.n_tiles, 0, nb_out, nullptr, s);
   // dA from the saved 8-bit rows, dB as ever
   const int32_t of_a = MLORA_BWD_DA | MLORA_BWD_SGD_A, of_b = MLORA_BWD_DB | MLORA_BWD_SGD_B;
-  if (dA_pack && (stages & MLORA_BWD_DA)) {
+  if (dA_pack && (stages & MLORA_BWD_DA) && impl == MLORA_IMPL_TC) {
+    st = q8_da_tc(saved_call(prob, route, p, dev, A_pack, dA_pack, stages, q8), s);
+    if (st != MLORA_OK) return st;
+  } else if (dA_pack && (stages & MLORA_BWD_DA)) {
     st = backward_kernels(prob, route, p, dev, MLORA_IMPL_SIMT, dY, nullptr, W, A_pack, B_pack, zsave, dzsave,
                           nullptr, dA_pack, nullptr, stages & of_a, 0, p.n_tiles, 0, nb_out, q8, s);
     if (st != MLORA_OK) return st;
@@ -432,6 +457,11 @@ int backward_staged(const mlora_problem* prob, const mlora_routing* route, const
   if (!aligned(workspace, 16)) return MLORA_ERR_UNSUPPORTED;  // plan tables hold 16-byte entries
   const int impl = choose_impl(prob, {dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack});
   if (impl < 0) return MLORA_ERR_UNSUPPORTED;
+  if (saved8 && lora && dA_pack && (stages & MLORA_BWD_DA) && impl == MLORA_IMPL_TC) {
+    if (!q8->scratch) return MLORA_ERR_INVALID_ARG;
+    if (!aligned(q8->scratch, 16)) return MLORA_ERR_UNSUPPORTED;
+    if (q8->scratch_bytes < q8_scratch_bytes(p)) return MLORA_ERR_WORKSPACE;
+  }
   cudaStream_t s = (cudaStream_t)stream;
   PlanDev dev;
   st = stage_plan(prob, p, workspace, s, &dev);
@@ -511,6 +541,15 @@ int check_q8_problem(const mlora_problem* prob) {
 }
 
 }  // namespace
+
+extern "C" int mlora_q8_scratch_bytes(const mlora_problem* prob, const mlora_routing* route, size_t* bytes) {
+  if (!bytes) return MLORA_ERR_INVALID_ARG;
+  Plan p;
+  int st = build_plan(prob, route, &p);
+  if (st != MLORA_OK) return st;
+  *bytes = prob->dtype == MLORA_F32 ? 0 : q8_scratch_bytes(p);
+  return MLORA_OK;
+}
 
 extern "C" int mlora_q8_quantize(const void* src, int64_t rows, int64_t cols, int64_t ld_src, int32_t dtype,
                                  const float* col_scale, int8_t* q, float* scale, void* stream) {

@@ -49,10 +49,22 @@ struct ReduceItem {
   int32_t nks;                  // 64-row slices of the adapter's tiles that hold its rows (the K extent)
 };
 
+// Work item of dA from inputs saved in 8 bits: one 64-column rank chunk of one
+// adapter, one 256-wide block of d_in, summed over nks of the 64-row slices of
+// the adapter's list, from slice q0 of entry e0 on.  The slices of one output
+// block may be split over nparts items (the same group); the item that
+// finishes last adds the parts up in their order.
+struct SavedItem {
+  int32_t j, block, e0, q0;
+  int32_t nks, lb, le, rank;
+  int32_t part, nparts, group, part0;  // part0: index of the group's first part among the stored parts
+};
+static_assert(sizeof(SavedItem) == 48, "SavedItem is 48 bytes");
+
 // Device-side plan header, followed in the workspace by the arrays.
 struct PlanDev {
-  int32_t n_tiles, n_chunks, n_shrink, n_reduce, n_list;
-  int32_t pad[3];
+  int32_t n_tiles, n_chunks, n_shrink, n_reduce, n_list, n_saved;
+  int32_t pad[2];
   const int32_t* tile_chunk_begin;  // [n_tiles + 1]
   const Chunk* chunks;              // [n_chunks]
   const ShrinkItem* shrink;         // [n_shrink]
@@ -61,6 +73,8 @@ struct PlanDev {
   const int4* list_desc;            // [n_list] {base chunk, tile, first 64-row slice, one past the last}
   int32_t* counters;                // [16] work counters of the persistent kernels, one per role;
                                     // zeroed by every plan upload (one per API call)
+  const SavedItem* saved;           // [n_saved]
+  int32_t* saved_done;              // [saved groups] finished parts, zeroed with the counters
   int* err;                         // status word of this call (mlora_problem.err_word), or nullptr
                                     // for the library-wide word g_err_word
 };
@@ -73,13 +87,15 @@ struct Plan {
   std::vector<Chunk> chunks;
   std::vector<ShrinkItem> shrink;
   std::vector<ReduceItem> reduce;
+  std::vector<SavedItem> saved;
+  int32_t saved_groups = 0, saved_parts = 0;  // groups of several parts, and their parts
   std::vector<int32_t> list;
   std::vector<int4> list_desc;      // per list entry: {base chunk, tile, first slice, end slice}
   std::vector<int32_t> list_begin;  // [n_adapters + 1]
   std::vector<uint8_t> adapter_active;
   // byte layout of the plan inside the workspace
   size_t off_tcb = 0, off_chunks = 0, off_shrink = 0, off_reduce = 0, off_list = 0, off_list_desc = 0,
-         off_counters = 0, bytes = 0;
+         off_saved = 0, off_counters = 0, bytes = 0;
 };
 
 int build_plan(const mlora_problem* prob, const mlora_routing* route, Plan* plan);

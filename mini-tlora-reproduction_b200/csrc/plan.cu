@@ -53,6 +53,8 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
   p->chunks.clear();
   p->shrink.clear();
   p->reduce.clear();
+  p->saved.clear();
+  p->saved_groups = p->saved_parts = 0;
   p->list.clear();
   const int nad = r->n_adapters;
   p->adapter_active.assign(nad, 0);
@@ -153,6 +155,59 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
   std::stable_sort(p->reduce.begin(), p->reduce.end(),
                    [](const ReduceItem& x, const ReduceItem& y) { return x.nks > y.nks; });
 
+  // items of dA from saved 8-bit inputs: the slices of an output block are
+  // split so that there are about two items per SM of a B200 (2 x 148) of
+  // much the same length, but none under kSavedMin slices, whose part would
+  // cost as much to store and add as to compute
+  {
+    constexpr int64_t kSavedItems = 296, kSavedMin = 32;
+    const int nb = (prob->d_in + 255) / 256;
+    std::vector<int32_t> nks(nad, 0);
+    int64_t work = 0;
+    for (int a = 0; a < nad; ++a) {
+      for (int e = p->list_begin[a]; e < p->list_begin[a + 1]; ++e) nks[a] += p->list_desc[e].w - p->list_desc[e].z;
+      work += int64_t(nks[a]) * nb * ((r->rank[a] + kChunk - 1) / kChunk);
+    }
+    const int64_t quota = std::max<int64_t>(kSavedMin, (work + kSavedItems - 1) / kSavedItems);
+    for (int a = 0; a < nad; ++a) {
+      const int lb = p->list_begin[a], le = p->list_begin[a + 1];
+      if (le == lb) continue;
+      const int parts = int((nks[a] + quota - 1) / quota);
+      const int nch = (r->rank[a] + kChunk - 1) / kChunk;
+      // the first entry and slice of every part
+      std::vector<std::pair<int, int>> from;
+      for (int k = 0, e = lb, q = p->list_desc[lb].z, k0 = 0; k < parts; ++k) {
+        const int k1 = int(int64_t(nks[a]) * k / parts);
+        for (; k0 < k1; ++k0)
+          if (++q >= p->list_desc[e].w && ++e < le) q = p->list_desc[e].z;
+        from.push_back({e, q});
+      }
+      for (int b = 0; b < nb; ++b)
+        for (int j = 0; j < nch; ++j) {
+          const int group = parts > 1 ? p->saved_groups++ : 0, part0 = p->saved_parts;
+          if (parts > 1) p->saved_parts += parts;
+          for (int k = 0; k < parts; ++k) {
+            SavedItem it;
+            it.j = j;
+            it.block = b;
+            it.e0 = from[k].first;
+            it.q0 = from[k].second;
+            it.nks = int(int64_t(nks[a]) * (k + 1) / parts - int64_t(nks[a]) * k / parts);
+            it.lb = lb;
+            it.le = le;
+            it.rank = r->rank[a];
+            it.part = k;
+            it.nparts = parts;
+            it.group = group;
+            it.part0 = part0;
+            p->saved.push_back(it);
+          }
+        }
+    }
+    std::stable_sort(p->saved.begin(), p->saved.end(),
+                     [](const SavedItem& x, const SavedItem& y) { return x.nks > y.nks; });
+  }
+
   // workspace layout
   size_t off = align_up(sizeof(PlanDev), 256);
   p->off_tcb = off;
@@ -167,8 +222,10 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
   off = align_up(off + sizeof(int32_t) * p->list.size(), 256);
   p->off_list_desc = off;
   off = align_up(off + sizeof(int4) * p->list_desc.size(), 256);
-  p->off_counters = off;
-  off = align_up(off + 64, 256);
+  p->off_saved = off;
+  off = align_up(off + sizeof(SavedItem) * p->saved.size(), 256);
+  p->off_counters = off;  // the persistent kernels' counters, then the saved groups' (all zeroed per call)
+  off = align_up(off + 64 + sizeof(int32_t) * size_t(p->saved_groups), 256);
   p->bytes = off;
   return MLORA_OK;
 }

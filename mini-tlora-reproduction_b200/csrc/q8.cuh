@@ -43,6 +43,29 @@ struct Q8Main {
   int* err = nullptr;
 };
 
+// dA from inputs saved in 8 bits (tensor-core family):
+//   dA chunk = sum_i (x_scale[i] dZ[i, :])^T Xq[i, :]
+// `scratch`: x_scale dZ as bf16 high and low parts, [2][n_chunks][256][64],
+// left by the backward shrink, then the parts of split items.
+struct Q8Saved {
+  int64_t M = 0;
+  int d_in = 0, dtype = MLORA_BF16;
+  const int8_t* Xq = nullptr;
+  PlanDev plan = {};
+  void* scratch = nullptr;
+  void* dA = nullptr;
+  void* A_upd = nullptr;  // fused SGD step on A_pack
+  float lr = 0.f;
+  int max_ctas = 0;
+};
+constexpr int kSavedCols = 256;  // d_in columns of an item
+
+inline size_t q8_dz8_bytes(size_t n_chunks) { return 2 * n_chunks * kTileRows * kChunk * 2; }
+inline size_t q8_scratch_bytes(const Plan& p) {
+  return q8_dz8_bytes(p.chunks.size()) + size_t(p.saved_parts) * kChunk * kSavedCols * 4;
+}
+int q8_da_tc(const Q8Saved& a, cudaStream_t st);
+
 int q8_main_simt(const Q8Main& a, cudaStream_t st);
 bool q8_tc_ok(const Q8Main& a);
 int q8_main_tc(const Q8Main& a, cudaStream_t st);

@@ -84,6 +84,12 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const float (&f)[32]) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Bounded wait of a whole warp: true only if every lane's wait succeeded, so
+// that the lanes go on, or give up, together.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, err));
+}
+
 struct Q8Item {
   int t, nb;   // plan tile, 256-wide N block
   int c0, nc;  // its expand chunks
@@ -416,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
       const int n0 = it.nb * 256;
       const float sa = row_w0 + lane < p.M ? __ldg(p.a_scale + row_w0 + lane) : 0.f;
       const uint32_t tbase = tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kAccCols);
-      if (!mbar_wait(&ifull[acc], acc_phase, abort_flag, p.err)) break;
+      if (!warp_wait(&ifull[acc], acc_phase, abort_flag, p.err)) break;
       tc_fence_after();
       auto scaled = [&](int col, float (&f)[32]) {
         uint32_t v[32];
@@ -436,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(conv0 + 8u * uint32_t(acc));
-        if (!mbar_wait(&xfull[acc], x_phase[acc], abort_flag, p.err)) break;
+        if (!warp_wait(&xfull[acc], x_phase[acc], abort_flag, p.err)) break;
         x_phase[acc] ^= 1;
         tc_fence_after();
       }
@@ -475,15 +481,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
   }
 }
 
-// 2-D map over an 8-bit matrix [rows, cols] with rows ld bytes apart; 128 x
-// 128 byte boxes, 128-byte swizzle.  The extent is q8_ld(cols): its last
+// 2-D map over an 8-bit matrix [rows, cols] with rows ld bytes apart; boxes of
+// box_rows x 128 bytes, 128-byte swizzle.  The extent is q8_ld(cols): its last
 // bytes are zero.
-bool make_map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t ld) {
+bool make_map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t ld, int box_rows = 128) {
   EncodeFn enc = get_encode();
   if (!enc || rows < 1 || ld < 16 || ld % 16 || reinterpret_cast<uintptr_t>(base) % 16) return false;
   cuuint64_t dims[2] = {cuuint64_t(ld), cuuint64_t(rows)};
   cuuint64_t strides[1] = {cuuint64_t(ld)};
-  cuuint32_t box[2] = {128u, 128u}, estr[2] = {1u, 1u};
+  cuuint32_t box[2] = {128u, cuuint32_t(box_rows)}, estr[2] = {1u, 1u};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -538,6 +544,416 @@ int q8_main_tc(const Q8Main& a, cudaStream_t st) {
   const unsigned grid = 2u * unsigned(std::min(prm.n_items, sms / 2));
   if (a.bwd) k_q8<true><<<grid, kThreads, kQ8Smem, st>>>(prm);
   else k_q8<false><<<grid, kThreads, kQ8Smem, st>>>(prm);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
+}
+
+}  // namespace mlora
+
+// ------------------------------------------------------------------ dA from saved 8-bit inputs
+//   dA chunk [64 ranks, 256 columns] = sum_i w[i, :]^T Xq[i, :],   w = x_scale dZ
+//
+// k_q8_da reads every saved byte once per rank chunk and is meant to be bound
+// by that.  The scales went into w (fp32, then two bf16 numbers: 16 bits), so
+// the integers enter the product as they are: eight warps turn each 64 x 256
+// block of bytes into bf16 (exact up to 256) in the layout of an MN-major
+// operand, and one M = 128, N = 256 MMA per 16 rows multiplies the stacked
+// high and low parts of w (ranks 0..63 twice) with it.  The high and the low
+// sums are added in the epilogue.
+//
+// Per 64 rows of a block the shared memory moves 32 KB in by TMA, 48 KB
+// through the conversion and 48 KB into the MMAs, about 1000 cycles, against
+// 700 cycles of the SM's share of HBM for the 16 KB of new bytes.
+//
+// Long sums are split over several items (SavedItem): each stores its fp32
+// block, and the last to finish adds the blocks in their order, so the result
+// does not depend on which one that is.
+namespace mlora {
+namespace {
+
+constexpr int kDaStages = 4, kDaStageBytes = 32 * 1024;  // 64 x 256 bytes of X, 2 x 64 x 64 of w
+constexpr int kDaConv = 2, kDaConvBytes = 32 * 1024;     // 64 x 256 bf16
+constexpr int kDaConvWarps = 8, kDaProducers = 2;
+constexpr int kDaThreads = 32 * (4 + kDaConvWarps + 1 + kDaProducers);
+constexpr int kDaSumBytes = 2 * 32 * 32 * 4;             // low sums of one 32-column slice, two warps
+constexpr int kDaSmem = kDaStages * kDaStageBytes + kDaConv * kDaConvBytes + kDaSumBytes + 1024 + 512;
+static_assert(kDaSmem <= 232448, "dynamic shared memory above 227 KB");
+
+struct DaParams {
+  CUtensorMap mX;  // saved rows, 128-byte x 64-row boxes
+  CUtensorMap mW;  // [2 n_chunks 256, 64] high parts, then low parts
+  PlanDev plan;
+  int d_in, f16, zrows;
+  float* parts;  // stored parts, [.][64][256]
+  __nv_bfloat16* dA;
+  __nv_bfloat16* A_upd;
+  float lr;
+};
+
+// Item `i`; false (and flagged) if the plan is corrupted.
+__device__ __forceinline__ bool da_item(const DaParams& p, int i, SavedItem& it) {
+  it = p.plan.saved[i];
+  const bool ok = it.lb >= 0 && it.le <= p.plan.n_list && it.e0 >= it.lb && it.e0 < it.le && it.j >= 0 &&
+                  it.block >= 0 && it.nks > 0 && it.nks <= 4 * (it.le - it.lb) && it.part >= 0 &&
+                  it.part < it.nparts;
+  if (!ok) flag_error(p.plan.err, kErrBounds);
+  return ok;
+}
+
+// {chunk, tile, first slice, end slice} of list entry e (clamped and flagged
+// if the plan is corrupted)
+__device__ __forceinline__ int4 da_entry(const DaParams& p, int e) {
+  int4 d = p.plan.list_desc[e];
+  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > 4 || d.z >= d.w) {
+    flag_error(p.plan.err, kErrBounds);
+    d = make_int4(0, 0, 0, 1);
+  }
+  return d;
+}
+
+// two bytes of `w` (selected into the low bytes of the halves) as bf16: a
+// byte with bits s vvvvvvv stands for vvvvvvv - 128 s, and (128 + vvvvvvv) -
+// (128 + 128 s) is exact
+__device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t w, uint32_t sel) {
+  const uint32_t b = __byte_perm(w, 0, sel);
+  const uint32_t m = (b & 0x007f007fu) | 0x43004300u, c = (b & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 r =
+      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+__global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__ DaParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* conv = smem + kDaStages * kDaStageBytes;
+  float* sums = reinterpret_cast<float*>(conv + kDaConv * kDaConvBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sums) + kDaSumBytes);
+  uint64_t* empty = full + kDaStages;   // the converting warps and the MMAs
+  uint64_t* cfull = empty + kDaStages;  // [kDaConv] converted
+  uint64_t* cempty = cfull + kDaConv;   // [kDaConv] read by the MMAs
+  uint64_t* tfull = cempty + kDaConv;   // [2]
+  uint64_t* tempty = tfull + 2;         // [2]
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* last_part = abort_flag + 1;  // [2] per pair of epilogue warps
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  constexpr int kMma = 4 + kDaConvWarps;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kDaStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kDaConvWarps + 1);
+    }
+    for (int s = 0; s < kDaConv; ++s) {
+      mbar_init(&cfull[s], kDaConvWarps);
+      mbar_init(&cempty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int n_items = p.plan.n_saved;
+
+  if (warp > kMma && lane == 0) {
+    // ---------------------------------------------------------------- TMA producers (alternate k-blocks)
+    const uint32_t pid = uint32_t(warp - kMma - 1);
+    uint32_t gk = 0, phase = 0, issued = 0, issued_par = 0;
+    int stage = 0;
+    bool ok = true;
+    const uint64_t pol_stream = policy_evict_first(), pol_norm = policy_evict_normal();
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      SavedItem it;
+      if (!da_item(p, item, it)) continue;
+      int e = it.e0, q = it.q0;
+      int4 d = da_entry(p, e);
+      for (int kb = 0; kb < it.nks; ++kb) {
+        if ((gk++ % kDaProducers) == pid) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.plan.err)) { ok = false; break; }
+          uint8_t* sX = smem + stage * kDaStageBytes;
+          uint8_t* sW = sX + 16 * 1024;
+          mbar_expect_tx(&full[stage], kDaStageBytes);
+          for (int h = 0; h < 2; ++h)
+            tma_load(sX + h * 8192, &p.mX, &full[stage], it.block * kSavedCols + 128 * h, d.y * kTileRows + 64 * q,
+                     pol_stream);
+          const int wrow = (d.x + it.j) * kTileRows + 64 * q;
+          for (int h = 0; h < 2; ++h)
+            tma_load(sW + h * kBox64, &p.mW, &full[stage], 0, wrow + h * p.zrows, pol_norm);
+          issued |= 1u << stage;
+          issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+        }
+        if (++stage == kDaStages) { stage = 0; phase ^= 1; }
+        if (++q >= d.w && ++e < it.le) {
+          d = da_entry(p, e);
+          q = d.z;
+        }
+      }
+    }
+    if (!ok) {
+      const unsigned long long t0 = now_ns();
+      for (int s = 0; s < kDaStages; ++s) {
+        if (!((issued >> s) & 1u)) continue;
+        while (!mbar_try(su32(&full[s]), (issued_par >> s) & 1u)) {
+          if (now_ns() - t0 > kTimeoutNs) break;
+        }
+      }
+    }
+  } else if (warp == kMma && lane == 0) {
+    // ---------------------------------------------------------------- MMA issuer
+    int stage = 0, cs = 0, acc = 0;
+    uint32_t phase = 0, cphase = 0, acc_phase = 0;
+    bool ok = true;
+    const uint32_t idesc = idesc_16(128, 256, true, true, false);  // bf16 for either type of the layer
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      SavedItem it;
+      if (!da_item(p, item, it)) continue;
+      if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(acc * kAccCols);
+      for (int kb = 0; kb < it.nks; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, p.plan.err) ||
+            !mbar_wait(&cfull[cs], cphase, abort_flag, p.plan.err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t ad = sdesc(su32(smem + stage * kDaStageBytes) + 16u * 1024u, uint32_t(kBox64), 1024);
+        const uint64_t bd = sdesc(su32(conv + cs * kDaConvBytes), uint32_t(kBox64), 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma(d, ad + uint64_t(k * 128), bd + uint64_t(k * 128), idesc, (kb | k) != 0);
+        tc_commit(&empty[stage]);
+        tc_commit(&cempty[cs]);
+        if (++stage == kDaStages) { stage = 0; phase ^= 1; }
+        if (++cs == kDaConv) { cs = 0; cphase ^= 1; }
+      }
+      if (!ok) break;
+      tc_commit(&tfull[acc]);
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    tc_commit(drain);
+    const unsigned long long t0 = now_ns();
+    while (!mbar_try(su32(drain), 0)) {
+      if (now_ns() - t0 > kTimeoutNs) { flag_error(p.plan.err, kErrTimeout); break; }
+    }
+  } else if (warp >= 4 && warp < kMma) {
+    // ---------------------------------------------------------------- conversion
+    // 16-byte piece c (0..7) of row k of 128-column half h: columns 16 c.. of
+    // the half become two 16-byte groups of bf16 box 2 h + c / 4.  Lanes of
+    // the upper boxes write their second group first, so that a quarter warp
+    // covers all banks.
+    const int t = (warp - 4) * 32 + lane;  // 0..255
+    int stage = 0, cs = 0;
+    uint32_t phase = 0, cphase = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      SavedItem it;
+      if (!da_item(p, item, it)) continue;
+      for (int kb = 0; kb < it.nks; ++kb) {
+        if (!warp_wait(&full[stage], phase, abort_flag, p.plan.err) ||
+            !warp_wait(&cempty[cs], cphase ^ 1, abort_flag, p.plan.err)) {
+          ok = false;
+          break;
+        }
+        const uint32_t src = su32(smem + stage * kDaStageBytes), dst = su32(conv + cs * kDaConvBytes);
+        const uint32_t c = uint32_t(t & 7), k0 = uint32_t(t >> 3);  // rows k0 and k0 + 32 of both halves
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h = uint32_t(i) >> 1, k = k0 + 32u * (uint32_t(i) & 1u);
+          v[i] = lds128(src + h * 8192u + k * 128u + ((c ^ (k & 7u)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h = uint32_t(i) >> 1, k = k0 + 32u * (uint32_t(i) & 1u);
+          const uint32_t row = dst + (2u * h + (c >> 2)) * uint32_t(kBox64) + k * 128u;
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            o[2 * q] = bytes_to_bf16x2(w[q], 0x4140);
+            o[2 * q + 1] = bytes_to_bf16x2(w[q], 0x4342);
+          }
+          const uint32_t g = (c & 3u) * 2u, first = c >> 2;
+          const uint32_t a0 = row + (((g + first) ^ (k & 7u)) << 4), a1 = row + (((g + 1u - first) ^ (k & 7u)) << 4);
+          if (first) {
+            sts128(a0, o[4], o[5], o[6], o[7]);
+            sts128(a1, o[0], o[1], o[2], o[3]);
+          } else {
+            sts128(a0, o[0], o[1], o[2], o[3]);
+            sts128(a1, o[4], o[5], o[6], o[7]);
+          }
+        }
+        fence_async_smem();  // the MMAs read what was written here
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&cfull[cs]);
+          mbar_arrive(&empty[stage]);
+        }
+        if (++stage == kDaStages) { stage = 0; phase ^= 1; }
+        if (++cs == kDaConv) { cs = 0; cphase ^= 1; }
+      }
+    }
+  } else if (warp < 4) {
+    // ---------------------------------------------------------------- epilogue
+    // Lanes 0..63 of the accumulator hold the high sums of ranks 0..63 (warps
+    // 0 and 1), lanes 64..127 the low sums (warps 2 and 3): warp 2 + i hands
+    // its sums to warp i through shared memory.
+    const int half = warp & 1;  // ranks 32 half ..
+    const bool low = warp >= 2;
+    float* mine = sums + half * 32 * 32;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+      SavedItem it;
+      if (!da_item(p, item, it)) continue;
+      // both warps of a pair must agree to go on before they meet at a barrier
+      ok = warp_wait(&tfull[acc], acc_phase, abort_flag, p.plan.err);
+      if (lane == 0 && low) last_part[half] = ok ? 1 : 0;
+      pair_barrier(1 + half);
+      const bool both = ok && last_part[half] != 0;
+      pair_barrier(1 + half);
+      if (lane == 0 && !low) last_part[half] = both ? 1 : 0;
+      pair_barrier(1 + half);
+      if (last_part[half] == 0) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem + (uint32_t(warp * 32) << 16) + uint32_t(acc * kAccCols);
+      const int c0 = it.block * kSavedCols;
+      const int r = 32 * half + lane;              // rank row inside the chunk
+      const int pcol = p.plan.chunks[p.plan.list[it.lb] + it.j].pcol;
+      const bool live = r < it.rank - it.j * 64;
+      float* part = it.nparts > 1 ? p.parts + (int64_t(it.part0 + it.part) * 64 + r) * kSavedCols : nullptr;
+      auto finish = [&](int col, const float (&f)[32]) {
+        // 32 columns of one rank row of dA: 64 contiguous bytes (d_in is a multiple of 8)
+        const int64_t e0 = int64_t(pcol + r) * p.d_in + c0 + col;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (!live || c0 + col + 8 * g >= p.d_in) break;
+          uint32_t w[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) w[h] = pack2(f[8 * g + 2 * h], f[8 * g + 2 * h + 1], p.f16 != 0);
+          reinterpret_cast<uint4*>(p.dA + e0)[g] = make_uint4(w[0], w[1], w[2], w[3]);
+          if (p.A_upd) {  // fused SGD step, from the gradient as stored
+            uint4* P = reinterpret_cast<uint4*>(p.A_upd + e0) + g;
+            const uint4 old = *P;
+            uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const float2 g2 = unpack2(w[h], p.f16 != 0), o2 = unpack2(o[h], p.f16 != 0);
+              o[h] = pack2(sgd_new(o2.x, g2.x, p.lr, p.f16 != 0), sgd_new(o2.y, g2.y, p.lr, p.f16 != 0), p.f16 != 0);
+            }
+            *P = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+      };
+      for (int col = 0; col < kSavedCols && c0 + col < p.d_in; col += 32) {
+        uint32_t v[32];
+        tc_ld32(tbase + col, v);
+        if (low) {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) mine[lane * 32 + ((q + lane) & 31)] = __uint_as_float(v[q]);
+        }
+        pair_barrier(1 + half);
+        if (!low) {
+          float f[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(v[q]) + mine[lane * 32 + ((q + lane) & 31)];
+          if (part) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              __stcg(reinterpret_cast<float4*>(part + col) + q,
+                     make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]));
+          } else {
+            finish(col, f);
+          }
+        }
+        pair_barrier(1 + half);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+      if (it.nparts > 1 && !low) {
+        // this warp's 32 ranks of the part are stored: the warp that stores
+        // the last part of these ranks adds them all up, in order
+        int last = 0;
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          last = atomicAdd(p.plan.saved_done + it.group, half ? 1 << 16 : 1);
+          last = (half ? last >> 16 : last & 0xffff) == it.nparts - 1;
+        }
+        last = __shfl_sync(0xffffffffu, last, 0);
+        __threadfence();
+        if (last) {
+          for (int col = 0; col < kSavedCols && c0 + col < p.d_in; col += 32) {
+            float f[32];
+#pragma unroll
+            for (int q = 0; q < 32; ++q) f[q] = 0.f;
+            for (int k = 0; k < it.nparts; ++k) {
+              const float* src = p.parts + (int64_t(it.part0 + k) * 64 + r) * kSavedCols + col;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float4 u = __ldcg(reinterpret_cast<const float4*>(src) + q);
+                f[4 * q] += u.x; f[4 * q + 1] += u.y; f[4 * q + 2] += u.z; f[4 * q + 3] += u.w;
+              }
+            }
+            finish(col, f);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+}  // namespace
+
+int q8_da_tc(const Q8Saved& a, cudaStream_t st) {
+  if (a.plan.n_saved == 0) return MLORA_OK;
+  DaParams prm;
+  memset(&prm, 0, sizeof(prm));
+  const int64_t zrows = int64_t(a.plan.n_chunks) * kTileRows;
+  if (2 * zrows > INT32_MAX) return MLORA_ERR_UNSUPPORTED;
+  if (!make_map8(&prm.mX, a.Xq, a.M, q8_ld(a.d_in), 64) || !make_map(&prm.mW, a.scratch, 2 * zrows, 64, 64))
+    return MLORA_ERR_UNSUPPORTED;
+  prm.plan = a.plan;
+  prm.d_in = a.d_in;
+  prm.f16 = a.dtype == MLORA_F16 ? 1 : 0;
+  prm.zrows = int(zrows);
+  prm.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.scratch) + q8_dz8_bytes(a.plan.n_chunks));
+  prm.dA = static_cast<__nv_bfloat16*>(a.dA);
+  prm.A_upd = static_cast<__nv_bfloat16*>(a.A_upd);
+  prm.lr = a.lr;
+  const int sms = cta_budget(a.max_ctas);
+  if (sms <= 0) return MLORA_ERR_CUDA;
+  MLORA_CUDA_TRY(set_smem_once(reinterpret_cast<const void*>(&k_q8_da), kDaSmem));
+  k_q8_da<<<std::min(a.plan.n_saved, sms), kDaThreads, kDaSmem, st>>>(prm);
   count_launch();
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }

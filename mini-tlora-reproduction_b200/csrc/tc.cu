@@ -144,6 +144,10 @@ struct TcParams {
   __nv_bfloat16* A_upd;
   __nv_bfloat16* B_upd;
   float lr;
+  // backward shrink: x_scale[row] dZ in two bf16 parts, high at dz8 and low
+  // n_chunks blocks after it (nullptr = not wanted)
+  const float* x_scale;
+  __nv_bfloat16* dz8;
   // forward main with the peer all-reduce: partial tiles go to their owner
   // rank's receive buffer (slot ar_rank) instead of Y
   int ar_on, ar_rank, ar_world, ar_lt_stride;
@@ -959,6 +963,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
 #pragma unroll
             for (int q = 0; q < 32; ++q) f[q] = in ? ch.scale * __uint_as_float(v[q]) : 0.f;
             store32(dst + col, f, p.f16);
+            if (MODE == SHRINK_BWD && p.dz8) {
+              // the product with the saved integers has no rounding of its
+              // own: 16 bits of x_scale dZ in two bf16 numbers (the exponent
+              // of fp16 would not hold it), so dA is rounded once, at the end
+              const float sx = in ? p.x_scale[int64_t(it.t) * kTileRows + rt] : 0.f;
+              float lo[32];
+#pragma unroll
+              for (int q = 0; q < 32; ++q) {
+                const float w = in ? ch.scale * __uint_as_float(v[q]) * sx : 0.f;
+                f[q] = __bfloat162float(__float2bfloat16_rn(w));
+                lo[q] = w - f[q];
+              }
+              __nv_bfloat16* d8 = p.dz8 + (dst + col - p.out);
+              store32(d8, f, false);
+              store32(d8 + int64_t(p.plan.n_chunks) * kTileRows * 64, lo, false);
+            }
           }
         }
       } else {  // REDUCE
@@ -1905,6 +1925,8 @@ int tc_backward(const TcCall& a, cudaStream_t st) {
     prm.nk_main = (a.d_out + 63) / 64;
     set_ring(prm, kA1Bytes, max_nc(lo, hi) * kBox64);
     prm.out = reinterpret_cast<__nv_bfloat16*>(a.dzt);
+    prm.x_scale = a.x_scale;
+    prm.dz8 = reinterpret_cast<__nv_bfloat16*>(a.dz8);
     if ((s = launch1<SHRINK_BWD>(prm, st, a.max_ctas)) != MLORA_OK) return s;
     after_shrink = prm.n_items > 0;
   }

@@ -143,6 +143,8 @@ class Q8(ctypes.Structure):
         ("x_scale", ctypes.c_void_p),
         ("Gq", ctypes.c_void_p),
         ("g_scale", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_size_t),
     ]
 
 
@@ -186,6 +188,8 @@ SIGNATURES = {
                                              _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, ctypes.c_int32,
                                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _VP]),
     "mlora_q8_ld": (ctypes.c_int64, [ctypes.c_int64]),
+    "mlora_q8_scratch_bytes": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Routing),
+                                              ctypes.POINTER(ctypes.c_size_t)]),
     "mlora_q8_quantize": (ctypes.c_int, [_VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _VP,
                                          _VP, _VP, _VP]),
     "mlora_q8_dequantize": (ctypes.c_int, [_VP, _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _VP, _VP]),

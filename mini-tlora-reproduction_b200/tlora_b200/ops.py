@@ -593,6 +593,11 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     if st.base8 is not None or rows8 is not None:
         grad8 = _new_rows8(rows, d_out, dev) if st.base8 is not None and want_dx else None
         q8 = _q8_struct(st.base8, rows8, grad8)
+        if rows8 is not None and want_dA:
+            sb = ctypes.c_size_t(0)
+            _lib.call("mlora_q8_scratch_bytes", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(sb))
+            scratch = torch.empty(max(int(sb.value), 1), dtype=torch.uint8, device=dev)
+            q8.scratch, q8.scratch_bytes = scratch.data_ptr(), sb.value
         _lib.call("mlora_backward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8),
                   _ptr(dys), _ptr(xs), _ptr(W), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA),
                   _ptr(dB), _ptr(ws), wb, _stream(dev))
