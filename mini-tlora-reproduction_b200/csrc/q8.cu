@@ -9,6 +9,9 @@
 // of zeros has s = 0 and q = 0; a row that holds an infinity or a NaN has
 // s = NaN and q = 0, so that whatever is computed from the row is NaN, as it
 // would be from the row itself, and no other row is touched.
+#include <algorithm>
+#include <type_traits>
+
 #include "q8.cuh"
 
 namespace mlora {
@@ -19,7 +22,7 @@ namespace {
 // rounding wherever it decides (x and s have 24 bits and |r| is about s / 2
 // there, so r is a multiple of half an ulp of s that fits 24 bits; a larger
 // |r| may round, but not past s / 2).
-__device__ __forceinline__ int q8_exact(float x, float s) {
+__device__ __noinline__ int q8_exact(float x, float s) {
   const float q0 = rintf(__fdiv_rn(x, s));
   const float r = fmaf(-q0, s, x), r2 = r + r;
   int q = int(fminf(fmaxf(q0, -128.f), 128.f));
@@ -28,7 +31,8 @@ __device__ __forceinline__ int q8_exact(float x, float s) {
   return max(-127, min(127, q));  // s may have been rounded down where it is subnormal
 }
 
-template <class T> struct Vec8;  // eight elements as loaded
+// Eight elements of a row as loaded, their values and the magnitudes' maximum.
+template <class T> struct Vec8;
 template <> struct Vec8<float> {
   float4 a, b;
   __device__ __forceinline__ void get(float (&f)[8]) const {
@@ -59,13 +63,48 @@ template <> struct Vec8<__half> {
   }
 };
 
+// Running maximum of magnitudes, as float bits; a NaN stays (it is larger than
+// an infinity as bits).  16-bit elements two at a time.
+template <class T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair<__half> { using type = __half2; };
+template <class T> struct Top {
+  using P = typename Pair<T>::type;
+  uint32_t v = 0;
+  __device__ __forceinline__ void see(const Vec8<T>& x) {
+    const uint32_t w[4] = {x.a.x & 0x7fff7fffu, x.a.y & 0x7fff7fffu, x.a.z & 0x7fff7fffu, x.a.w & 0x7fff7fffu};
+    auto larger = [](uint32_t a, uint32_t b) {
+      const P m = __hmax2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    };
+    v = larger(v, larger(larger(w[0], w[1]), larger(w[2], w[3])));
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    const float lo = to_f(*reinterpret_cast<const T*>(&v)), hi = to_f(*(reinterpret_cast<const T*>(&v) + 1));
+    return max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu);
+  }
+};
+template <> struct Top<float> {
+  uint32_t v = 0;
+  __device__ __forceinline__ void see(const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v = max(v, __float_as_uint(f[i]) & 0x7fffffffu);
+  }
+  __device__ __forceinline__ void see(const Vec8<float>& x) {
+    float f[8];
+    x.get(f);
+    see(f);
+  }
+  __device__ __forceinline__ uint32_t bits() const { return v; }
+};
+
 // eight elements from column c of a row; past `cols` they are zero
 template <class T, bool VEC>
 __device__ __forceinline__ Vec8<T> load8(const T* row, int64_t c, int64_t cols) {
   Vec8<T> v;
   if constexpr (VEC) {
-    if (c < cols) return *reinterpret_cast<const Vec8<T>*>(row + c);
     memset(&v, 0, sizeof(v));
+    if (c < cols) v = *reinterpret_cast<const Vec8<T>*>(row + c);
   } else {
     T e[8];
 #pragma unroll
@@ -75,32 +114,68 @@ __device__ __forceinline__ Vec8<T> load8(const T* row, int64_t c, int64_t cols) 
   return v;
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void values8(const Vec8<T>& v, const float* col_scale, int64_t c, int64_t cols,
-                                        float (&f)[8]) {
-  v.get(f);
-  if (!col_scale) return;
+// f *= col_scale[c ..] (fp32, one rounding)
+template <bool VEC>
+__device__ __forceinline__ void scale8(float (&f)[8], const float* col_scale, int64_t c, int64_t cols) {
+  if constexpr (VEC) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (c < cols) {
+      a = __ldg(reinterpret_cast<const float4*>(col_scale + c));
+      b = __ldg(reinterpret_cast<const float4*>(col_scale + c) + 1);
+    }
+    f[0] *= a.x; f[1] *= a.y; f[2] *= a.z; f[3] *= a.w;
+    f[4] *= b.x; f[5] *= b.y; f[6] *= b.z; f[7] *= b.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c + i < cols) f[i] *= __ldg(col_scale + c + i);
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) f[i] *= __ldg(col_scale + c + i);
+  }
 }
 
-// The 8-bit row of eight values: bits of t + 1.5 2^23 hold the integer
-// nearest t = x (1 / s), whose error is below 127 2^-22; a t within 1e-4 of a
-// border is decided exactly (one value in ten thousand).
-__device__ __forceinline__ uint2 round8(const float (&f)[8], float s, float inv, bool plain) {
+// How the quotients of a row are rounded.  The low bits of x r + 1.5 2^23 (one
+// fma) hold the integer nearest x r.
+//
+// kOne: r = `above` is a reciprocal of s moved by 2^-21, and that one product
+// decides.  For 16-bit x and a scale that is their maximum over 127: with
+// 11-bit (or 8-bit) significands m1 of x and m2 of the maximum, 127 x / max =
+// 127 m1 2^-e / m2 is either a border k + 1/2 or at least a relative
+// 1 / (254 m1) > 2^-19 away from it, more than the move and the roundings of s
+// and r (2^-21 + 2^-23) bridge.  It is a border only at |x| = max / 2, unless
+// 127 divides m2, which makes s exact (such rows are kTwo); there the
+// rounding of s decides, and r is moved the way that s was rounded.
+//
+// kTwo: reciprocals moved by 2^-20 down and up enclose the quotient; where both
+// give one integer it is the quotient's, else the sign of x - (n + 1/2) s, which
+// one fma has exactly, decides between n and n + 1.
+//
+// kSlow: s is so small that its reciprocal is not accurate, or 0 or NaN.
+enum Rounding { kOne, kTwo, kSlow };
+struct RowScale {
+  float s, below, above;
+  Rounding how;
+};
+
+__device__ __forceinline__ uint2 round8(const float (&f)[8], const RowScale& r) {
   constexpr float kMagic = 12582912.f;
-  int q[8];
-  float far = 0.f;
+  uint32_t q[8], differ = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = f[i] * inv, m = t + kMagic;
-    q[i] = __float_as_int(m);
-    far = fmaxf(far, fabsf(t - (m - kMagic)));
-  }
-  if (!plain || far > 0.4999f) {
+  for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fmaf(f[i], r.above, kMagic));
+  if (r.how != kOne) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = s > 0.f ? q8_exact(f[i], s) : 0;
+    for (int i = 0; i < 8; ++i) differ |= q[i] ^ __float_as_uint(fmaf(f[i], r.below, kMagic));
+    if (r.how == kSlow) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = r.s > 0.f ? uint32_t(q8_exact(f[i], r.s)) : 0u;
+    } else if (differ) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float n = fminf(fmaf(f[i], r.above, kMagic), fmaf(f[i], r.below, kMagic)) - kMagic;
+        const float d = fmaf(-(n + 0.5f), r.s, f[i]);
+        const uint32_t u = __float_as_uint(n + kMagic);
+        if (q[i] != __float_as_uint(fmaf(f[i], r.below, kMagic)))
+          q[i] = u + (d > 0.f || (d == 0.f && (u & 1u)) ? 1u : 0u);
+      }
+    }
   }
   uint2 w;
   w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
@@ -108,92 +183,137 @@ __device__ __forceinline__ uint2 round8(const float (&f)[8], float s, float inv,
   return w;
 }
 
-constexpr int kQT = 256;  // threads of a quantizer block
-
-// Scale of a row from its largest magnitude (as float bits); `plain`: the
-// reciprocal route of round8 holds (1 / s is finite and accurate).
-__device__ __forceinline__ float row_scale(uint32_t top, bool* plain) {
+// Scale of a row from its largest magnitude (as float bits); SHORT: the row's
+// values have 16-bit significands' precision (see kOne).
+template <bool SHORT>
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+  RowScale r;
   if (top >= 0x7f800000u) {  // an infinity or a NaN in the row
-    *plain = false;
-    return __int_as_float(0x7fc00000);
+    r.s = __int_as_float(0x7fc00000);
+    r.below = r.above = 0.f;
+    r.how = kSlow;
+    return r;
   }
-  const float s = __fdiv_rn(__uint_as_float(top), 127.f);
-  *plain = s > 1e-30f;
-  return s;
+  r.s = __fdiv_rn(__uint_as_float(top), 127.f);
+  const float inv = 1.f / r.s;
+  r.how = r.s > 1e-30f ? kTwo : kSlow;
+  r.below = inv * (1.f - 0x1p-20f);
+  r.above = inv * (1.f + 0x1p-20f);
+  if (SHORT && r.how == kTwo) {
+    const float left = fmaf(-127.f, r.s, __uint_as_float(top));  // > 0: s was rounded down
+    if (left != 0.f) {
+      r.above = inv * (left > 0.f ? 1.f + 0x1p-21f : 1.f - 0x1p-21f);
+      r.how = kOne;
+    }
+  }
+  return r;
 }
 
-// `tpr` threads (a power of two, 32..256) per row, kQT / tpr rows per block,
-// thread t of a row takes columns 8 t + 8 tpr v.  NV > 0: the row is held in
-// registers between the maximum and the rounding; NV = 0: it is read twice.
-template <class T, bool VEC, int NV>
-__global__ void __launch_bounds__(kQT) k_quantize(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t ld,
+// 2^sh threads (32..512) per row, several rows per block; thread t of a row
+// takes the 8-column groups t, t + 2^sh, ...  NV > 0: the row (CS: its products
+// with the column scales) is held in registers between the maximum and the
+// rounding, so it is read once; NV = 0: twice.  Bound by HBM, 2 bytes in and 1
+// out per 16-bit element, if the work around each row is spread over enough
+// elements of a thread: NV up to 16 (8 with column scales).
+template <class T, bool VEC, bool CS, int NV>
+__global__ void __launch_bounds__(512) k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
                                                    const float* __restrict__ col_scale, int8_t* __restrict__ q,
-                                                   float* __restrict__ scale, int tpr) {
-  __shared__ uint32_t part[kQT / 32];
-  const int t = threadIdx.x % tpr, rb = threadIdx.x / tpr;
-  const int64_t row = int64_t(blockIdx.x) * (kQT / tpr) + rb;
+                                                   float* __restrict__ scale, int sh) {
+  using Held = typename std::conditional<CS, Vec8<float>, Vec8<T>>::type;
+  using HeldT = typename std::conditional<CS, float, T>::type;
+  __shared__ uint32_t part[16];
+  const int tpr = 1 << sh, t = threadIdx.x & (tpr - 1);
+  const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> sh;
   const bool live = row < rows;
   const T* x = src + (live ? row : 0) * ld;
-  const int64_t ldq = q8_ld(cols), step = int64_t(tpr) * 8;
-  Vec8<T> v[NV > 0 ? NV : 1];
-  uint32_t top = 0;
-  auto widen = [&](const Vec8<T>& u, int64_t c) {
-    float f[8];
-    values8<T, VEC>(u, col_scale, c, cols, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  const int ldq = int(q8_ld(cols)), step = tpr * 8;
+  const int end = live ? cols : 0;
+  auto product = [&](const Vec8<T>& u, int c) -> Held {
+    if constexpr (CS) {
+      float f[8];
+      u.get(f);
+      scale8<VEC>(f, col_scale, c, end);
+      Held h;
+      h.a = make_float4(f[0], f[1], f[2], f[3]);
+      h.b = make_float4(f[4], f[5], f[6], f[7]);
+      return h;
+    } else {
+      return u;
+    }
   };
+  Held v[NV > 0 ? NV : 1];
+  Top<HeldT> most;
   if (NV > 0) {
+    Vec8<T> u[NV > 0 ? NV : 1];  // all loads first: they are in flight together
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load8<T, VEC>(x, live ? t * 8 + i * step : cols, cols);
+    for (int i = 0; i < NV; ++i) u[i] = load8<T, VEC>(x, t * 8 + i * step, end);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) widen(v[i], t * 8 + i * step);
-  } else if (live) {
-    for (int64_t c = t * 8; c < cols; c += step) widen(load8<T, VEC>(x, c, cols), c);
+    for (int i = 0; i < NV; ++i) v[i] = product(u[i], t * 8 + i * step);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) most.see(v[i]);
+  } else {
+    for (int c = t * 8; c < end; c += step) most.see(product(load8<T, VEC>(x, c, end), c));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (tpr > 32) {
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
+  uint32_t top = __reduce_max_sync(0xffffffffu, most.bits());
+  if (sh > 5) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) part[warp] = top;
     __syncthreads();
-    const int w0 = rb * (tpr / 32);
-    for (int w = 0; w < tpr / 32; ++w) top = max(top, part[w0 + w]);
+    // the warps of this row: 2^(sh - 5) aligned entries
+    const int nw = 1 << (sh - 5);
+    top = __reduce_max_sync(0xffffffffu, part[(warp & ~(nw - 1)) + (lane & (nw - 1))]);
   }
   if (!live) return;
-  bool plain;
-  const float s = row_scale(top, &plain);
-  const float inv = 1.f / s;
-  if (t == 0) scale[row] = s;
+  const RowScale r = row_scale<!CS && sizeof(T) == 2>(top);
+  if (t == 0) scale[row] = r.s;
   int8_t* out = q + row * ldq;
-  auto emit = [&](const Vec8<T>& u, int64_t c) {
+  auto emit = [&](const Held& u, int c) {
     float f[8];
-    values8<T, VEC>(u, col_scale, c, cols, f);
-    *reinterpret_cast<uint2*>(out + c) = round8(f, s, inv, plain);
+    u.get(f);
+    *reinterpret_cast<uint2*>(out + c) = round8(f, r);
   };
   if (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (t * 8 + i * step < ldq) emit(v[i], t * 8 + i * step);
   } else {
-    for (int64_t c = t * 8; c < ldq; c += step) emit(load8<T, VEC>(x, c, cols), c);
+    for (int c = t * 8; c < ldq; c += step) emit(product(load8<T, VEC>(x, c, end), c), c);
   }
 }
 
-template <class T, bool VEC>
+// Launch shape of a row kernel over `groups` column groups: the fewest threads
+// per row (2^sh) that leave a thread at most `most` groups, and, where the rows
+// alone do not fill the SMs, as many as shorten a row's time.
+struct RowGrid {
+  int sh, block, nv;
+  unsigned grid;
+};
+RowGrid row_grid(int64_t rows, int64_t groups, int most) {
+  RowGrid g;
+  g.sh = 5;
+  while (g.sh < 9 && groups > (int64_t(most) << g.sh)) ++g.sh;
+  while (g.sh < 9 && groups > (int64_t(1) << g.sh) && (rows << g.sh) < 148 * 1024) ++g.sh;
+  g.block = std::max(1 << g.sh, 128);
+  g.nv = int((groups + (int64_t(1) << g.sh) - 1) >> g.sh);
+  g.grid = unsigned(((rows << g.sh) + g.block - 1) / g.block);
+  return g;
+}
+
+template <class T, bool VEC, bool CS>
 int launch_quantize(const T* src, int64_t rows, int64_t cols, int64_t ld, const float* cs, int8_t* q, float* scale,
                     cudaStream_t st) {
-  // about four 8-element groups per thread: enough 16-byte loads in flight,
-  // few enough registers for full occupancy
   const int64_t groups = q8_ld(cols) / 8;  // the zero bytes past `cols` included
-  int tpr = 32;
-  while (tpr < kQT && groups > 4 * tpr) tpr *= 2;
-  const int64_t per = kQT / tpr, nv = (groups + tpr - 1) / tpr;
-  const unsigned grid = unsigned((rows + per - 1) / per);
-#define MLORA_QUANT(NV) k_quantize<T, VEC, NV><<<grid, kQT, 0, st>>>(src, rows, cols, ld, cs, q, scale, tpr)
-  if (nv <= 1) MLORA_QUANT(1);
-  else if (nv <= 2) MLORA_QUANT(2);
-  else if (nv <= 4) MLORA_QUANT(4);
-  else if (nv <= 8) MLORA_QUANT(8);
+  constexpr bool kWide = CS || sizeof(T) == 4;  // held as float32
+  const RowGrid g = row_grid(rows, groups, kWide ? 8 : 16);
+#define MLORA_QUANT(NV) \
+  k_quantize<T, VEC, CS, NV><<<g.grid, g.block, 0, st>>>(src, rows, int(cols), ld, cs, q, scale, g.sh)
+  if (g.nv <= 1) MLORA_QUANT(1);
+  else if (g.nv <= 2) MLORA_QUANT(2);
+  else if (g.nv <= 4) MLORA_QUANT(4);
+  else if (g.nv <= 6) MLORA_QUANT(6);
+  else if (g.nv <= 8) MLORA_QUANT(8);
+  else if (!kWide && g.nv <= 12) MLORA_QUANT((kWide ? 0 : 12));
+  else if (!kWide && g.nv <= 16) MLORA_QUANT((kWide ? 0 : 16));
   else MLORA_QUANT(0);
 #undef MLORA_QUANT
   count_launch();
@@ -205,51 +325,63 @@ int quantize_t(const void* src, int64_t rows, int64_t cols, int64_t ld, const fl
                cudaStream_t st) {
   const T* x = static_cast<const T*>(src);
   // 16-byte loads: aligned rows of whole 8-element groups
-  const bool vec = aligned(src, 16) && cols % 8 == 0 && (ld * int64_t(sizeof(T))) % 16 == 0;
-  return vec ? launch_quantize<T, true>(x, rows, cols, ld, cs, q, scale, st)
-             : launch_quantize<T, false>(x, rows, cols, ld, cs, q, scale, st);
+  const bool vec = aligned(src, 16) && cols % 8 == 0 && (ld * int64_t(sizeof(T))) % 16 == 0 && aligned(cs, 16);
+  if (cs)
+    return vec ? launch_quantize<T, true, true>(x, rows, cols, ld, cs, q, scale, st)
+               : launch_quantize<T, false, true>(x, rows, cols, ld, cs, q, scale, st);
+  return vec ? launch_quantize<T, true, false>(x, rows, cols, ld, cs, q, scale, st)
+             : launch_quantize<T, false, false>(x, rows, cols, ld, cs, q, scale, st);
 }
 
 // dst[i, k] = T(s[i] q[i, k]): one fp32 product, rounded once.  127 s of a row
 // whose largest magnitude is that of float32 can round past it: a finite scale
-// gives finite values.  A block takes 8-column groups of consecutive rows.
+// gives finite float32 values.  Thread t of a row takes the groups t, t + 2^sh,
+// ... of 16 bytes of the output (4 or 8 columns); rows of any width (VEC
+// false) go element by element, neighbouring threads on neighbouring columns.
+template <class T>
+__device__ __forceinline__ T q8_value(int q, float s) {
+  float v = float(q) * s;
+  if (std::is_same<T, float>::value && isinf(v) && isfinite(s)) v = copysignf(3.402823466e38f, v);
+  return from_f<T>(v);
+}
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) k_dequantize(const int8_t* __restrict__ q, const float* __restrict__ scale,
-                                                     int64_t rows, int64_t cols, T* __restrict__ dst) {
-  const int64_t groups = (cols + 7) / 8, ldq = q8_ld(cols), n = rows * groups;
-  const int64_t stride = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += stride) {
-    const int64_t row = e / groups, c = (e - row * groups) * 8;
-    const uint2 w = *reinterpret_cast<const uint2*>(q + row * ldq + c);
-    const float s = __ldg(scale + row);
-    const float lim = isfinite(s) ? 3.402823466e38f : __int_as_float(0x7fc00000);  // NaN: no limit
-    T o[8];
+__global__ void __launch_bounds__(512) k_dequantize(const int8_t* __restrict__ q, const float* __restrict__ scale,
+                                                     int64_t rows, int cols, T* __restrict__ dst, int sh) {
+  constexpr int PER = VEC ? 16 / int(sizeof(T)) : 1;
+  const int tpr = 1 << sh, t = threadIdx.x & (tpr - 1);
+  const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> sh;
+  if (row >= rows) return;
+  const float s = __ldg(scale + row);
+  const int8_t* in = q + row * q8_ld(cols);
+  T* out = dst + row * cols;
+#pragma unroll 4
+  for (int c = t * PER; c < cols; c += tpr * PER) {
+    if constexpr (VEC) {
+      alignas(16) T o[PER];
+      uint32_t w[2];
+      if constexpr (PER == 8) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(in + c));
+        w[0] = u.x; w[1] = u.y;
+      } else {
+        w[0] = __ldg(reinterpret_cast<const uint32_t*>(in + c));
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = (i < 4 ? w.x : w.y) >> (8 * (i % 4));
-      const float v = float(int8_t(u & 0xff)) * s;
-      o[i] = from_f<T>(isinf(v) ? copysignf(lim, v) : v);
-    }
-    T* d = dst + row * cols + c;
-    if (VEC) {
-      memcpy(__builtin_assume_aligned(d, 16), o, sizeof(o));
+      for (int i = 0; i < PER; ++i) o[i] = q8_value<T>(int8_t((w[i / 4] >> (8 * (i % 4))) & 0xff), s);
+      *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(o);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < cols) d[i] = o[i];
+      out[c] = q8_value<T>(in[c], s);
     }
   }
 }
 
 template <class T>
 int dequantize_t(const int8_t* q, const float* scale, int64_t rows, int64_t cols, void* dst, cudaStream_t st) {
-  const int64_t n = rows * ((cols + 7) / 8);
-  const int64_t blocks = (n + 255) / 256;
-  const unsigned grid = unsigned(blocks < 65536 * 8 ? blocks : 65536 * 8);
-  if (aligned(dst, 16) && cols % 8 == 0)
-    k_dequantize<T, true><<<grid, 256, 0, st>>>(q, scale, rows, cols, static_cast<T*>(dst));
+  const bool vec = aligned(dst, 16) && cols % 8 == 0;
+  const RowGrid g = row_grid(rows, vec ? cols * int64_t(sizeof(T)) / 16 : cols, 4);
+  if (vec)
+    k_dequantize<T, true><<<g.grid, g.block, 0, st>>>(q, scale, rows, int(cols), static_cast<T*>(dst), g.sh);
   else
-    k_dequantize<T, false><<<grid, 256, 0, st>>>(q, scale, rows, cols, static_cast<T*>(dst));
+    k_dequantize<T, false><<<g.grid, g.block, 0, st>>>(q, scale, rows, int(cols), static_cast<T*>(dst), g.sh);
   count_launch();
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
