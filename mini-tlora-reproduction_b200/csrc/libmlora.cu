@@ -8,6 +8,7 @@
 #include "route.cu"
 #include "tc.cu"
 #include "q8_tc.cu"
+#include "q8_small.cu"
 #include "allreduce.cu"
 #include "multimem.cu"
 #include "api.cu"

@@ -219,6 +219,7 @@ template <class T, bool VEC, bool CS, int NV>
 __global__ void __launch_bounds__(512) k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
                                                    const float* __restrict__ col_scale, int8_t* __restrict__ q,
                                                    float* __restrict__ scale, int sh) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product after it may start
   using Held = typename std::conditional<CS, Vec8<float>, Vec8<T>>::type;
   using HeldT = typename std::conditional<CS, float, T>::type;
   __shared__ uint32_t part[16];
@@ -278,6 +279,26 @@ __global__ void __launch_bounds__(512) k_quantize(const T* __restrict__ src, int
       if (t * 8 + i * step < ldq) emit(v[i], t * 8 + i * step);
   } else {
     for (int c = t * 8; c < ldq; c += step) emit(product(load8<T, VEC>(x, c, end), c), c);
+  }
+}
+
+// One row by a block of 256 threads, read twice (it is small and stays in L1):
+// 16-byte aligned, cols a multiple of 8.
+template <class T>
+__device__ void quantize_row(const T* x, int cols, int8_t* out, float* scale) {
+  __shared__ uint32_t part[8];
+  const int ldq = int(q8_ld(cols)), t = threadIdx.x;
+  Top<T> most;
+  for (int c = t * 8; c < cols; c += 2048) most.see(load8<T, true>(x, c, cols));
+  const uint32_t w = __reduce_max_sync(0xffffffffu, most.bits());
+  if (t % 32 == 0) part[t / 32] = w;
+  __syncthreads();
+  const RowScale r = row_scale<true>(__reduce_max_sync(0xffffffffu, part[t & 7]));
+  if (t == 0) *scale = r.s;
+  for (int c = t * 8; c < ldq; c += 2048) {
+    float f[8];
+    load8<T, true>(x, c, cols).get(f);
+    *reinterpret_cast<uint2*>(out + c) = round8(f, r);
   }
 }
 

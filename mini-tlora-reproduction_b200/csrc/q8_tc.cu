@@ -180,16 +180,24 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
     orow = -1;
   }
   if (p.dtype == MLORA_F32) {
-    if (orow < 0) return;
-    float* dst = static_cast<float*>(p.out) + orow * p.N + n;
-    if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    // through shared memory (the warp's whole 4 KB): a warp writes 128
+    // neighbouring bytes of one row at a time, at any alignment
+    const uint32_t base = buf & ~4095u;
+    __syncwarp();
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        reinterpret_cast<float4*>(dst)[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
-    } else {
-#pragma unroll
-      for (int q = 0; q < 32; ++q)
-        if (n + q < p.N) dst[q] = f[q];
+    for (int q = 0; q < 8; ++q)
+      sts128(base + uint32_t(lane) * 128u + ((uint32_t(q) ^ (uint32_t(lane) & 7u)) << 4), __float_as_uint(f[4 * q]),
+             __float_as_uint(f[4 * q + 1]), __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3]));
+    __syncwarp();
+    float* out = static_cast<float*>(p.out);
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      const int64_t o = __shfl_sync(0xffffffffu, orow, r);
+      const uint32_t a =
+          base + uint32_t(r) * 128u + (((uint32_t(lane) >> 2) ^ (uint32_t(r) & 7u)) << 4) + (uint32_t(lane) & 3u) * 4u;
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+      if (o >= 0 && n + lane < p.N) out[o * p.N + n + lane] = v;
     }
     return;
   }
@@ -208,6 +216,7 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
            pack2(f[8 * q + 2], f[8 * q + 3], f16), pack2(f[8 * q + 4], f[8 * q + 5], f16),
            pack2(f[8 * q + 6], f[8 * q + 7], f16));
   __syncwarp();
+#pragma unroll 8
   for (int r = 0; r < 32; ++r) {
     const int64_t o = __shfl_sync(0xffffffffu, orow, r);
     const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
