@@ -128,11 +128,10 @@ int check_q8(std::initializer_list<const void*> mats, std::initializer_list<cons
 
 // One 8-bit product: a few rows by streaming the weight, more on the tensor
 // cores, whatever their size, unless the call asks for the CUDA cores.
-// `after_rows`: the launch before it made the 8-bit rows.
-int q8_main(const Q8Main& a, int impl, bool after_rows, cudaStream_t st) {
-  if (impl != MLORA_IMPL_SIMT && q8_few_ok(a)) return q8_main_few(a, after_rows, st);
+int q8_main(const Q8Main& a, int impl, Q8After after, cudaStream_t st) {
+  if (impl != MLORA_IMPL_SIMT && q8_few_ok(a)) return q8_main_few(a, after, st);
   const bool tc = impl != MLORA_IMPL_SIMT && q8_tc_ok(a);
-  return tc ? q8_main_tc(a, st) : q8_main_simt(a, st);
+  return tc ? q8_main_tc(a, after, st) : q8_main_simt(a, st);
 }
 
 }  // namespace
@@ -186,7 +185,7 @@ int q8_impl(const mlora_problem* prob, int impl) {
 // The 8-bit backbone product of mlora_forward_q8, with the LoRA expand of the
 // intermediate that the shrink before it left in zsave.
 int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8, const PlanDev& dev,
-                    int impl, bool after_rows, const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
+                    int impl, Q8After after, const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
                     cudaStream_t s) {
   Q8Main m;
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
@@ -197,7 +196,7 @@ int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const
   m.plan = dev; m.zt = zsave; m.pack = B_pack;
   m.max_ctas = prob->max_ctas;
   m.err = prob->err_word;
-  return q8_main(m, impl, after_rows, s);
+  return q8_main(m, impl, after, s);
 }
 
 // mlora_forward_staged, or with `ar` mlora_forward_push (MAIN pushes the
@@ -235,12 +234,12 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   // a few rows in 16 bits: rows and shrink in one launch
   const bool few = q8_base && impl == MLORA_IMPL_TC && prob->rows <= kQ8Few && dev.n_chunks > 0 &&
                    (stages & MLORA_STAGE_SHRINK);
-  // the 8-bit product directly follows the launch that made its rows
-  const bool rows_last = few || dev.n_chunks == 0;
+  // the launch that the 8-bit product follows
+  const Q8After after = few || dev.n_chunks == 0 ? kAfterRows : impl == MLORA_IMPL_TC ? kAfterShrink : kAfterOther;
   if (few) {
     st = q8_few_prep(X, prob->rows, prob->d_in, prob->dtype, q8->Xq, q8->x_scale, dev, A_pack, zsave, s);
     if (st != MLORA_OK) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), rows_last, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
   }
   if (q8 && q8->Xq) {  // operand of the 8-bit product, the saved form of X, or both
     st = q8_quantize(X, prob->rows, prob->d_in, prob->d_in, prob->dtype, nullptr, (int8_t*)q8->Xq,
@@ -266,7 +265,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     st = tc_forward(a, s);
     if (st != MLORA_OK || !q8_base) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), rows_last, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
   }
   SimtCall a;
   a.plan = dev;
@@ -281,7 +280,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   a.c_end = p.tile_chunk_begin[tile_end];
   st = simt_forward(a, s);
   if (st != MLORA_OK || !q8_base) return st;
-  return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), rows_last, bias, B_pack, Y, zsave, all_stages, s);
+  return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
 }
 
 }  // namespace
@@ -410,7 +409,7 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     m.plan = dev; m.zt = dzsave; m.pack = A_pack;
     m.max_ctas = prob->max_ctas;
     m.err = prob->err_word;
-    st = q8_main(m, q8_impl(prob, impl), false, s);
+    st = q8_main(m, q8_impl(prob, impl), kAfterRows, s);
     if (st != MLORA_OK) return st;
   }
   if (!saved8)
@@ -602,7 +601,7 @@ extern "C" int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
   m.Aq = Xq; m.a_scale = x_scale; m.Wq = Wq; m.w_scale = w_scale; m.bias = bias; m.out = Y;
   m.max_ctas = prob->max_ctas; m.err = prob->err_word;
-  return q8_main(m, prob->impl, X != nullptr, s);
+  return q8_main(m, prob->impl, X ? kAfterRows : kAfterOther, s);
 }
 
 extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale,
@@ -621,7 +620,7 @@ extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.dtype = prob->dtype;
   m.Aq = Gq; m.a_scale = g_scale; m.Wq = Wq; m.out = dX;
   m.max_ctas = prob->max_ctas; m.err = prob->err_word;
-  return q8_main(m, prob->impl, false, s);
+  return q8_main(m, prob->impl, kAfterRows, s);
 }
 
 extern "C" int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,

@@ -66,16 +66,20 @@ inline size_t q8_scratch_bytes(const Plan& p) {
 }
 int q8_da_tc(const Q8Saved& a, cudaStream_t st);
 
-// The forward of at most kQ8Few rows; `after_rows`: the launch before it on the
-// stream is the one that made the 8-bit rows (and allows an early start).
+// What the launch before an 8-bit product on its stream was: the one that made
+// the 8-bit rows, or the shrink that made the low-rank blocks (then the rows
+// are older), which both allow the product to start early; or another.
+enum Q8After { kAfterOther, kAfterRows, kAfterShrink };
+
+// The forward of at most kQ8Few rows.
 constexpr int kQ8Few = 16;
 bool q8_few_ok(const Q8Main& a);
-int q8_main_few(const Q8Main& a, bool after_rows, cudaStream_t st);
+int q8_main_few(const Q8Main& a, Q8After after, cudaStream_t st);
 int q8_few_prep(const void* X, int64_t rows, int d_in, int dtype, int8_t* Xq, float* x_scale, const PlanDev& plan,
                 const void* A_pack, void* zt, cudaStream_t st);
 
 int q8_main_simt(const Q8Main& a, cudaStream_t st);
 bool q8_tc_ok(const Q8Main& a);
-int q8_main_tc(const Q8Main& a, cudaStream_t st);
+int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st);
 
 }  // namespace mlora

@@ -268,7 +268,7 @@ cudaError_t launch_few(K kern, unsigned grid, cudaStream_t st, bool pdl, const P
 }
 
 template <class T>
-int launch_q8_few(const Q8Main& a, bool after_rows, cudaStream_t st) {
+int launch_q8_few(const Q8Main& a, Q8After after, cudaStream_t st) {
   FewParams p;
   memset(&p, 0, sizeof(p));
   p.rows = int(a.M); p.d_in = a.d_in; p.d_out = a.d_out; p.R = a.R;
@@ -277,7 +277,7 @@ int launch_q8_few(const Q8Main& a, bool after_rows, cudaStream_t st) {
   p.expand = a.expand ? 1 : 0;
   if (a.expand) p.plan = a.plan;
   p.zt = a.zt; p.pack = a.pack; p.err = a.err;
-  p.pdl = after_rows && pdl_enabled() ? 1 : 0;
+  p.pdl = after != kAfterOther && pdl_enabled() ? 1 : 0;
   const unsigned grid = unsigned((a.d_out + kFewCh - 1) / kFewCh);
   if (a.M <= 8) MLORA_CUDA_TRY(launch_few(k_q8_few<T, 1>, grid, st, p.pdl != 0, p));
   else MLORA_CUDA_TRY(launch_few(k_q8_few<T, 2>, grid, st, p.pdl != 0, p));
@@ -295,11 +295,11 @@ bool q8_few_ok(const Q8Main& a) {
          (!a.expand || (aligned(a.zt, 16) && aligned(a.pack, 16)));  // 16-byte loads of the expand
 }
 
-int q8_main_few(const Q8Main& a, bool after_rows, cudaStream_t st) {
+int q8_main_few(const Q8Main& a, Q8After after, cudaStream_t st) {
   if (a.M == 0) return MLORA_OK;
-  if (a.dtype == MLORA_BF16) return launch_q8_few<__nv_bfloat16>(a, after_rows, st);
-  if (a.dtype == MLORA_F16) return launch_q8_few<__half>(a, after_rows, st);
-  return launch_q8_few<float>(a, after_rows, st);
+  if (a.dtype == MLORA_BF16) return launch_q8_few<__nv_bfloat16>(a, after, st);
+  if (a.dtype == MLORA_F16) return launch_q8_few<__half>(a, after, st);
+  return launch_q8_few<float>(a, after, st);
 }
 
 // Rows in 8 bits and the low-rank intermediate of a few rows in one launch

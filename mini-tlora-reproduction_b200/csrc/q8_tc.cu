@@ -33,7 +33,8 @@ constexpr int kDefer = 8;       // k-blocks of the next tile before a tile's exp
 constexpr int kQ8K = 128;       // bytes of K per k-block
 constexpr int kQ8Stages = 6;    // 32 KB per CTA each
 constexpr int kQ8StageBytes = 32 * 1024;
-constexpr int kQ8Smem = kQ8Stages * kQ8StageBytes + kStageOut2Bytes + 1024 + 512;
+constexpr int kQ8ColBytes = 4 * 2 * 256 * 4;  // column scales and biases of a tile, per epilogue warp
+constexpr int kQ8Smem = kQ8Stages * kQ8StageBytes + kStageOut2Bytes + kQ8ColBytes + 1024 + 512;
 static_assert(kQ8Smem <= 232448, "dynamic shared memory above 227 KB");
 
 struct Q8Params {
@@ -47,6 +48,8 @@ struct Q8Params {
   int nk;              // 128-byte k-blocks of the integer product
   int expand;
   int dtype;
+  int pdl_rows, pdl_z;  // launched to overlap the kernel before it, which makes the 8-bit rows / the
+                        // low-rank blocks: wait for it before reading them
   int tma_out;         // 16-bit output rows that TMA can describe, in place
   const float* a_scale;
   const float* w_scale;  // forward
@@ -114,41 +117,16 @@ __device__ __forceinline__ Q8Item q8_item(const Q8Params& p, int i) {
   return it;
 }
 
-// 32 fp32 values of columns n0.. of N: multiplied / added elementwise
-template <bool VECTOR_OK = true>
-__device__ __forceinline__ void q8_scale_cols(float (&f)[32], const float* s, int n, int N) {
-  if (n + 32 <= N && VECTOR_OK) {
-    const bool a16 = (reinterpret_cast<uintptr_t>(s + n) & 15) == 0;
-    if (a16) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(s + n) + q);
-        f[4 * q] *= v.x; f[4 * q + 1] *= v.y; f[4 * q + 2] *= v.z; f[4 * q + 3] *= v.w;
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < 32; ++q)
-    if (n + q < N) f[q] *= __ldg(s + n + q);
+// bias[n] of an output of type `dtype`
+__device__ __forceinline__ float q8_bias(const Q8Params& p, int n) {
+  if (p.dtype == MLORA_BF16) return to_f(static_cast<const __nv_bfloat16*>(p.bias)[n]);
+  if (p.dtype == MLORA_F16) return to_f(static_cast<const __half*>(p.bias)[n]);
+  return static_cast<const float*>(p.bias)[n];
 }
-
-template <class T>
-__device__ __forceinline__ void q8_add_bias(float (&f)[32], const T* b, int n, int N) {
-  if (n + 32 <= N && (reinterpret_cast<uintptr_t>(b + n) & 15) == 0) {
-    constexpr int PER = 16 / int(sizeof(T));
-#pragma unroll
-    for (int q = 0; q < 32 / PER; ++q) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + n) + q);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int k = 0; k < PER; ++k) f[q * PER + k] += to_f(e[k]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int q = 0; q < 32; ++q)
-    if (n + q < N) f[q] += to_f(b[n + q]);
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
 }
 
 // One 32 x 32 slice of finished values (lane = row row_w0 + lane, columns n..)
@@ -232,7 +210,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage_out = smem + kQ8Stages * kQ8StageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kStageOut2Bytes);
+  float* cols = reinterpret_cast<float*>(stage_out + kStageOut2Bytes);  // [4][scales 256, biases 256]
+  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kStageOut2Bytes + kQ8ColBytes);
   uint64_t* empty = full + kQ8Stages;
   uint64_t* ifull = empty + kQ8Stages;  // [2] integer sums of the accumulator complete
   uint64_t* conv = ifull + 2;           // [2] rewritten as fp32 in both CTAs (used in the even CTA)
@@ -297,7 +276,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
       if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
       return s;
     };
+    bool rows_ready = !p.pdl_rows, z_ready = !p.pdl_z;
     auto expand = [&](const Q8Item& it) {
+      if (it.nc > 0 && !z_ready) {
+        grid_dep_wait();
+        z_ready = true;
+      }
       for (int i = 0; i < it.nc && ok; ++i) {
         const int s = claim();
         if (s < 0) continue;
@@ -328,14 +312,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
         uint8_t* sA = smem + s * kQ8StageBytes;
         uint8_t* sB = sA + kA2Bytes;
         const uint32_t bar = mapa(su32(&full[s]), 0);
-        tma_load_pair(sA, &p.mA, bar, kb * kQ8K, row0, pol_norm);
         if (!BWD) tma_load_pair(sB, &p.mB, bar, kb * kQ8K, nh, pol_keep);
         else tma_load_pair(sB, &p.mB, bar, nh, kb * kQ8K, pol_keep);
+        if (!rows_ready) {
+          grid_dep_wait();
+          rows_ready = true;
+        }
+        tma_load_pair(sA, &p.mA, bar, kb * kQ8K, row0, pol_norm);
       }
       if (ok && defer == p.nk) expand(last);
       last = it;
     }
     if (ok) expand(last);
+    if (!rows_ready || !z_ready) grid_dep_wait();  // never finish before the kernel this launch overlaps
     if (!ok && leader) {
       // let copies already in flight land before the CTAs exit
       const unsigned long long t0 = now_ns();
@@ -425,8 +414,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
     int acc = 0;
     uint32_t acc_phase = 0;
     uint32_t x_phase[2] = {0, 0};
+    if (p.pdl_rows) grid_dep_wait();  // the row scales are that kernel's
     for (int item = pair; item < p.n_items; item += n_pairs) {
       const Q8Item it = q8_item(p, item);
+      // the tile's column scales and biases, fetched while its sums are formed
+      // (a copy per warp: no warp waits for another)
+      float* cs = cols + (warp - 2) * 512;
+      if (!BWD) {
+        __syncwarp();
+#pragma unroll
+        for (int c = lane; c < 256; c += 32) {
+          const int n = it.nb * 256 + c;
+          cs[c] = n < p.N ? __ldg(p.w_scale + n) : 0.f;
+          cs[256 + c] = n < p.N && p.bias ? q8_bias(p, n) : 0.f;
+        }
+        __syncwarp();
+      }
+      const uint32_t cs32 = su32(cs);
       const int64_t row_w0 = int64_t(it.t) * kTileRows + int(crank) * kHalfRows + quad * 32;
       const int n0 = it.nb * 256;
       const float sa = row_w0 + lane < p.M ? __ldg(p.a_scale + row_w0 + lane) : 0.f;
@@ -438,7 +442,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
         tc_ld32(tbase + col, v);
 #pragma unroll
         for (int q = 0; q < 32; ++q) f[q] = __int2float_rn(int(v[q])) * sa;
-        if (!BWD) q8_scale_cols(f, p.w_scale, n0 + col, p.N);
+        if (!BWD) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 s = lds_f4(cs32 + uint32_t(col + 4 * q) * 4u);
+            f[4 * q] *= s.x; f[4 * q + 1] *= s.y; f[4 * q + 2] *= s.z; f[4 * q + 3] *= s.w;
+          }
+        }
       };
       const bool expanded = it.nc > 0;
       if (expanded) {
@@ -466,9 +476,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
           scaled(col, f);
         }
         if (!BWD && p.bias) {
-          if (p.dtype == MLORA_BF16) q8_add_bias(f, static_cast<const __nv_bfloat16*>(p.bias), n0 + col, p.N);
-          else if (p.dtype == MLORA_F16) q8_add_bias(f, static_cast<const __half*>(p.bias), n0 + col, p.N);
-          else q8_add_bias(f, static_cast<const float*>(p.bias), n0 + col, p.N);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 s = lds_f4(cs32 + 1024u + uint32_t(col + 4 * q) * 4u);
+            f[4 * q] += s.x; f[4 * q + 1] += s.y; f[4 * q + 2] += s.z; f[4 * q + 3] += s.w;
+          }
         }
         q8_store_slice(p, f, row_w0, n0 + col, obuf + (slices & 1u) * 2048u, lane);
         ++slices;
@@ -514,7 +526,7 @@ bool q8_tc_ok(const Q8Main& a) {
   return tc_available();
 }
 
-int q8_main_tc(const Q8Main& a, cudaStream_t st) {
+int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
   Q8Params prm;
   memset(&prm, 0, sizeof(prm));
   const int K = a.bwd ? a.d_out : a.d_in, N = a.bwd ? a.d_in : a.d_out;
@@ -551,8 +563,20 @@ int q8_main_tc(const Q8Main& a, cudaStream_t st) {
   const void* fn = a.bwd ? reinterpret_cast<const void*>(&k_q8<true>) : reinterpret_cast<const void*>(&k_q8<false>);
   MLORA_CUDA_TRY(set_smem_once(fn, kQ8Smem));
   const unsigned grid = 2u * unsigned(std::min(prm.n_items, sms / 2));
-  if (a.bwd) k_q8<true><<<grid, kThreads, kQ8Smem, st>>>(prm);
-  else k_q8<false><<<grid, kThreads, kQ8Smem, st>>>(prm);
+  const bool pdl = after != kAfterOther && pdl_enabled();
+  prm.pdl_rows = pdl && after == kAfterRows ? 1 : 0;
+  prm.pdl_z = pdl ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kQ8Smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  MLORA_CUDA_TRY(cudaLaunchKernelEx(&cfg, a.bwd ? &k_q8<true> : &k_q8<false>, prm));
   count_launch();
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
