@@ -1,7 +1,9 @@
 // C-ABI entry points (include/mlora.h): argument checks, plan upload and
 // dispatch between the tcgen05 tensor-core family and the SIMT family.
+#include <algorithm>
 #include <cstring>
 #include <initializer_list>
+#include <memory>
 
 #include "common.cuh"
 #include "q8.cuh"
@@ -14,6 +16,50 @@ namespace {
 
 size_t zt_bytes(const Plan& p, int dtype) {
   return size_t(p.chunks.size()) * kTileRows * kChunk * elem_bytes(dtype);
+}
+
+// Plan of a routing description.  A step calls with the same description
+// several times, and so do the steps of a fixed job mix: the last few plans of
+// the thread are kept and found again by their description's content.  The
+// reference stays valid until the thread's next call.
+const Plan* plan_of(const mlora_problem* prob, const mlora_routing* route, int* status) {
+  struct Kept {
+    int64_t rows;
+    int32_t d_in, d_out, r_pack;
+    std::vector<int32_t> seg_start, seg_adapter, rank, pack_off;
+    std::vector<float> scaling;
+    Plan plan;
+  };
+  constexpr size_t kKept = 8;
+  thread_local std::vector<std::unique_ptr<Kept>> kept;  // most recently used first
+  *status = validate(prob, route);
+  if (*status != MLORA_OK) return nullptr;
+  auto same = [](const auto& v, const auto* a, size_t n) {
+    return v.size() == n && (n == 0 || std::memcmp(v.data(), a, n * sizeof(*a)) == 0);
+  };
+  const size_t ns = size_t(route->n_seg), na = size_t(route->n_adapters), nb = ns ? ns + 1 : 0;
+  for (size_t i = 0; i < kept.size(); ++i) {
+    const Kept& k = *kept[i];
+    if (k.rows == prob->rows && k.d_in == prob->d_in && k.d_out == prob->d_out && k.r_pack == route->r_pack &&
+        same(k.seg_start, route->seg_start, nb) && same(k.seg_adapter, route->seg_adapter, ns) &&
+        same(k.rank, route->rank, na) && same(k.pack_off, route->pack_off, na) &&
+        same(k.scaling, route->scaling, na)) {
+      std::rotate(kept.begin(), kept.begin() + i, kept.begin() + i + 1);
+      return &kept[0]->plan;
+    }
+  }
+  auto k = std::make_unique<Kept>();
+  *status = build_plan(prob, route, &k->plan);
+  if (*status != MLORA_OK) return nullptr;
+  k->rows = prob->rows; k->d_in = prob->d_in; k->d_out = prob->d_out; k->r_pack = route->r_pack;
+  k->seg_start.assign(route->seg_start, route->seg_start + nb);
+  k->seg_adapter.assign(route->seg_adapter, route->seg_adapter + ns);
+  k->rank.assign(route->rank, route->rank + na);
+  k->pack_off.assign(route->pack_off, route->pack_off + na);
+  k->scaling.assign(route->scaling, route->scaling + na);
+  kept.insert(kept.begin(), std::move(k));
+  if (kept.size() > kKept) kept.pop_back();
+  return &kept[0]->plan;
 }
 
 // layout of the caller's workspace: [plan tables | dZt scratch]
@@ -141,27 +187,28 @@ using namespace mlora;
 
 extern "C" int mlora_zsave_bytes(const mlora_problem* prob, const mlora_routing* route, size_t* bytes) {
   if (!bytes) return MLORA_ERR_INVALID_ARG;
-  Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
-  *bytes = zt_bytes(p, prob->dtype);
+  int st;
+  const Plan* p = plan_of(prob, route, &st);
+  if (!p) return st;
+  *bytes = zt_bytes(*p, prob->dtype);
   return MLORA_OK;
 }
 
 extern "C" int mlora_workspace_bytes(const mlora_problem* prob, const mlora_routing* route, size_t* bytes) {
   if (!bytes) return MLORA_ERR_INVALID_ARG;
-  Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
-  *bytes = ws_bytes(p, prob->dtype);
+  int st;
+  const Plan* p = plan_of(prob, route, &st);
+  if (!p) return st;
+  *bytes = ws_bytes(*p, prob->dtype);
   return MLORA_OK;
 }
 
 extern "C" int mlora_plan_upload(const mlora_problem* prob, const mlora_routing* route, void* workspace,
                                  size_t workspace_bytes, void* stream) {
-  Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
+  int st;
+  const Plan* plan = plan_of(prob, route, &st);
+  if (!plan) return st;
+  const Plan& p = *plan;
   if (!workspace) return MLORA_ERR_INVALID_ARG;
   if (!aligned(workspace, 16)) return MLORA_ERR_UNSUPPORTED;
   if (workspace_bytes < ws_bytes(p, prob->dtype)) return MLORA_ERR_WORKSPACE;
@@ -206,9 +253,10 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
                    const void* bias, const void* A_pack, const void* B_pack, void* Y, void* zsave,
                    void* workspace, size_t workspace_bytes, int32_t stages, int32_t tile_begin,
                    int32_t tile_end, const mlora_peer_ar* ar, const mlora_q8* q8, void* stream) {
-  thread_local Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
+  int st;
+  const Plan* plan = plan_of(prob, route, &st);
+  if (!plan) return st;
+  const Plan& p = *plan;
   if (stages & ~(MLORA_STAGE_SHRINK | MLORA_STAGE_MAIN | MLORA_STAGE_NO_EXPAND)) return MLORA_ERR_INVALID_ARG;
   if (tile_begin < 0 || tile_end < tile_begin || tile_end > p.n_tiles) return MLORA_ERR_INVALID_ARG;
   if (prob->rows == 0 || tile_end == tile_begin) return MLORA_OK;
@@ -440,9 +488,10 @@ int backward_staged(const mlora_problem* prob, const mlora_routing* route, const
                     void* dA_pack, void* dB_pack, void* workspace, size_t workspace_bytes, int32_t stages,
                     int32_t tile_begin, int32_t tile_end, int32_t db_begin, int32_t db_end, const mlora_q8* q8,
                     void* stream) {
-  thread_local Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
+  int st;
+  const Plan* plan = plan_of(prob, route, &st);
+  if (!plan) return st;
+  const Plan& p = *plan;
   if (stages & ~(MLORA_BWD_DZ | MLORA_BWD_DX | MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B))
     return MLORA_ERR_INVALID_ARG;
   // the fused SGD step updates the weights whose gradients the call writes
@@ -503,10 +552,10 @@ int backward_all(const mlora_problem* prob, const mlora_routing* route, const vo
   if (!prob || !route) return MLORA_ERR_INVALID_ARG;
   size_t plan_bytes = 0;
   {
-    Plan p;
-    int st = build_plan(prob, route, &p);
-    if (st != MLORA_OK) return st;
-    plan_bytes = p.bytes;
+    int st;
+    const Plan* p = plan_of(prob, route, &st);
+    if (!p) return st;
+    plan_bytes = p->bytes;
   }
   // dZ scratch lives in the workspace after the plan tables
   void* dzt = workspace ? (uint8_t*)workspace + align_up(plan_bytes, 1024) : nullptr;
@@ -555,10 +604,10 @@ int check_q8_problem(const mlora_problem* prob) {
 
 extern "C" int mlora_q8_scratch_bytes(const mlora_problem* prob, const mlora_routing* route, size_t* bytes) {
   if (!bytes) return MLORA_ERR_INVALID_ARG;
-  Plan p;
-  int st = build_plan(prob, route, &p);
-  if (st != MLORA_OK) return st;
-  *bytes = prob->dtype == MLORA_F32 ? 0 : q8_scratch_bytes(p);
+  int st;
+  const Plan* p = plan_of(prob, route, &st);
+  if (!p) return st;
+  *bytes = prob->dtype == MLORA_F32 ? 0 : q8_scratch_bytes(*p);
   return MLORA_OK;
 }
 

@@ -168,6 +168,19 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
              __float_as_uint(f[4 * q + 1]), __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3]));
     __syncwarp();
     float* out = static_cast<float*>(p.out);
+    if (!p.out_rows) {  // consecutive rows
+      float* dst = out + row_w0 * p.N + n + lane;
+      const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const uint32_t a = base + uint32_t(r) * 128u + (((uint32_t(lane) >> 2) ^ (uint32_t(r) & 7u)) << 4) +
+                           (uint32_t(lane) & 3u) * 4u;
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+        if (r < live) dst[int64_t(r) * p.N] = v;
+      }
+      return;
+    }
 #pragma unroll 8
     for (int r = 0; r < 32; ++r) {
       const int64_t o = __shfl_sync(0xffffffffu, orow, r);
@@ -194,6 +207,19 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
            pack2(f[8 * q + 2], f[8 * q + 3], f16), pack2(f[8 * q + 4], f[8 * q + 5], f16),
            pack2(f[8 * q + 6], f[8 * q + 7], f16));
   __syncwarp();
+  if (!p.out_rows) {  // consecutive rows
+    uint16_t* dst = reinterpret_cast<uint16_t*>(out) + row_w0 * p.N + n + lane;
+    const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
+                         (uint32_t(lane) & 7u) * 2u;
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+      if (r < live) dst[int64_t(r) * p.N] = v;
+    }
+    return;
+  }
 #pragma unroll 8
   for (int r = 0; r < 32; ++r) {
     const int64_t o = __shfl_sync(0xffffffffu, orow, r);

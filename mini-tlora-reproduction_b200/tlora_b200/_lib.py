@@ -264,8 +264,16 @@ def check(fn_name, status):
     raise MloraError(fn_name, status, text)
 
 
+_fns = {}
+
+
 def call(fn_name, *args):
-    check(fn_name, getattr(lib(), fn_name)(*args))
+    f = _fns.get(fn_name)
+    if f is None:
+        f = _fns[fn_name] = getattr(lib(), fn_name)
+    status = f(*args)
+    if status != OK:
+        check(fn_name, status)
 
 
 def launch_count() -> int:

@@ -18,6 +18,7 @@ place, and gradients come back as views of packed gradient buffers.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Dict, Iterable, Optional
 
 import numpy as np
@@ -79,7 +80,11 @@ class Int8Base(nn.Module):
 
     @property
     def rows8(self) -> ops.Int8Rows:
-        return ops.Int8Rows(self.weight_q8, self.weight_scale, self.in_features)
+        q, scale = self._buffers["weight_q8"], self._buffers["weight_scale"]
+        r = self.__dict__.get("_rows8")
+        if r is None or r.q is not q or r.scale is not scale:  # moved or replaced buffers
+            r = self.__dict__["_rows8"] = ops.Int8Rows(q, scale, self.in_features)
+        return r
 
     def _apply(self, fn, recurse=True):
         scale = self.weight_scale
@@ -183,25 +188,28 @@ class _PackedAdapters:
         self.A_pack: Optional[torch.Tensor] = None
         self.B_pack: Optional[torch.Tensor] = None
         self._views = None
+        self._scaling = None
 
     def owns(self, adapters: Dict[str, LoRAAdapter]) -> bool:
-        return list(adapters.keys()) == self.keys and all(
-            a is b for a, b in zip((adapters[k] for k in self.keys), self.adapters))
+        return list(adapters.keys()) == self.keys and all(map(operator.is_, adapters.values(), self.adapters))
 
-    def _in_sync(self) -> bool:
-        if self._views is None:
-            return False
-        for ad, (pa, pb) in zip(self.adapters, self._views):
-            if ad.A.data_ptr() != pa or ad.B.data_ptr() != pb:
-                return False
-            if ad.A.device != self.A_pack.device or ad.A.dtype != self.A_pack.dtype:
-                return False
-            if ad.B.device != self.A_pack.device or ad.B.dtype != self.A_pack.dtype:
-                return False
-        return True
+    def params(self) -> list:
+        """A_0, B_0, A_1, ... as the adapters hold them now."""
+        out = []
+        for ad in self.adapters:
+            p = ad._parameters
+            out.append(p["A"])
+            out.append(p["B"])
+        return out
 
-    def sync(self):
-        if self._in_sync():
+    def _in_sync(self, params) -> bool:
+        # a parameter that no longer views the packs has another address: the
+        # packs are alive, so no new storage can share theirs
+        return (self._views is not None and params[0].dtype == self.A_pack.dtype and
+                [p.data_ptr() for p in params] == self._views)
+
+    def sync(self, params=None):
+        if self._in_sync(params if params is not None else self.params()):
             return
         ref = self.adapters[0].A
         dev, dt = ref.device, ref.dtype
@@ -220,11 +228,14 @@ class _PackedAdapters:
                 B_pack[:, o:o + r].copy_(ad.B)
                 ad.A.data = A_pack[o:o + r]
                 ad.B.data = B_pack[:, o:o + r]
-                views.append((ad.A.data_ptr(), ad.B.data_ptr()))
+                views += [ad.A.data_ptr(), ad.B.data_ptr()]
         self.A_pack, self.B_pack, self._views = A_pack, B_pack, views
 
     def scaling(self) -> np.ndarray:
-        return np.array([float(a.scaling) for a in self.adapters], dtype=np.float32)
+        s = [a.scaling for a in self.adapters]
+        if self._scaling is None or self._scaling[0] != s:
+            self._scaling = (s, np.array([float(v) for v in s], dtype=np.float32))
+        return self._scaling[1]
 
     def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
               base8: Optional[ops.Int8Rows] = None, save8: bool = False):
@@ -232,7 +243,8 @@ class _PackedAdapters:
             raise RuntimeError(
                 "tlora_b200 computes on CUDA devices only (sm_100a); move the module and inputs to a "
                 "B200 with .cuda() -- there is no CPU path")
-        self.sync()
+        params = self.params()
+        self.sync(params)
         if self.A_pack.device != x.device:
             raise RuntimeError(f"input on {x.device} but adapters on {self.A_pack.device}")
         if x.dtype != self.A_pack.dtype or (W is not None and W.dtype != x.dtype):
@@ -246,16 +258,15 @@ class _PackedAdapters:
         x = x.contiguous()
         if plan is None:
             plan = ops.route(ids, self.table, x.device)
+        train = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params))
         # nothing is kept for a backward that cannot follow
-        save8 = save8 and torch.is_grad_enabled()
         st = ops.LayerState(self.table, self.scaling(), plan, self.A_pack, self.B_pack, impl, base8=base8,
-                            save8=save8)
-        params = []
-        for ad in self.adapters:
-            params += [ad.A, ad.B]
+                            save8=save8 and train)
         Wc = W.contiguous() if W is not None else None
         bc = bias.contiguous() if bias is not None else None
-        with torch.cuda.device(x.device):
+        with ops._on(x.device):
+            if not train:
+                return ops.forward_raw(x.detach(), Wc, bc, st)[0]
             return ops.MultiLoRAFunction.apply(x, Wc, bc, st, *params)
 
 
@@ -293,7 +304,7 @@ class MultiLoRALinear(_Int8BaseMixin, nn.Module):
         return self.adapters[str(adapter_id)].parameters()
 
     def _pack(self) -> _PackedAdapters:
-        ads = dict(self.adapters.items())
+        ads = self.adapters._modules
         if self._packed is None or not self._packed.owns(ads):
             self._packed = _PackedAdapters(ads)
         return self._packed

@@ -32,11 +32,30 @@ def mlora_dtype(dt: torch.dtype) -> int:
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _on:
+    """``torch.cuda.device(device)`` that costs nothing where the device is
+    the current one already."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device: torch.device):
+        self.device, self.guard = device, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 # ---------------------------------------------------------------------------
@@ -96,6 +115,12 @@ class RoutePlan:
     # workspaces that already hold this plan on the device (make_resident),
     # keyed by the call shape; calls with such a key upload nothing
     resident: dict = field(default_factory=dict)
+    # the C descriptions of calls made with this plan, by call shape and
+    # adapter layout (built once)
+    calls: dict = field(default_factory=dict, repr=False)
+
+    def __getstate__(self):
+        return {**self.__dict__, "calls": {}}  # C structures are neither copied nor pickled
 
     @property
     def n_seg(self) -> int:
@@ -230,7 +255,7 @@ class Int8Rows:
 
     @property
     def shape(self):
-        return torch.Size((self.q.shape[0], self.cols))
+        return (self.q.shape[0], self.cols)
 
     @property
     def device(self) -> torch.device:
@@ -243,15 +268,33 @@ def q8_ld(cols: int) -> int:
 
 
 def _new_rows8(rows: int, cols: int, device) -> Int8Rows:
-    return Int8Rows(torch.empty(rows, q8_ld(cols), dtype=torch.int8, device=device),
-                    torch.empty(rows, dtype=torch.float32, device=device), cols)
+    r = Int8Rows.__new__(Int8Rows)  # the layout is right by construction
+    r.q = torch.empty((rows, q8_ld(cols)), dtype=torch.int8, device=device)
+    r.scale = torch.empty(rows, dtype=torch.float32, device=device)
+    r.cols = cols
+    return r
 
 
-def _q8_struct(base8: Optional[Int8Rows], rows8: Optional[Int8Rows], grad8: Optional[Int8Rows] = None):
-    def pair(m):
-        return (m.q.data_ptr(), m.scale.data_ptr()) if m is not None else (None, None)
+class _Scratch8:
+    """8-bit rows that live for one call: one buffer, the scales after the rows."""
 
-    return _lib.Q8(*pair(base8), *pair(rows8), *pair(grad8))
+    __slots__ = ("buf", "ptrs")
+
+    def __init__(self, rows: int, cols: int, device):
+        n = rows * q8_ld(cols)
+        self.buf = torch.empty(n + 4 * rows, dtype=torch.uint8, device=device)
+        p = self.buf.data_ptr()
+        self.ptrs = (p, p + n)
+
+
+def _ptrs8(m):
+    if m is None:
+        return None, None
+    return m.ptrs if isinstance(m, _Scratch8) else (m.q.data_ptr(), m.scale.data_ptr())
+
+
+def _q8_struct(base8: Optional[Int8Rows], rows8, grad8=None):
+    return _lib.Q8(*_ptrs8(base8), *_ptrs8(rows8), *_ptrs8(grad8))
 
 
 def _check_cuda(t: torch.Tensor, what: str) -> None:
@@ -268,7 +311,6 @@ def _row_major(x: torch.Tensor):
     return x, x.stride(0)
 
 
-@torch.no_grad()
 def quantize_rows(x: torch.Tensor, col_scale: Optional[torch.Tensor] = None) -> Int8Rows:
     """8-bit rows of ``x`` [rows, cols] (float32, bfloat16 or float16):
     ``scale[i] = float32(max_k |x[i, k]| / 127)`` and
@@ -284,21 +326,20 @@ def quantize_rows(x: torch.Tensor, col_scale: Optional[torch.Tensor] = None) -> 
     if col_scale is not None and (col_scale.dtype != torch.float32 or col_scale.shape != (x.shape[1],) or
                                   col_scale.device != x.device):
         raise ValueError("col_scale must be a float32 vector on x's device, one element per column")
-    with torch.cuda.device(x.device):
-        x, ld = _row_major(x)
-        cs = col_scale.contiguous() if col_scale is not None else None
+    with _on(x.device):
+        x, ld = _row_major(x.detach())
+        cs = col_scale.detach().contiguous() if col_scale is not None else None
         out = _new_rows8(x.shape[0], x.shape[1], x.device)
         _lib.call("mlora_q8_quantize", _ptr(x), x.shape[0], x.shape[1], ld, dt, _ptr(cs), _ptr(out.q),
                   _ptr(out.scale), _stream(x.device))
     return out
 
 
-@torch.no_grad()
 def dequantize_rows(rows8: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The matrix [rows, cols] that 8-bit rows stand for, rounded once to ``dtype``."""
     _check_cuda(rows8.q, "dequantize_rows")
     dt = mlora_dtype(dtype)
-    with torch.cuda.device(rows8.device):
+    with _on(rows8.device):
         out = torch.empty(rows8.rows, rows8.cols, dtype=dtype, device=rows8.device)
         _lib.call("mlora_q8_dequantize", _ptr(rows8.q), _ptr(rows8.scale), rows8.rows, rows8.cols, dt, _ptr(out),
                   _stream(rows8.device))
@@ -320,27 +361,28 @@ class Int8LinearFunction(torch.autograd.Function):
         wq, w_scale = ctx.saved_tensors
         rows, d_out, d_in = dy.shape[0], wq.shape[0], ctx.d_in
         dev = dy.device
-        with torch.cuda.device(dev):
+        with _on(dev):
             dy = dy.contiguous()
-            g8 = _new_rows8(rows, d_out, dev)
-            dx = torch.empty(rows, d_in, dtype=dy.dtype, device=dev)
+            g8 = _Scratch8(rows, d_out, dev)
+            dx = torch.empty((rows, d_in), dtype=dy.dtype, device=dev)
             prob = _lib.Problem(rows, d_in, d_out, mlora_dtype(dy.dtype), _lib.IMPL_AUTO)
-            _lib.call("mlora_q8_linear_dx", ctypes.byref(prob), _ptr(dy), _ptr(g8.q), _ptr(g8.scale), _ptr(wq),
-                      _ptr(w_scale), _ptr(dx), _stream(dev))
+            _lib.call("mlora_q8_linear_dx", ctypes.byref(prob), _ptr(dy), *g8.ptrs, _ptr(wq), _ptr(w_scale),
+                      _ptr(dx), _stream(dev))
         return dx, None, None, None, None
 
 
 def _int8_product(x, weight: Int8Rows, bias, dtype):
     dev = weight.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         if isinstance(x, Int8Rows):
             x8, src, ld = x, None, 0
         else:
-            src, ld = _row_major(x)
-            x8 = _new_rows8(x.shape[0], x.shape[1], dev)
-        y = torch.empty(x8.rows, weight.rows, dtype=dtype, device=dev)
-        prob = _lib.Problem(x8.rows, weight.cols, weight.rows, mlora_dtype(dtype), _lib.IMPL_AUTO)
-        _lib.call("mlora_q8_linear", ctypes.byref(prob), _ptr(src), ld, _ptr(x8.q), _ptr(x8.scale), _ptr(weight.q),
+            src, ld = _row_major(x.detach())
+            x8 = _Scratch8(x.shape[0], x.shape[1], dev)
+        rows, (d_out, d_in) = x.shape[0], weight.shape
+        y = torch.empty((rows, d_out), dtype=dtype, device=dev)
+        prob = _lib.Problem(rows, d_in, d_out, mlora_dtype(dtype), _lib.IMPL_AUTO)
+        _lib.call("mlora_q8_linear", ctypes.byref(prob), _ptr(src), ld, *_ptrs8(x8), _ptr(weight.q),
                   _ptr(weight.scale), _ptr(bias), _ptr(y), _stream(dev))
     return y
 
@@ -381,7 +423,7 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
         if bias.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the 8-bit linear is frozen: no gradient of its bias")
         bias = bias.contiguous()
-    if eight:
+    if eight or not (x.requires_grad and torch.is_grad_enabled()):
         return _int8_product(x, weight, bias, dtype)
     return Int8LinearFunction.apply(x, weight.q, weight.scale, bias, weight.cols)
 
@@ -420,6 +462,38 @@ class _CallArgs:
         _lib.call("mlora_zsave_bytes", ctypes.byref(self.prob), ctypes.byref(self.route), ctypes.byref(z))
         _lib.call("mlora_workspace_bytes", ctypes.byref(self.prob), ctypes.byref(self.route), ctypes.byref(w))
         return int(z.value), int(w.value)
+
+
+class _Call:
+    """One call made with a routing plan: a fresh mlora_problem over the plan's
+    kept mlora_routing and buffer sizes."""
+
+    __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "_scratch")
+
+    def __init__(self, rows, d_in, d_out, dtype, st: "LayerState"):
+        plan, table = st.plan, st.table
+        key = (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.rank.tobytes(), st.scaling.tobytes())
+        kept = plan.calls.get(key)
+        if kept is None:
+            args = _CallArgs(rows, d_in, d_out, dtype, st.impl, plan, table, st.scaling, out_rows=plan.perm)
+            kept = (args, args.sizes(), {})
+            plan.calls[key] = kept
+        self.args, (self.zbytes, self.wbytes), self._scratch = kept
+        word = st.err_word
+        if word is not None and (word.dtype != torch.int32 or word.device.type != "cuda"):
+            raise ValueError("err_word must be a CUDA int32 tensor")
+        self.prob = _lib.Problem(rows, d_in, d_out, dtype, _IMPLS[st.impl], 0, 0,
+                                 word.data_ptr() if word is not None else None)
+        self.route = self.args.route
+
+    def scratch8(self) -> int:
+        """mlora_q8_scratch_bytes of the call."""
+        n = self._scratch.get("bytes")
+        if n is None:
+            sb = ctypes.c_size_t(0)
+            _lib.call("mlora_q8_scratch_bytes", ctypes.byref(self.prob), ctypes.byref(self.route), ctypes.byref(sb))
+            n = self._scratch["bytes"] = int(sb.value)
+        return n
 
 
 @dataclass
@@ -485,9 +559,8 @@ def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8
     rows, d_in = x.shape
     d_out = st.B_pack.shape[0]
     xs = x_sorted if x_sorted is not None else (gather_rows(x, st.plan.perm) if st.plan.perm is not None else x)
-    args = _CallArgs(rows, d_in, d_out, mlora_dtype(x.dtype), st.impl, st.plan, st.table, st.scaling,
-                     out_rows=st.plan.perm, err_word=st.err_word)
-    zb, wb = args.sizes()
+    args = _Call(rows, d_in, d_out, mlora_dtype(x.dtype), st)
+    zb, wb = args.zbytes, args.wbytes
     dev = x.device
     y = torch.empty(rows, d_out, dtype=x.dtype, device=dev)
     z = torch.empty(max(zb, 1), dtype=torch.uint8, device=dev)
@@ -497,7 +570,7 @@ def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8
                   _ptr(st.A_pack), _ptr(st.B_pack), _ptr(y), _ptr(z), _ptr(ws), wb, _stream(dev))
         return y, z, xs, args
     if rows8 is None:
-        rows8 = _new_rows8(rows, d_in, dev)
+        rows8 = _Scratch8(rows, d_in, dev)
     q8 = _q8_struct(st.base8, rows8)
     _lib.call("mlora_forward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8), _ptr(xs),
               _ptr(W), _ptr(bias), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(y), _ptr(z), _ptr(ws), wb, _stream(dev))
@@ -581,9 +654,8 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     d_out = st.B_pack.shape[0]
     dev = dy.device
     dys = gather_rows(dy, st.plan.perm) if st.plan.perm is not None else dy
-    args = _CallArgs(rows, d_in, d_out, mlora_dtype(dy.dtype), st.impl, st.plan, st.table, st.scaling,
-                     out_rows=st.plan.perm, err_word=st.err_word)
-    _, wb = args.sizes()
+    args = _Call(rows, d_in, d_out, mlora_dtype(dy.dtype), st)
+    wb = args.wbytes
     ws, args.prob.flags = _workspace(st, args, wb, dev)
     dx = torch.empty(rows, d_in, dtype=dy.dtype, device=dev) if want_dx else None
     # every rank row / column of an adapter that owns rows is written; the
@@ -591,13 +663,12 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     dA = torch.empty_like(st.A_pack) if want_dA else None
     dB = torch.empty_like(st.B_pack) if want_dB else None
     if st.base8 is not None or rows8 is not None:
-        grad8 = _new_rows8(rows, d_out, dev) if st.base8 is not None and want_dx else None
+        grad8 = _Scratch8(rows, d_out, dev) if st.base8 is not None and want_dx else None
         q8 = _q8_struct(st.base8, rows8, grad8)
         if rows8 is not None and want_dA:
-            sb = ctypes.c_size_t(0)
-            _lib.call("mlora_q8_scratch_bytes", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(sb))
-            scratch = torch.empty(max(int(sb.value), 1), dtype=torch.uint8, device=dev)
-            q8.scratch, q8.scratch_bytes = scratch.data_ptr(), sb.value
+            q8.scratch_bytes = args.scratch8()
+            scratch = torch.empty(max(q8.scratch_bytes, 1), dtype=torch.uint8, device=dev)
+            q8.scratch = scratch.data_ptr()
         _lib.call("mlora_backward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8),
                   _ptr(dys), _ptr(xs), _ptr(W), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA),
                   _ptr(dB), _ptr(ws), wb, _stream(dev))
