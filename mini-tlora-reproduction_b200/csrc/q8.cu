@@ -31,6 +31,29 @@ __device__ __noinline__ int q8_exact(float x, float s) {
   return max(-127, min(127, q));  // s may have been rounded down where it is subnormal
 }
 
+// Two fp32 operations in one instruction (each rounded as the single one is).
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Eight elements of a row as loaded, their values and the magnitudes' maximum.
 template <class T> struct Vec8;
 template <> struct Vec8<float> {
@@ -85,17 +108,14 @@ template <class T> struct Top {
   }
 };
 template <> struct Top<float> {
-  uint32_t v = 0;
-  __device__ __forceinline__ void see(const float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v = max(v, __float_as_uint(f[i]) & 0x7fffffffu);
-  }
+  float v = 0.f;
   __device__ __forceinline__ void see(const Vec8<float>& x) {
     float f[8];
     x.get(f);
-    see(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v = max_nan(v, fabsf(f[i]));
   }
-  __device__ __forceinline__ uint32_t bits() const { return v; }
+  __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(v); }
 };
 
 // eight elements from column c of a row; past `cols` they are zero
@@ -123,8 +143,10 @@ __device__ __forceinline__ void scale8(float (&f)[8], const float* col_scale, in
       a = __ldg(reinterpret_cast<const float4*>(col_scale + c));
       b = __ldg(reinterpret_cast<const float4*>(col_scale + c) + 1);
     }
-    f[0] *= a.x; f[1] *= a.y; f[2] *= a.z; f[3] *= a.w;
-    f[4] *= b.x; f[5] *= b.y; f[6] *= b.z; f[7] *= b.w;
+    mul2(F2(f[0], f[1]), F2(a.x, a.y)).get(f[0], f[1]);
+    mul2(F2(f[2], f[3]), F2(a.z, a.w)).get(f[2], f[3]);
+    mul2(F2(f[4], f[5]), F2(b.x, b.y)).get(f[4], f[5]);
+    mul2(F2(f[6], f[7]), F2(b.z, b.w)).get(f[6], f[7]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -157,23 +179,35 @@ struct RowScale {
 
 __device__ __forceinline__ uint2 round8(const float (&f)[8], const RowScale& r) {
   constexpr float kMagic = 12582912.f;
-  uint32_t q[8], differ = 0;
+  const F2 magic(kMagic, kMagic);
+  // the integers of f times a reciprocal, as float bits
+  auto round = [&](float by, uint32_t (&o)[8]) {
+    const F2 by2(by, by);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fmaf(f[i], r.above, kMagic));
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      fma2(F2(f[2 * i], f[2 * i + 1]), by2, magic).get(a, b);
+      o[2 * i] = __float_as_uint(a);
+      o[2 * i + 1] = __float_as_uint(b);
+    }
+  };
+  uint32_t q[8];
+  round(r.above, q);
   if (r.how != kOne) {
+    uint32_t lo[8], differ = 0;
+    round(r.below, lo);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) differ |= q[i] ^ __float_as_uint(fmaf(f[i], r.below, kMagic));
+    for (int i = 0; i < 8; ++i) differ |= q[i] ^ lo[i];
     if (r.how == kSlow) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) q[i] = r.s > 0.f ? uint32_t(q8_exact(f[i], r.s)) : 0u;
     } else if (differ) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float n = fminf(fmaf(f[i], r.above, kMagic), fmaf(f[i], r.below, kMagic)) - kMagic;
+        const float n = fminf(__uint_as_float(q[i]), __uint_as_float(lo[i])) - kMagic;
         const float d = fmaf(-(n + 0.5f), r.s, f[i]);
         const uint32_t u = __float_as_uint(n + kMagic);
-        if (q[i] != __float_as_uint(fmaf(f[i], r.below, kMagic)))
-          q[i] = u + (d > 0.f || (d == 0.f && (u & 1u)) ? 1u : 0u);
+        if (q[i] != lo[i]) q[i] = u + (d > 0.f || (d == 0.f && (u & 1u)) ? 1u : 0u);
       }
     }
   }
@@ -325,11 +359,12 @@ int launch_quantize(const T* src, int64_t rows, int64_t cols, int64_t ld, const 
                     cudaStream_t st) {
   const int64_t groups = q8_ld(cols) / 8;  // the zero bytes past `cols` included
   constexpr bool kWide = CS || sizeof(T) == 4;  // held as float32
-  const RowGrid g = row_grid(rows, groups, kWide ? 8 : 16);
+  const RowGrid g = row_grid(rows, groups, kWide ? 4 : 16);
 #define MLORA_QUANT(NV) \
   k_quantize<T, VEC, CS, NV><<<g.grid, g.block, 0, st>>>(src, rows, int(cols), ld, cs, q, scale, g.sh)
   if (g.nv <= 1) MLORA_QUANT(1);
   else if (g.nv <= 2) MLORA_QUANT(2);
+  else if (g.nv <= 3) MLORA_QUANT(3);
   else if (g.nv <= 4) MLORA_QUANT(4);
   else if (g.nv <= 6) MLORA_QUANT(6);
   else if (g.nv <= 8) MLORA_QUANT(8);
