@@ -74,7 +74,7 @@ struct PlanDev {
   int32_t* counters;                // [16] work counters of the persistent kernels, one per role;
                                     // zeroed by every plan upload (one per API call)
   const SavedItem* saved;           // [n_saved]
-  int32_t* saved_done;              // [saved groups] finished parts, zeroed with the counters
+  int32_t* saved_done;              // [saved groups][4] finished parts per epilogue warp, zeroed with the counters
   int* err;                         // status word of this call (mlora_problem.err_word), or nullptr
                                     // for the library-wide word g_err_word
 };

@@ -225,7 +225,7 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
   p->off_saved = off;
   off = align_up(off + sizeof(SavedItem) * p->saved.size(), 256);
   p->off_counters = off;  // the persistent kernels' counters, then the saved groups' (all zeroed per call)
-  off = align_up(off + 64 + sizeof(int32_t) * size_t(p->saved_groups), 256);
+  off = align_up(off + 64 + 4 * sizeof(int32_t) * size_t(p->saved_groups), 256);
   p->bytes = off;
   return MLORA_OK;
 }

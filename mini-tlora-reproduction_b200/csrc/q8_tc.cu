@@ -634,7 +634,7 @@ constexpr int kDaStages = 4, kDaStageBytes = 32 * 1024;  // 64 x 256 bytes of X,
 constexpr int kDaConv = 2, kDaConvBytes = 32 * 1024;     // 64 x 256 bf16
 constexpr int kDaConvWarps = 8, kDaProducers = 2;
 constexpr int kDaThreads = 32 * (4 + kDaConvWarps + 1 + kDaProducers);
-constexpr int kDaSumBytes = 2 * 32 * 32 * 4;             // low sums of one 32-column slice, two warps
+constexpr int kDaSumBytes = 4 * 32 * 32 * 4;             // sums that the epilogue warps hand over
 constexpr int kDaSmem = kDaStages * kDaStageBytes + kDaConv * kDaConvBytes + kDaSumBytes + 1024 + 512;
 static_assert(kDaSmem <= 232448, "dynamic shared memory above 227 KB");
 
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* last_part = abort_flag + 1;  // [2] per pair of epilogue warps
+  volatile int* going = abort_flag + 1;  // [4] per epilogue warp
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   constexpr int kMma = 4 + kDaConvWarps;
@@ -873,45 +873,41 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
   } else if (warp < 4) {
     // ---------------------------------------------------------------- epilogue
     // Lanes 0..63 of the accumulator hold the high sums of ranks 0..63 (warps
-    // 0 and 1), lanes 64..127 the low sums (warps 2 and 3): warp 2 + i hands
-    // its sums to warp i through shared memory.
+    // 0 and 1), lanes 64..127 the low sums (warps 2 and 3).  Warps i and i + 2
+    // trade 32-column slices through shared memory: of every two, the one
+    // finishes the even and the other the odd slice.
     const int half = warp & 1;  // ranks 32 half ..
     const bool low = warp >= 2;
-    float* mine = sums + half * 32 * 32;
+    const uint32_t give = su32(sums) + uint32_t(warp) * 4096u, take = su32(sums) + uint32_t(warp ^ 2) * 4096u;
     int acc = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
     for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
       SavedItem it;
       if (!da_item(p, item, it)) continue;
       // both warps of a pair must agree to go on before they meet at a barrier
-      ok = warp_wait(&tfull[acc], acc_phase, abort_flag, p.plan.err);
-      if (lane == 0 && low) last_part[half] = ok ? 1 : 0;
+      const bool ok = warp_wait(&tfull[acc], acc_phase, abort_flag, p.plan.err);
+      if (lane == 0) going[warp] = ok ? 1 : 0;
       pair_barrier(1 + half);
-      const bool both = ok && last_part[half] != 0;
+      const bool both = going[half] != 0 && going[half + 2] != 0;
       pair_barrier(1 + half);
-      if (lane == 0 && !low) last_part[half] = both ? 1 : 0;
-      pair_barrier(1 + half);
-      if (last_part[half] == 0) break;
+      if (!both) break;
       tc_fence_after();
       const uint32_t tbase = tmem + (uint32_t(warp * 32) << 16) + uint32_t(acc * kAccCols);
       const int c0 = it.block * kSavedCols;
-      const int r = 32 * half + lane;              // rank row inside the chunk
-      const int pcol = p.plan.chunks[p.plan.list[it.lb] + it.j].pcol;
+      const int r = 32 * half + lane;  // rank row inside the chunk
       const bool live = r < it.rank - it.j * 64;
-      float* part = it.nparts > 1 ? p.parts + (int64_t(it.part0 + it.part) * 64 + r) * kSavedCols : nullptr;
+      const int64_t row0 = int64_t(p.plan.chunks[p.plan.list[it.lb] + it.j].pcol + r) * p.d_in + c0;
       auto finish = [&](int col, const float (&f)[32]) {
         // 32 columns of one rank row of dA: 64 contiguous bytes (d_in is a multiple of 8)
-        const int64_t e0 = int64_t(pcol + r) * p.d_in + c0 + col;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (!live || c0 + col + 8 * g >= p.d_in) break;
           uint32_t w[4];
 #pragma unroll
           for (int h = 0; h < 4; ++h) w[h] = pack2(f[8 * g + 2 * h], f[8 * g + 2 * h + 1], p.f16 != 0);
-          reinterpret_cast<uint4*>(p.dA + e0)[g] = make_uint4(w[0], w[1], w[2], w[3]);
+          reinterpret_cast<uint4*>(p.dA + row0 + col)[g] = make_uint4(w[0], w[1], w[2], w[3]);
           if (p.A_upd) {  // fused SGD step, from the gradient as stored
-            uint4* P = reinterpret_cast<uint4*>(p.A_upd + e0) + g;
+            uint4* P = reinterpret_cast<uint4*>(p.A_upd + row0 + col) + g;
             const uint4 old = *P;
             uint32_t o[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
@@ -923,61 +919,70 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
           }
         }
       };
-      for (int col = 0; col < kSavedCols && c0 + col < p.d_in; col += 32) {
+      // a part is [64 column groups][64 ranks][4 columns]: a warp's stores are contiguous
+      auto part_of = [&](int k, int col) {
+        return reinterpret_cast<float4*>(p.parts) + (int64_t(it.part0 + k) * 64 + col / 4) * 64 + r;
+      };
+      for (int col2 = 0; col2 < kSavedCols && c0 + col2 < p.d_in; col2 += 64) {
+        const int col = col2 + (low ? 32 : 0);  // the slice this warp finishes
         uint32_t v[32];
+        tc_ld32(tbase + (col ^ 32), v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          sts128(give + uint32_t(lane) * 128u + ((uint32_t(q) ^ (uint32_t(lane) & 7u)) << 4), v[4 * q], v[4 * q + 1],
+                 v[4 * q + 2], v[4 * q + 3]);
         tc_ld32(tbase + col, v);
-        if (low) {
+        pair_barrier(1 + half);
+        float f[32];
 #pragma unroll
-          for (int q = 0; q < 32; ++q) mine[lane * 32 + ((q + lane) & 31)] = __uint_as_float(v[q]);
+        for (int q = 0; q < 8; ++q) {
+          const float4 o = lds_f4(take + uint32_t(lane) * 128u + ((uint32_t(q) ^ (uint32_t(lane) & 7u)) << 4));
+          f[4 * q] = __uint_as_float(v[4 * q]) + o.x;
+          f[4 * q + 1] = __uint_as_float(v[4 * q + 1]) + o.y;
+          f[4 * q + 2] = __uint_as_float(v[4 * q + 2]) + o.z;
+          f[4 * q + 3] = __uint_as_float(v[4 * q + 3]) + o.w;
         }
         pair_barrier(1 + half);
-        if (!low) {
-          float f[32];
+        if (it.nparts > 1) {
+          float4* dst = part_of(it.part, col);
 #pragma unroll
-          for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(v[q]) + mine[lane * 32 + ((q + lane) & 31)];
-          if (part) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              __stcg(reinterpret_cast<float4*>(part + col) + q,
-                     make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]));
-          } else {
-            finish(col, f);
-          }
+          for (int q = 0; q < 8; ++q)
+            __stcg(dst + q * 64, make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]));
+        } else if (c0 + col < p.d_in) {
+          finish(col, f);
         }
-        pair_barrier(1 + half);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
-      if (it.nparts > 1 && !low) {
-        // this warp's 32 ranks of the part are stored: the warp that stores
-        // the last part of these ranks adds them all up, in order
+      if (it.nparts > 1) {
+        // this warp's slices of the part are stored: the warp that stores the
+        // last part's adds them all up, in the parts' order
         int last = 0;
         __threadfence();
         __syncwarp();
-        if (lane == 0) {
-          last = atomicAdd(p.plan.saved_done + it.group, half ? 1 << 16 : 1);
-          last = (half ? last >> 16 : last & 0xffff) == it.nparts - 1;
-        }
+        if (lane == 0) last = atomicAdd(p.plan.saved_done + 4 * it.group + warp, 1) == it.nparts - 1;
         last = __shfl_sync(0xffffffffu, last, 0);
         __threadfence();
-        if (last) {
-          for (int col = 0; col < kSavedCols && c0 + col < p.d_in; col += 32) {
-            float f[32];
+        if (!last) continue;
+        for (int col = low ? 32 : 0; col < kSavedCols && c0 + col < p.d_in; col += 64) {
+          float f[32];
 #pragma unroll
-            for (int q = 0; q < 32; ++q) f[q] = 0.f;
-            for (int k = 0; k < it.nparts; ++k) {
-              const float* src = p.parts + (int64_t(it.part0 + k) * 64 + r) * kSavedCols + col;
+          for (int q = 0; q < 32; ++q) f[q] = 0.f;
+#pragma unroll 2
+          for (int k = 0; k < it.nparts; ++k) {
+            const float4* src = part_of(k, col);
+            float4 u[8];
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float4 u = __ldcg(reinterpret_cast<const float4*>(src) + q);
-                f[4 * q] += u.x; f[4 * q + 1] += u.y; f[4 * q + 2] += u.z; f[4 * q + 3] += u.w;
-              }
+            for (int q = 0; q < 8; ++q) u[q] = __ldcg(src + q * 64);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              f[4 * q] += u[q].x; f[4 * q + 1] += u[q].y; f[4 * q + 2] += u[q].z; f[4 * q + 3] += u[q].w;
             }
-            finish(col, f);
           }
+          finish(col, f);
         }
       }
     }
