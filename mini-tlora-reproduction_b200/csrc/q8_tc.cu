@@ -633,6 +633,7 @@ namespace {
 constexpr int kDaStages = 4, kDaStageBytes = 32 * 1024;  // 64 x 256 bytes of X, 2 x 64 x 64 of w
 constexpr int kDaConv = 2, kDaConvBytes = 32 * 1024;     // 64 x 256 bf16
 constexpr int kDaConvWarps = 8, kDaProducers = 2;
+constexpr int kDaConvGroup = kDaConvWarps / kDaConv;     // warps that convert one k-block
 constexpr int kDaThreads = 32 * (4 + kDaConvWarps + 1 + kDaProducers);
 constexpr int kDaSumBytes = 4 * 32 * 32 * 4;             // sums that the epilogue warps hand over
 constexpr int kDaSmem = kDaStages * kDaStageBytes + kDaConv * kDaConvBytes + kDaSumBytes + 1024 + 512;
@@ -657,6 +658,14 @@ __device__ __forceinline__ bool da_item(const DaParams& p, int i, SavedItem& it)
                   it.part < it.nparts;
   if (!ok) flag_error(p.plan.err, kErrBounds);
   return ok;
+}
+
+// Item of this block's round k, or -1: the items are sorted by length, and every
+// other round deals them out backwards, so that a block with a long item of
+// one round has a short one in the next.
+__device__ __forceinline__ int da_deal(int k, int n_items) {
+  const int i = k * int(gridDim.x) + int((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  return i < n_items ? i : -1;
 }
 
 // {chunk, tile, first slice, end slice} of list entry e (clamped and flagged
@@ -704,10 +713,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
   if (threadIdx.x == 0) {
     for (int s = 0; s < kDaStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kDaConvWarps + 1);
+      mbar_init(&empty[s], kDaConvGroup + 1);
     }
     for (int s = 0; s < kDaConv; ++s) {
-      mbar_init(&cfull[s], kDaConvWarps);
+      mbar_init(&cfull[s], kDaConvGroup);
       mbar_init(&cempty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -737,7 +746,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
     int stage = 0;
     bool ok = true;
     const uint64_t pol_stream = policy_evict_first(), pol_norm = policy_evict_normal();
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (int round = 0; round * int(gridDim.x) < n_items && ok; ++round) {
+      const int item = da_deal(round, n_items);
+      if (item < 0) break;
       SavedItem it;
       if (!da_item(p, item, it)) continue;
       int e = it.e0, q = it.q0;
@@ -779,7 +790,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
     uint32_t phase = 0, cphase = 0, acc_phase = 0;
     bool ok = true;
     const uint32_t idesc = idesc_16(128, 256, true, true, false);  // bf16 for either type of the layer
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (int round = 0; round * int(gridDim.x) < n_items && ok; ++round) {
+      const int item = da_deal(round, n_items);
+      if (item < 0) break;
       SavedItem it;
       if (!da_item(p, item, it)) continue;
       if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err)) { ok = false; break; }
@@ -814,60 +827,63 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
     }
   } else if (warp >= 4 && warp < kMma) {
     // ---------------------------------------------------------------- conversion
-    // 16-byte piece c (0..7) of row k of 128-column half h: columns 16 c.. of
-    // the half become two 16-byte groups of bf16 box 2 h + c / 4.  Lanes of
-    // the upper boxes write their second group first, so that a quarter warp
-    // covers all banks.
-    const int t = (warp - 4) * 32 + lane;  // 0..255
-    int stage = 0, cs = 0;
+    // Two groups of four warps convert alternate k-blocks, each into its own
+    // buffer, so that one group's waits and stores overlap the other's.
+    // A thread turns a 16-byte piece (columns 16 cl .. of a 64-column box, one
+    // row) into two 16-byte groups of bf16.  A quarter warp covers the four
+    // pieces of a box in rows r and r ^ 5: with the 128-byte swizzle its loads
+    // (bit 2 of the row differs) and its stores (bit 0) both touch all banks.
+    const int cs = (warp - 4) / kDaConvGroup;
+    const int t = ((warp - 4) % kDaConvGroup) * 32 + lane;  // 0..127
+    const uint32_t dst = su32(conv + cs * kDaConvBytes);
+    const uint32_t cl = uint32_t(t & 3), flip = (t & 4) ? 5u : 0u, r0 = 2u * uint32_t(t >> 3);
+    int stage = 0, turn = 0;
     uint32_t phase = 0, cphase = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (int round = 0; round * int(gridDim.x) < n_items && ok; ++round) {
+      const int item = da_deal(round, n_items);
+      if (item < 0) break;
       SavedItem it;
       if (!da_item(p, item, it)) continue;
       for (int kb = 0; kb < it.nks; ++kb) {
-        if (!warp_wait(&full[stage], phase, abort_flag, p.plan.err) ||
-            !warp_wait(&cempty[cs], cphase ^ 1, abort_flag, p.plan.err)) {
-          ok = false;
-          break;
-        }
-        const uint32_t src = su32(smem + stage * kDaStageBytes), dst = su32(conv + cs * kDaConvBytes);
-        const uint32_t c = uint32_t(t & 7), k0 = uint32_t(t >> 3);  // rows k0 and k0 + 32 of both halves
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t h = uint32_t(i) >> 1, k = k0 + 32u * (uint32_t(i) & 1u);
-          v[i] = lds128(src + h * 8192u + k * 128u + ((c ^ (k & 7u)) << 4));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t h = uint32_t(i) >> 1, k = k0 + 32u * (uint32_t(i) & 1u);
-          const uint32_t row = dst + (2u * h + (c >> 2)) * uint32_t(kBox64) + k * 128u;
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-          uint32_t o[8];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            o[2 * q] = bytes_to_bf16x2(w[q], 0x4140);
-            o[2 * q + 1] = bytes_to_bf16x2(w[q], 0x4342);
+        if (turn == cs) {
+          if (!warp_wait(&full[stage], phase, abort_flag, p.plan.err) ||
+              !warp_wait(&cempty[cs], cphase ^ 1, abort_flag, p.plan.err)) {
+            ok = false;
+            break;
           }
-          const uint32_t g = (c & 3u) * 2u, first = c >> 2;
-          const uint32_t a0 = row + (((g + first) ^ (k & 7u)) << 4), a1 = row + (((g + 1u - first) ^ (k & 7u)) << 4);
-          if (first) {
-            sts128(a0, o[4], o[5], o[6], o[7]);
-            sts128(a1, o[0], o[1], o[2], o[3]);
-          } else {
-            sts128(a0, o[0], o[1], o[2], o[3]);
-            sts128(a1, o[4], o[5], o[6], o[7]);
+          const uint32_t src = su32(smem + stage * kDaStageBytes);
+          // rows (r0 + 32 i) ^ flip, the four boxes of each
+          uint4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t k = (r0 + 32u * (uint32_t(i) >> 2)) ^ flip, box = uint32_t(i) & 3u;
+            v[i] = lds128(src + (box >> 1) * 8192u + k * 128u + ((((box & 1u) * 4u + cl) ^ (k & 7u)) << 4));
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t k = (r0 + 32u * (uint32_t(i) >> 2)) ^ flip, box = uint32_t(i) & 3u;
+            const uint32_t row = dst + box * uint32_t(kBox64) + k * 128u, g = (2u * cl) ^ (k & 7u);
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              o[2 * q] = bytes_to_bf16x2(w[q], 0x4140);
+              o[2 * q + 1] = bytes_to_bf16x2(w[q], 0x4342);
+            }
+            sts128(row + (g << 4), o[0], o[1], o[2], o[3]);
+            sts128(row + ((g ^ 1u) << 4), o[4], o[5], o[6], o[7]);
+          }
+          fence_async_smem();  // the MMAs read what was written here
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&cfull[cs]);
+            mbar_arrive(&empty[stage]);
+          }
+          cphase ^= 1;
         }
-        fence_async_smem();  // the MMAs read what was written here
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&cfull[cs]);
-          mbar_arrive(&empty[stage]);
-        }
+        turn = turn + 1 == kDaConv ? 0 : turn + 1;
         if (++stage == kDaStages) { stage = 0; phase ^= 1; }
-        if (++cs == kDaConv) { cs = 0; cphase ^= 1; }
       }
     }
   } else if (warp < 4) {
@@ -881,7 +897,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_q8_da(const __grid_constant__
     const uint32_t give = su32(sums) + uint32_t(warp) * 4096u, take = su32(sums) + uint32_t(warp ^ 2) * 4096u;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int round = 0; round * int(gridDim.x) < n_items; ++round) {
+      const int item = da_deal(round, n_items);
+      if (item < 0) break;
       SavedItem it;
       if (!da_item(p, item, it)) continue;
       // both warps of a pair must agree to go on before they meet at a barrier
