@@ -132,7 +132,8 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
 // One 32 x 32 slice of finished values (lane = row row_w0 + lane, columns n..)
 // to the output.  Warp-collective.
 __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&f)[32], int64_t row_w0, int n,
-                                               uint32_t buf, int lane) {
+                                               uint32_t obuf, uint32_t slice, int lane) {
+  const uint32_t buf = obuf + (slice & 1u) * 2048u;  // the warp's 4 KB hold two slices of 16-bit values
   const bool f16 = p.dtype == MLORA_F16;
   if (p.tma_out) {
     if (lane == 0) bulk_wait_read_1();  // the store issued from this buffer two slices ago
@@ -160,7 +161,7 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
   if (p.dtype == MLORA_F32) {
     // through shared memory (the warp's whole 4 KB): a warp writes 128
     // neighbouring bytes of one row at a time, at any alignment
-    const uint32_t base = buf & ~4095u;
+    const uint32_t base = obuf;
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -171,14 +172,16 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
     if (!p.out_rows) {  // consecutive rows
       float* dst = out + row_w0 * p.N + n + lane;
       const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
+      float v[32];  // all reads first: their latency is paid once
 #pragma unroll
       for (int r = 0; r < 32; ++r) {
         const uint32_t a = base + uint32_t(r) * 128u + (((uint32_t(lane) >> 2) ^ (uint32_t(r) & 7u)) << 4) +
                            (uint32_t(lane) & 3u) * 4u;
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-        if (r < live) dst[int64_t(r) * p.N] = v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[r]) : "r"(a));
       }
+#pragma unroll
+      for (int r = 0; r < 32; ++r)
+        if (r < live) dst[int64_t(r) * p.N] = v[r];
       return;
     }
 #pragma unroll 8
@@ -210,14 +213,16 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
   if (!p.out_rows) {  // consecutive rows
     uint16_t* dst = reinterpret_cast<uint16_t*>(out) + row_w0 * p.N + n + lane;
     const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
+    uint16_t v[32];  // all reads first: their latency is paid once
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
       const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
                          (uint32_t(lane) & 7u) * 2u;
-      uint16_t v;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-      if (r < live) dst[int64_t(r) * p.N] = v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[r]) : "r"(a));
     }
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (r < live) dst[int64_t(r) * p.N] = v[r];
     return;
   }
 #pragma unroll 8
@@ -508,8 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
             f[4 * q] += s.x; f[4 * q + 1] += s.y; f[4 * q + 2] += s.z; f[4 * q + 3] += s.w;
           }
         }
-        q8_store_slice(p, f, row_w0, n0 + col, obuf + (slices & 1u) * 2048u, lane);
-        ++slices;
+        q8_store_slice(p, f, row_w0, n0 + col, obuf, slices++, lane);
       }
       tc_fence_before();
       __syncwarp();
