@@ -176,6 +176,14 @@ int check_q8(std::initializer_list<const void*> mats, std::initializer_list<cons
 // cores, whatever their size, unless the call asks for the CUDA cores.
 int q8_main(const Q8Main& a, int impl, Q8After after, cudaStream_t st) {
   if (impl != MLORA_IMPL_SIMT && q8_few_ok(a)) return q8_main_few(a, after, st);
+  if (impl != MLORA_IMPL_SIMT && a.expand && a.dtype == MLORA_F32 && tc_available()) {
+    // float32: the expand is not a tensor-core operand; it is added after
+    Q8Main product = a;
+    product.expand = false;
+    const int s = q8_main_tc(product, after, st);
+    return s != MLORA_OK ? s : simt_expand_add32(a.bwd, a.plan, (const float*)a.pack, (const float*)a.zt,
+                                                 (float*)a.out, a.out_rows, a.M, a.d_in, a.d_out, a.R, st);
+  }
   const bool tc = impl != MLORA_IMPL_SIMT && q8_tc_ok(a);
   return tc ? q8_main_tc(a, after, st) : q8_main_simt(a, st);
 }
@@ -315,6 +323,12 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     if (st != MLORA_OK || !q8_base) return st;
     return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
   }
+  if (q8_base && prob->dtype == MLORA_F32) {
+    st = q8_low32(false, dev, (const float*)X, (const float*)A_pack, (float*)zsave, prob->rows, prob->d_in,
+                  prob->d_out, route->r_pack, s);
+    if (st != MLORA_OK) return st;
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
+  }
   SimtCall a;
   a.plan = dev;
   a.n_chunks = dev.n_chunks;
@@ -436,13 +450,21 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
   const bool q8_dx = dX && q8->Wq && (stages & MLORA_BWD_DX);
   const bool saved8 = q8->Xq != nullptr;
   const int32_t reduce = MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B;
-  if (!q8_dx && !saved8)
+  if (!q8_dx && !saved8 && prob->dtype != MLORA_F32)
     return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack,
                             dB_pack, stages, 0, p.n_tiles, 0, nb_out, nullptr, s);
   // dZ (and the 16-bit dX), then the 8-bit dX, then the reductions
-  int st = backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave,
-                            q8_dx ? nullptr : dX, dA_pack, dB_pack, stages & ~reduce, 0, p.n_tiles, 0, nb_out,
-                            saved8 && dA_pack ? q8 : nullptr, s);
+  const bool f32 = prob->dtype == MLORA_F32;
+  int32_t first = stages & ~reduce;
+  int st = MLORA_OK;
+  if (f32 && (first & MLORA_BWD_DZ)) {
+    st = q8_low32(true, dev, (const float*)dY, (const float*)B_pack, (float*)dzsave, prob->rows, prob->d_in,
+                  prob->d_out, route->r_pack, s);
+    if (st != MLORA_OK) return st;
+    first &= ~MLORA_BWD_DZ;
+  }
+  st = backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, q8_dx ? nullptr : dX,
+                        dA_pack, dB_pack, first, 0, p.n_tiles, 0, nb_out, saved8 && dA_pack ? q8 : nullptr, s);
   if (st != MLORA_OK) return st;
   if (q8_dx) {
     st = q8_quantize(dY, prob->rows, prob->d_out, prob->d_out, prob->dtype, q8->w_scale, q8->Gq, q8->g_scale, s);
@@ -459,6 +481,18 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     m.err = prob->err_word;
     st = q8_main(m, q8_impl(prob, impl), kAfterRows, s);
     if (st != MLORA_OK) return st;
+  }
+  if (f32) {
+    if (dA_pack && (stages & MLORA_BWD_DA)) {
+      float* upd = (stages & MLORA_BWD_SGD_A) ? (float*)const_cast<void*>(A_pack) : nullptr;
+      st = q8_sum32(0, dev, q8->Xq, q8->x_scale, (const float*)X, (const float*)dzsave, (float*)dA_pack, prob->rows,
+                    prob->d_in, prob->d_in, upd, prob->lr, s);
+      if (st != MLORA_OK) return st;
+    }
+    if (!dB_pack || !(stages & MLORA_BWD_DB)) return MLORA_OK;
+    float* upd = (stages & MLORA_BWD_SGD_B) ? (float*)const_cast<void*>(B_pack) : nullptr;
+    return q8_sum32(1, dev, nullptr, nullptr, (const float*)dY, (const float*)zsave, (float*)dB_pack, prob->rows,
+                    prob->d_out, route->r_pack, upd, prob->lr, s);
   }
   if (!saved8)
     return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, nullptr, dA_pack,

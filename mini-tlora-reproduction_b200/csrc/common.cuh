@@ -31,7 +31,7 @@ struct Chunk {
   int32_t pcol;   // packed rank column / row of the first entry of this chunk
   int32_t j;      // chunk index inside the adapter
   float scale;    // s_a
-  int32_t seg;    // segment index
+  int32_t nr;     // ranks of the adapter in this chunk (<= 64)
 };
 static_assert(sizeof(Chunk) == 32, "Chunk is 32 bytes");
 

@@ -82,7 +82,7 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
         c.pcol = r->pack_off[a] + j * kChunk;
         c.j = j;
         c.scale = r->scaling[a];
-        c.seg = q;
+        c.nr = std::min(kChunk, r->rank[a] - j * kChunk);
         p->chunks.push_back(c);
       }
     }

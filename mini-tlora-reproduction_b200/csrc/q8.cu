@@ -546,6 +546,155 @@ __global__ void __launch_bounds__(NT) k_q8_main(Q8Main a) {
   }
 }
 
+// ---------------------------------------------------------------- float32 layers
+// The low-rank terms of float32 layers stay on the CUDA cores, next to the
+// 8-bit product on the tensor cores.
+//
+// k_low32: Zt[c] = mask(s_a src A_chunk^T) (forward; K = d_in, a pack row is
+// contiguous in k) or dZt[c] = mask(s_a src B_chunk) (backward; K = d_out, a
+// pack row holds the ranks of one k).  A block takes kLowRows rows of one
+// chunk and its eight warps share out K; lane l sums ranks l and l + 32, the
+// warps' sums are added in their order.  Ranks past the adapter's are zero
+// without being computed.
+constexpr int kLowRows = 8, kLowWarps = 8, kLowStep = 32;
+
+template <bool BWD>
+__global__ void __launch_bounds__(kLowWarps * 32) k_low32(PlanDev plan, const float* __restrict__ src,
+                                                          const float* __restrict__ pack, float* __restrict__ zt,
+                                                          int64_t M, int K, int64_t ldp) {
+  __shared__ float xs[kLowWarps][kLowRows][kLowStep];
+  // forward: 32 k x 32 ranks of A per warp; then the warps' sums
+  __shared__ float work[kLowWarps * 32 * 33];
+  static_assert(sizeof(work) >= sizeof(float) * kLowWarps * kLowRows * kChunk, "the sums fit the pack's space");
+  const int c = blockIdx.x, r0 = blockIdx.y * kLowRows;
+  const Chunk ch = plan.chunks[c];
+  float* out = zt + int64_t(c) * kTileRows * kChunk;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t row0 = int64_t(ch.tile) * kTileRows + r0;
+  float (*as)[33] = reinterpret_cast<float (*)[33]>(work + warp * 32 * 33);
+  float acc[2][kLowRows] = {};
+  if (ch.lo < r0 + kLowRows && ch.hi > r0) {
+    for (int k0 = warp * kLowStep; k0 < K; k0 += kLowWarps * kLowStep) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kLowRows; ++i)
+        xs[warp][i][lane] = row0 + i < M && k0 + lane < K ? src[(row0 + i) * K + k0 + lane] : 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = ch.nr - 32 * h;  // ranks of this half
+        if (n <= 0) continue;
+        float b[kLowStep];  // backward: this lane's rank of B, all k of the step
+        if (!BWD) {
+          __syncwarp();
+#pragma unroll 8
+          for (int j = 0; j < 32; ++j)
+            as[lane][j] = j < n && k0 + lane < K ? __ldg(pack + (ch.pcol + 32 * h + j) * ldp + k0 + lane) : 0.f;
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < kLowStep; ++kk)
+            b[kk] = lane < n && k0 + kk < K ? __ldg(pack + int64_t(k0 + kk) * ldp + ch.pcol + 32 * h + lane) : 0.f;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int kk = 0; kk < kLowStep; ++kk) {
+          const float a = BWD ? b[kk] : as[kk][lane];
+#pragma unroll
+          for (int i = 0; i < kLowRows; ++i) acc[h][i] = fmaf(xs[warp][i][kk], a, acc[h][i]);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  float (*sums)[kLowRows][kChunk] = reinterpret_cast<float (*)[kLowRows][kChunk]>(work);
+#pragma unroll
+  for (int i = 0; i < kLowRows; ++i) {
+    sums[warp][i][lane] = acc[0][i];
+    sums[warp][i][lane + 32] = acc[1][i];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < kLowRows * kChunk; e += kLowWarps * 32) {
+    const int i = e / kChunk, j = e % kChunk, r = r0 + i;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kLowWarps; ++w) s += sums[w][i][j];
+    out[r * kChunk + j] = r >= ch.lo && r < ch.hi ? ch.scale * s : 0.f;
+  }
+}
+
+// k_sum32: one 64-column block of d_in of dA (KIND 0; SRC8: from the saved 8-bit
+// rows) or of d_out of dB (KIND 1) for one adapter and 16 of its ranks:
+//   dA[r, col] = sum_i dZt[i, r] x[i, col],   dB[col, r] = sum_i Zt[i, r] dY[i, col].
+// The eight warps share out the rows of each tile, lane l holds columns 2 l and
+// 2 l + 1; their sums are added in order.  Only rows of the adapter's segments
+// are read.
+constexpr int kSumRanks = 16, kSumCols = 64;
+template <int KIND, bool SRC8>
+__global__ void __launch_bounds__(256) k_sum32(PlanDev plan, const int8_t* __restrict__ Xq,
+                                               const float* __restrict__ x_scale, const float* __restrict__ src,
+                                               const float* __restrict__ zt, float* __restrict__ out, int64_t M,
+                                               int D, int64_t ldo, float* upd, float lr) {
+  __shared__ float sums[8][kSumRanks][kSumCols];
+  const ReduceItem it = plan.reduce[blockIdx.x];
+  if (it.kind != KIND) return;
+  const int j = it.j0 + int(blockIdx.y) / 4, jr = (int(blockIdx.y) % 4) * kSumRanks;  // chunk, first rank in it
+  if (int(blockIdx.y) / 4 >= it.nc || j * kChunk + jr >= it.rank) return;
+  const int c0 = it.block * 128 + int(blockIdx.z) * kSumCols;
+  if (c0 >= D) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = c0 + 2 * lane;
+  const int64_t ldq = q8_ld(D);
+  float acc[kSumRanks][2] = {};
+  for (int e = it.lb; e < it.le; ++e) {
+    const int c = plan.list[e] + j;
+    const Chunk ch = plan.chunks[c];
+    const float* z = zt + int64_t(c) * kTileRows * kChunk + jr;
+    const int64_t row0 = int64_t(ch.tile) * kTileRows;
+#pragma unroll 4
+    for (int r = ch.lo + warp; r < ch.hi; r += 8) {
+      const int64_t row = row0 + r;
+      float x0, x1;
+      if (SRC8) {
+        const char2 q = col < ldq ? *reinterpret_cast<const char2*>(Xq + row * ldq + col) : make_char2(0, 0);
+        const float s = __ldg(x_scale + row);
+        x0 = float(q.x) * s;
+        x1 = float(q.y) * s;
+      } else {
+        x0 = col < D ? src[row * D + col] : 0.f;
+        x1 = col + 1 < D ? src[row * D + col + 1] : 0.f;
+      }
+      const float4* z4 = reinterpret_cast<const float4*>(z + r * kChunk);
+#pragma unroll
+      for (int g = 0; g < kSumRanks / 4; ++g) {
+        const float4 w = __ldg(z4 + g);
+        const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          acc[4 * g + k][0] = fmaf(v[k], x0, acc[4 * g + k][0]);
+          acc[4 * g + k][1] = fmaf(v[k], x1, acc[4 * g + k][1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSumRanks; ++k) {
+    sums[warp][k][2 * lane] = acc[k][0];
+    sums[warp][k][2 * lane + 1] = acc[k][1];
+  }
+  __syncthreads();
+  const int pcol = plan.chunks[plan.list[it.lb] + j].pcol + jr;
+  const int live = it.rank - j * kChunk - jr;
+  for (int e = threadIdx.x; e < kSumRanks * kSumCols; e += 256) {
+    // consecutive threads: consecutive elements of the output
+    const int k = KIND == 0 ? e / kSumCols : e % kSumRanks, x = KIND == 0 ? e % kSumCols : e / kSumRanks;
+    if (k >= live || c0 + x >= D) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][k][x];
+    const int64_t o = KIND == 0 ? int64_t(pcol + k) * ldo + c0 + x : int64_t(c0 + x) * ldo + pcol + k;
+    out[o] = s;
+    if (upd) sgd_apply(upd + o, s, lr);  // fused SGD step
+  }
+}
+
 template <class T>
 int launch_q8_main(const Q8Main& a, cudaStream_t st) {
   const int N = a.bwd ? a.d_in : a.d_out;
@@ -572,6 +721,27 @@ int q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64_t col
   if (dtype == MLORA_BF16) return dequantize_t<__nv_bfloat16>(q, scale, rows, cols, dst, st);
   if (dtype == MLORA_F16) return dequantize_t<__half>(q, scale, rows, cols, dst, st);
   return dequantize_t<float>(q, scale, rows, cols, dst, st);
+}
+
+int q8_low32(bool bwd, const PlanDev& plan, const float* src, const float* pack, float* zt, int64_t M, int d_in,
+             int d_out, int R, cudaStream_t st) {
+  if (plan.n_chunks == 0) return MLORA_OK;
+  const dim3 grid(plan.n_chunks, kTileRows / kLowRows);
+  if (bwd) k_low32<true><<<grid, kLowWarps * 32, 0, st>>>(plan, src, pack, zt, M, d_out, R);
+  else k_low32<false><<<grid, kLowWarps * 32, 0, st>>>(plan, src, pack, zt, M, d_in, d_in);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
+}
+
+int q8_sum32(int kind, const PlanDev& plan, const int8_t* Xq, const float* x_scale, const float* src, const float* zt,
+             float* out, int64_t M, int D, int64_t ldo, float* upd, float lr, cudaStream_t st) {
+  if (plan.n_reduce == 0) return MLORA_OK;
+  const dim3 grid(plan.n_reduce, 4 * kMaxChunksPerItem, 128 / kSumCols);
+  if (kind == 1) k_sum32<1, false><<<grid, 256, 0, st>>>(plan, nullptr, nullptr, src, zt, out, M, D, ldo, upd, lr);
+  else if (Xq) k_sum32<0, true><<<grid, 256, 0, st>>>(plan, Xq, x_scale, nullptr, zt, out, M, D, ldo, upd, lr);
+  else k_sum32<0, false><<<grid, 256, 0, st>>>(plan, nullptr, nullptr, src, zt, out, M, D, ldo, upd, lr);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
 
 int q8_main_simt(const Q8Main& a, cudaStream_t st) {

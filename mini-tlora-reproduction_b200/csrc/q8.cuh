@@ -78,6 +78,14 @@ int q8_main_few(const Q8Main& a, Q8After after, cudaStream_t st);
 int q8_few_prep(const void* X, int64_t rows, int d_in, int dtype, int8_t* Xq, float* x_scale, const PlanDev& plan,
                 const void* A_pack, void* zt, cudaStream_t st);
 
+// float32 layers: the low-rank intermediate of all tiles (forward or backward),
+// and dA (kind 0, from the saved 8-bit rows Xq or from src = X) or dB (kind 1,
+// src = dY).
+int q8_low32(bool bwd, const PlanDev& plan, const float* src, const float* pack, float* zt, int64_t M, int d_in,
+             int d_out, int R, cudaStream_t st);
+int q8_sum32(int kind, const PlanDev& plan, const int8_t* Xq, const float* x_scale, const float* src, const float* zt,
+             float* out, int64_t M, int D, int64_t ldo, float* upd, float lr, cudaStream_t st);
+
 int q8_main_simt(const Q8Main& a, cudaStream_t st);
 bool q8_tc_ok(const Q8Main& a);
 int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st);

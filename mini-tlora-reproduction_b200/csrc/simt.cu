@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(NT) k_main(PlanDev plan, const T* __restrict__
                                               const T* __restrict__ W, const T* __restrict__ bias,
                                               const T* __restrict__ pack, const T* __restrict__ zt,
                                               T* __restrict__ out, const int32_t* __restrict__ out_rows,
-                                              int64_t M, int d_in, int d_out, int R, int t0, int no_expand) {
+                                              int64_t M, int d_in, int d_out, int R, int t0, int no_expand, int add) {
   __shared__ float As[BK][LD], Bs[BK][LD];
   const int n0 = blockIdx.x * BN;
   const int64_t m0 = int64_t(t0) * kTileRows + int64_t(blockIdx.y) * BM;
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(NT) k_main(PlanDev plan, const T* __restrict__
       if (n >= N) continue;
       float v = acc[i][j];
       if (!BWD && bias) v += to_f(bias[n]);
+      if (add) v += to_f(out[orow * N + n]);  // onto a product already there
       out[orow * N + n] = from_f<T>(v);
     }
   }
@@ -263,7 +264,7 @@ int launch_forward(const SimtCall& a, cudaStream_t st) {
     const int no_expand = (a.stages & MLORA_STAGE_NO_EXPAND) ? 1 : 0;
     k_main<T, false><<<grid, NT, 0, st>>>(a.plan, (const T*)a.X, (const T*)a.W, (const T*)a.bias,
                                           (const T*)a.B_pack, (const T*)a.zsave, (T*)a.Y, a.out_rows,
-                                          a.M, a.d_in, a.d_out, a.R, a.t0, no_expand);
+                                          a.M, a.d_in, a.d_out, a.R, a.t0, no_expand, 0);
     count_launch();
   }
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
@@ -280,7 +281,7 @@ int launch_backward(const SimtCall& a, cudaStream_t st) {
     dim3 grid((a.d_in + BN - 1) / BN, unsigned((a.M + BM - 1) / BM));
     k_main<T, true><<<grid, NT, 0, st>>>(a.plan, (const T*)a.dY, (const T*)a.W, nullptr,
                                          (const T*)a.A_pack, (const T*)a.dzt, (T*)a.dX, a.out_rows,
-                                         a.M, a.d_in, a.d_out, a.R, 0, 0);
+                                         a.M, a.d_in, a.d_out, a.R, 0, 0, 0);
     count_launch();
   }
   void* dA = (a.bwd_stages & MLORA_BWD_DA) ? a.dA : nullptr;
@@ -327,6 +328,19 @@ int simt_backward(const SimtCall& a, cudaStream_t st) {
   if (a.dtype == MLORA_BF16) return launch_backward<__nv_bfloat16>(a, st);
   if (a.dtype == MLORA_F16) return launch_backward<__half>(a, st);
   return launch_backward<float>(a, st);
+}
+
+int simt_expand_add32(bool bwd, const PlanDev& plan, const float* pack, const float* zt, float* out,
+                      const int32_t* out_rows, int64_t M, int d_in, int d_out, int R, cudaStream_t st) {
+  const dim3 grid(unsigned(((bwd ? d_in : d_out) + BN - 1) / BN), unsigned((M + BM - 1) / BM));
+  if (bwd)
+    k_main<float, true><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in, d_out,
+                                             R, 0, 0, 1);
+  else
+    k_main<float, false><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in,
+                                              d_out, R, 0, 0, 1);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
 
 int sgd_items(int dtype, const mlora_sgd_item* items, int n, float lr, cudaStream_t st) {

@@ -33,6 +33,9 @@ struct SimtCall {
 
 int simt_forward(const SimtCall& a, cudaStream_t st);
 int simt_backward(const SimtCall& a, cudaStream_t st);
+// out += the LoRA expand of all rows (float32)
+int simt_expand_add32(bool bwd, const PlanDev& plan, const float* pack, const float* zt, float* out,
+                      const int32_t* out_rows, int64_t M, int d_in, int d_out, int R, cudaStream_t st);
 int sgd_items(int dtype, const mlora_sgd_item* items, int n, float lr, cudaStream_t st);
 
 }  // namespace mlora

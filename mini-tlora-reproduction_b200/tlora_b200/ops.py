@@ -73,6 +73,7 @@ class AdapterTable:
     pack_off: np.ndarray  # int32 [n]
     r_pack: int
     _dev_keys: dict = field(default_factory=dict, repr=False)
+    _spans: Optional[list] = field(default=None, repr=False)
 
     @staticmethod
     def build(ids: Sequence[int], ranks: Sequence[int]) -> "AdapterTable":
@@ -86,6 +87,12 @@ class AdapterTable:
     @property
     def n(self) -> int:
         return len(self.ids)
+
+    def spans(self) -> list:
+        """(first packed row, rank) of every slot, as plain integers."""
+        if self._spans is None:
+            self._spans = [(int(o), int(r)) for o, r in zip(self.pack_off, self.rank)]
+        return self._spans
 
     def slot_of(self) -> dict:
         return {a: i for i, a in enumerate(self.ids)}
@@ -267,12 +274,16 @@ def q8_ld(cols: int) -> int:
     return (int(cols) + 15) // 16 * 16
 
 
-def _new_rows8(rows: int, cols: int, device) -> Int8Rows:
-    r = Int8Rows.__new__(Int8Rows)  # the layout is right by construction
-    r.q = torch.empty((rows, q8_ld(cols)), dtype=torch.int8, device=device)
-    r.scale = torch.empty(rows, dtype=torch.float32, device=device)
-    r.cols = cols
+def _wrap8(q: torch.Tensor, scale: torch.Tensor, cols: int) -> Int8Rows:
+    """Int8Rows of tensors made here: the layout is right by construction."""
+    r = Int8Rows.__new__(Int8Rows)
+    r.q, r.scale, r.cols = q, scale, cols
     return r
+
+
+def _new_rows8(rows: int, cols: int, device) -> Int8Rows:
+    return _wrap8(torch.empty((rows, q8_ld(cols)), dtype=torch.int8, device=device),
+                  torch.empty(rows, dtype=torch.float32, device=device), cols)
 
 
 class _Scratch8:
@@ -798,19 +809,17 @@ class MultiLoRAFunction(torch.autograd.Function):
     def backward(ctx, dy):
         xs, z, W, _, _, *kept = ctx.saved_tensors
         st: LayerState = ctx.st
-        rows8 = Int8Rows(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
-        n = st.table.n
+        rows8 = _wrap8(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
         need = ctx.needs_input_grad
-        want_dx = need[0]
-        want_A = any(need[4 + 2 * i] for i in range(n))
-        want_B = any(need[5 + 2 * i] for i in range(n))
-        dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, want_dx, want_A, want_B, rows8)
-        grads = []
-        for i in range(n):
-            o, r = int(st.table.pack_off[i]), int(st.table.rank[i])
-            act = bool(st.plan.active[i])
-            grads.append(dA[o:o + r] if (act and dA is not None and need[4 + 2 * i]) else None)
-            grads.append(dB[:, o:o + r] if (act and dB is not None and need[5 + 2 * i]) else None)
+        dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
+        grads = [None] * (2 * st.table.n)
+        for i, ((o, r), act) in enumerate(zip(st.table.spans(), st.plan.active.tolist())):
+            if not act:
+                continue
+            if need[4 + 2 * i]:
+                grads[2 * i] = dA.narrow(0, o, r)
+            if need[5 + 2 * i]:
+                grads[2 * i + 1] = dB.narrow(1, o, r)
         return (dx, None, None, None, *grads)
 
 
