@@ -102,8 +102,9 @@ int upload_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
 }
 
 // Device view of a plan already in the workspace (MLORA_PLAN_RESIDENT): no
-// copy; the per-launch work counters are reset on the stream.
-int view_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
+// copy; the per-launch work counters are reset on the stream, if the call has
+// kernels that use them.
+int view_plan(const Plan& p, void* ws, bool counters, cudaStream_t st, PlanDev* dev) {
   uint8_t* b = (uint8_t*)ws;
   std::memset(dev, 0, sizeof(*dev));
   dev->n_tiles = p.n_tiles;
@@ -121,14 +122,16 @@ int view_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
   dev->n_saved = int32_t(p.saved.size());
   dev->saved = (const SavedItem*)(b + p.off_saved);
   dev->saved_done = dev->counters + 16;
-  MLORA_CUDA_TRY(cudaMemsetAsync(dev->counters, 0, p.bytes - p.off_counters, st));
+  if (counters) MLORA_CUDA_TRY(cudaMemsetAsync(dev->counters, 0, p.bytes - p.off_counters, st));
   return MLORA_OK;
 }
 
 // Plan of a call: uploaded now, or already resident in the workspace; the
 // kernels report their device-side checks into the call's status word.
-int stage_plan(const mlora_problem* prob, const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
-  const int s = (prob->flags & MLORA_PLAN_RESIDENT) ? view_plan(p, ws, st, dev) : upload_plan(p, ws, st, dev);
+int stage_plan(const mlora_problem* prob, const Plan& p, void* ws, cudaStream_t st, PlanDev* dev,
+               bool counters = true) {
+  const int s =
+      (prob->flags & MLORA_PLAN_RESIDENT) ? view_plan(p, ws, counters, st, dev) : upload_plan(p, ws, st, dev);
   dev->err = prob->err_word;
   return s;
 }
@@ -281,15 +284,15 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   const int impl = choose_impl(prob, {X, W, bias, A_pack, B_pack, Y, zsave});
   if (impl < 0) return MLORA_ERR_UNSUPPORTED;
   if (ar && (impl != MLORA_IMPL_TC || route->out_rows)) return MLORA_ERR_UNSUPPORTED;
-  cudaStream_t s = (cudaStream_t)stream;
-  PlanDev dev;
-  st = stage_plan(prob, p, workspace, s, &dev);
-  if (st != MLORA_OK) return st;
   const bool q8_base = q8 && q8->Wq;
   const int32_t all_stages = stages;
   // a few rows in 16 bits: rows and shrink in one launch
-  const bool few = q8_base && impl == MLORA_IMPL_TC && prob->rows <= kQ8Few && dev.n_chunks > 0 &&
+  const bool few = q8_base && impl == MLORA_IMPL_TC && prob->rows <= kQ8Few && !p.chunks.empty() &&
                    (stages & MLORA_STAGE_SHRINK);
+  cudaStream_t s = (cudaStream_t)stream;
+  PlanDev dev;
+  st = stage_plan(prob, p, workspace, s, &dev, !few);
+  if (st != MLORA_OK) return st;
   // the launch that the 8-bit product follows
   const Q8After after = few || dev.n_chunks == 0 ? kAfterRows : impl == MLORA_IMPL_TC ? kAfterShrink : kAfterOther;
   if (few) {

@@ -316,10 +316,12 @@ def _check_cuda(t: torch.Tensor, what: str) -> None:
 def _row_major(x: torch.Tensor):
     """(x, elements between rows): rows with unit column stride are read in
     place, anything else is copied."""
-    if x.shape[0] <= 1 or x.shape[1] <= 1 or x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        x = x.contiguous()
+    if x.is_contiguous():
         return x, x.shape[1]
-    return x, x.stride(0)
+    ld, one = x.stride()
+    if x.shape[0] <= 1 or x.shape[1] <= 1 or one != 1 or ld < x.shape[1]:
+        return x.contiguous(), x.shape[1]
+    return x, ld
 
 
 def quantize_rows(x: torch.Tensor, col_scale: Optional[torch.Tensor] = None) -> Int8Rows:
@@ -365,7 +367,7 @@ class Int8LinearFunction(torch.autograd.Function):
     def forward(ctx, x, wq, w_scale, bias, d_in):
         ctx.save_for_backward(wq, w_scale)
         ctx.d_in = d_in
-        return _int8_product(x, Int8Rows(wq, w_scale, d_in), bias, x.dtype)
+        return _int8_product(x, _wrap8(wq, w_scale, d_in), bias, x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
@@ -383,18 +385,22 @@ class Int8LinearFunction(torch.autograd.Function):
 
 
 def _int8_product(x, weight: Int8Rows, bias, dtype):
-    dev = weight.device
-    with _on(dev):
-        if isinstance(x, Int8Rows):
-            x8, src, ld = x, None, 0
-        else:
-            src, ld = _row_major(x.detach())
-            x8 = _Scratch8(x.shape[0], x.shape[1], dev)
-        rows, (d_out, d_in) = x.shape[0], weight.shape
-        y = torch.empty((rows, d_out), dtype=dtype, device=dev)
-        prob = _lib.Problem(rows, d_in, d_out, mlora_dtype(dtype), _lib.IMPL_AUTO)
-        _lib.call("mlora_q8_linear", ctypes.byref(prob), _ptr(src), ld, *_ptrs8(x8), _ptr(weight.q),
-                  _ptr(weight.scale), _ptr(bias), _ptr(y), _stream(dev))
+    q = weight.q
+    dev = q.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _int8_product(x, weight, bias, dtype)
+    rows, d_in, d_out = x.shape[0], weight.cols, q.shape[0]
+    if isinstance(x, Int8Rows):
+        src, ld, (xq, xs) = None, 0, _ptrs8(x)
+    else:
+        src, ld = _row_major(x.detach() if x.requires_grad else x)
+        kept = _Scratch8(rows, d_in, dev)  # noqa: F841  (alive until the launch)
+        src, (xq, xs) = src.data_ptr(), kept.ptrs
+    y = torch.empty((rows, d_out), dtype=dtype, device=dev)
+    prob = _lib.Problem(rows, d_in, d_out, _DTYPES[dtype], _lib.IMPL_AUTO)
+    _lib.call("mlora_q8_linear", ctypes.byref(prob), src, ld, xq, xs, q.data_ptr(), weight.scale.data_ptr(),
+              _ptr(bias), y.data_ptr(), _stream(dev))
     return y
 
 
@@ -411,14 +417,16 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
     frozen, like the backbone of ``MultiLoRALinear``."""
     if not isinstance(weight, Int8Rows):
         raise TypeError("int8_linear expects weight as Int8Rows (quantize_rows(W))")
+    dev = weight.q.device
+    if dev.type != "cuda":
+        _check_cuda(weight.q, "int8_linear")
     eight = isinstance(x, Int8Rows)
-    _check_cuda(weight.q, "int8_linear")
     if not eight and x.dim() != 2:
         raise ValueError("int8_linear expects x shaped [rows, in_features]")
     if x.shape[1] != weight.cols:
         raise ValueError(f"x has {x.shape[1]} features, the weight {weight.cols}")
-    if x.device != weight.device:
-        raise RuntimeError(f"input on {x.device} but weight on {weight.device}")
+    if x.device != dev:
+        raise RuntimeError(f"input on {x.device} but weight on {dev}")
     if not eight:
         if dtype is not None and dtype != x.dtype:
             raise ValueError("dtype applies to 8-bit input; a tensor's product has its own type")
@@ -428,15 +436,17 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
             raise ValueError("int8_linear of 8-bit rows needs the type of y (dtype or bias)")
         dtype = bias.dtype
     mlora_dtype(dtype)
+    grad = torch.is_grad_enabled()
     if bias is not None:
-        if bias.shape != (weight.rows,) or bias.dtype != dtype or bias.device != weight.device:
+        if bias.dtype != dtype or bias.dim() != 1 or bias.shape[0] != weight.q.shape[0] or bias.device != dev:
             raise ValueError("bias must be a vector of y's type on the weight's device, one element per output")
-        if bias.requires_grad and torch.is_grad_enabled():
+        if grad and bias.requires_grad:
             raise NotImplementedError("the 8-bit linear is frozen: no gradient of its bias")
-        bias = bias.contiguous()
-    if eight or not (x.requires_grad and torch.is_grad_enabled()):
-        return _int8_product(x, weight, bias, dtype)
-    return Int8LinearFunction.apply(x, weight.q, weight.scale, bias, weight.cols)
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    if grad and not eight and x.requires_grad:
+        return Int8LinearFunction.apply(x, weight.q, weight.scale, bias, weight.cols)
+    return _int8_product(x, weight, bias, dtype)
 
 
 # ---------------------------------------------------------------------------
