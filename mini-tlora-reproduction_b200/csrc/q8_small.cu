@@ -4,9 +4,9 @@
 //   Y[i, j] = s_x[i] s_w[j] sum_k Xq[i, k] Wq[j, k] + bias[j] + sum_c Zt[c][i, :] B_pack[j, chunk c]
 //
 // k_q8_few: a block owns 16 output channels and its eight warps share out K in
-// 128-byte pieces.  A lane's 16-byte loads go straight to registers, four
-// pieces (64 KB a block) in flight at once, and are the A operand of
-// mma.m16n8k32 as they come: the sum over k does not depend on the order of k,
+// 128-byte pieces.  A lane's 16-byte loads go straight to registers, two
+// pieces (32 KB a block, four blocks an SM) in flight at once, and are the A
+// operand of mma.m16n8k32 as they come: the sum over k does not depend on the order of k,
 // so the eight tokens of a B operand are read at the same offsets and no data
 // is rearranged.  (A 128-row tensor-memory tile would spend 15/16 of its rows
 // on nothing, and the tensor pipe is idle either way: HBM feeds a block less
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kFewThreads = 256, kFewWarps = 8;
 constexpr int kFewCh = 16;     // output channels (k_q8_few) or ranks (k_few_prep) of a block
-constexpr int kFewPieces = 4;  // pieces of K a warp has in flight
+constexpr int kFewPieces = 2;  // pieces of K a warp has in flight
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -74,7 +74,7 @@ __device__ __forceinline__ uint4 ldg_stream(const void* p) {  // read once: leav
 
 // NT = 8-token groups (rows <= 8 NT)
 template <class T, int NT>
-__global__ void __launch_bounds__(kFewThreads) k_q8_few(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(kFewThreads, 4) k_q8_few(const __grid_constant__ FewParams p) {
   __shared__ int sums[kFewWarps][kFewCh][8 * NT + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
   const int n0 = blockIdx.x * kFewCh;
