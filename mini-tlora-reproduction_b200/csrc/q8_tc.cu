@@ -33,8 +33,14 @@ constexpr int kDefer = 8;       // k-blocks of the next tile before a tile's exp
 constexpr int kQ8K = 128;       // bytes of K per k-block
 constexpr int kQ8Stages = 6;    // 32 KB per CTA each
 constexpr int kQ8StageBytes = 32 * 1024;
-constexpr int kQ8ColBytes = 4 * 2 * 256 * 4;  // column scales and biases of a tile, per epilogue warp
-constexpr int kQ8Smem = kQ8Stages * kQ8StageBytes + kStageOut2Bytes + kQ8ColBytes + 1024 + 512;
+// Warps: 0 and 6 issue TMA loads, 1 the MMAs, 2..5 drain columns 0..127 of a
+// tile and 8..11 columns 128..255 (a warp reaches the quarter of the TMEM lanes
+// that its number modulo four names), 7 has no part.
+constexpr int kQ8Threads = 32 * 12;
+constexpr int kQ8EpiWarps = 8, kQ8EpiCols = 128;
+constexpr int kQ8OutBytes = kQ8EpiWarps * 2048;               // a 32 x 32 slice of 16-bit values per warp
+constexpr int kQ8ColBytes = kQ8EpiWarps * 2 * kQ8EpiCols * 4;  // column scales and biases, per warp
+constexpr int kQ8Smem = kQ8Stages * kQ8StageBytes + kQ8OutBytes + kQ8ColBytes + 1024 + 512;
 static_assert(kQ8Smem <= 232448, "dynamic shared memory above 227 KB");
 
 struct Q8Params {
@@ -132,11 +138,10 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
 // One 32 x 32 slice of finished values (lane = row row_w0 + lane, columns n..)
 // to the output.  Warp-collective.
 __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&f)[32], int64_t row_w0, int n,
-                                               uint32_t obuf, uint32_t slice, int lane) {
-  const uint32_t buf = obuf + (slice & 1u) * 2048u;  // the warp's 4 KB hold two slices of 16-bit values
+                                               uint32_t buf, int lane) {
   const bool f16 = p.dtype == MLORA_F16;
   if (p.tma_out) {
-    if (lane == 0) bulk_wait_read_1();  // the store issued from this buffer two slices ago
+    if (lane == 0) bulk_wait_read_0();  // the store issued from this buffer one slice ago
     __syncwarp();
     const uint32_t rowb = buf + uint32_t(lane) * 64u, sw = uint32_t(lane >> 1) & 3u;
 #pragma unroll
@@ -158,40 +163,33 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
     flag_error(p.err, kErrBounds);
     orow = -1;
   }
+  // Any other output goes through shared memory, so that a warp writes
+  // neighbouring elements of a row, at any alignment: 64 bytes a row and pass,
+  // one row of 32 16-bit values or two half rows of 16 float32 values at a time.
   if (p.dtype == MLORA_F32) {
-    // through shared memory (the warp's whole 4 KB): a warp writes 128
-    // neighbouring bytes of one row at a time, at any alignment
-    const uint32_t base = obuf;
-    __syncwarp();
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      sts128(base + uint32_t(lane) * 128u + ((uint32_t(q) ^ (uint32_t(lane) & 7u)) << 4), __float_as_uint(f[4 * q]),
-             __float_as_uint(f[4 * q + 1]), __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3]));
-    __syncwarp();
     float* out = static_cast<float*>(p.out);
-    if (!p.out_rows) {  // consecutive rows
-      float* dst = out + row_w0 * p.N + n + lane;
-      const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
-      float v[32];  // all reads first: their latency is paid once
 #pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const uint32_t a = base + uint32_t(r) * 128u + (((uint32_t(lane) >> 2) ^ (uint32_t(r) & 7u)) << 4) +
-                           (uint32_t(lane) & 3u) * 4u;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[r]) : "r"(a));
+    for (int h = 0; h < 2; ++h) {
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        sts128(buf + uint32_t(lane) * 64u + ((uint32_t(q) ^ (uint32_t(lane >> 1) & 3u)) << 4),
+               __float_as_uint(f[16 * h + 4 * q]), __float_as_uint(f[16 * h + 4 * q + 1]),
+               __float_as_uint(f[16 * h + 4 * q + 2]), __float_as_uint(f[16 * h + 4 * q + 3]));
+      __syncwarp();
+      const int c = lane & 15, col = n + 16 * h + c;
+      float v[16];  // all reads first: their latency is paid once
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t r = 2u * uint32_t(i) + (uint32_t(lane) >> 4);
+        const uint32_t a = buf + r * 64u + (((uint32_t(c) >> 2) ^ ((r >> 1) & 3u)) << 4) + (uint32_t(c) & 3u) * 4u;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(a));
       }
 #pragma unroll
-      for (int r = 0; r < 32; ++r)
-        if (r < live) dst[int64_t(r) * p.N] = v[r];
-      return;
-    }
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-      const int64_t o = __shfl_sync(0xffffffffu, orow, r);
-      const uint32_t a =
-          base + uint32_t(r) * 128u + (((uint32_t(lane) >> 2) ^ (uint32_t(r) & 7u)) << 4) + (uint32_t(lane) & 3u) * 4u;
-      float v;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-      if (o >= 0 && n + lane < p.N) out[o * p.N + n + lane] = v;
+      for (int i = 0; i < 16; ++i) {
+        const int64_t o = __shfl_sync(0xffffffffu, orow, 2 * i + (lane >> 4));
+        if (o >= 0 && col < p.N) out[o * p.N + col] = v[i];
+      }
     }
     return;
   }
@@ -200,8 +198,6 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
     if (orow >= 0) store32(out + orow * p.N + n, f, f16);
     return;
   }
-  // rows that start anywhere: through shared memory, so that a warp writes 32
-  // neighbouring elements of one row at a time
   __syncwarp();
   const uint32_t rowb = buf + uint32_t(lane) * 64u, sw = uint32_t(lane >> 1) & 3u;
 #pragma unroll
@@ -210,39 +206,27 @@ __device__ __forceinline__ void q8_store_slice(const Q8Params& p, const float (&
            pack2(f[8 * q + 2], f[8 * q + 3], f16), pack2(f[8 * q + 4], f[8 * q + 5], f16),
            pack2(f[8 * q + 6], f[8 * q + 7], f16));
   __syncwarp();
-  if (!p.out_rows) {  // consecutive rows
-    uint16_t* dst = reinterpret_cast<uint16_t*>(out) + row_w0 * p.N + n + lane;
-    const int live = n + lane < p.N ? int(min(int64_t(32), p.M - row_w0)) : 0;
-    uint16_t v[32];  // all reads first: their latency is paid once
+  uint16_t v[32];
 #pragma unroll
-    for (int r = 0; r < 32; ++r) {
-      const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
-                         (uint32_t(lane) & 7u) * 2u;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[r]) : "r"(a));
-    }
-#pragma unroll
-    for (int r = 0; r < 32; ++r)
-      if (r < live) dst[int64_t(r) * p.N] = v[r];
-    return;
-  }
-#pragma unroll 8
   for (int r = 0; r < 32; ++r) {
-    const int64_t o = __shfl_sync(0xffffffffu, orow, r);
     const uint32_t a = buf + uint32_t(r) * 64u + (((uint32_t(lane) >> 3) ^ ((uint32_t(r) >> 1) & 3u)) << 4) +
                        (uint32_t(lane) & 7u) * 2u;
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-    if (o >= 0 && n + lane < p.N) reinterpret_cast<uint16_t*>(out)[o * p.N + n + lane] = v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[r]) : "r"(a));
+  }
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    const int64_t o = __shfl_sync(0xffffffffu, orow, r);
+    if (o >= 0 && n + lane < p.N) reinterpret_cast<uint16_t*>(out)[o * p.N + n + lane] = v[r];
   }
 }
 
 template <bool BWD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(const __grid_constant__ Q8Params p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8Threads, 1) k_q8(const __grid_constant__ Q8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage_out = smem + kQ8Stages * kQ8StageBytes;
-  float* cols = reinterpret_cast<float*>(stage_out + kStageOut2Bytes);  // [4][scales 256, biases 256]
-  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kStageOut2Bytes + kQ8ColBytes);
+  float* cols = reinterpret_cast<float*>(stage_out + kQ8OutBytes);  // [8][scales 128, biases 128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kQ8OutBytes + kQ8ColBytes);
   uint64_t* empty = full + kQ8Stages;
   uint64_t* ifull = empty + kQ8Stages;  // [2] integer sums of the accumulator complete
   uint64_t* conv = ifull + 2;           // [2] rewritten as fp32 in both CTAs (used in the even CTA)
@@ -264,9 +248,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&ifull[a], 1);
-      mbar_init(&conv[a], 8);  // one arrival per epilogue warp of both CTAs
+      mbar_init(&conv[a], 2 * kQ8EpiWarps);  // one arrival per epilogue warp of both CTAs
       mbar_init(&xfull[a], 1);
-      mbar_init(&tempty[a], 8);
+      mbar_init(&tempty[a], 2 * kQ8EpiWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -283,9 +267,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if ((warp == 0 || warp >= 6) && lane == 0) {
+  if ((warp == 0 || warp == 6) && lane == 0) {
     // ---------------------------------------------------------------- TMA producers (both CTAs)
-    const uint32_t pid = warp == 0 ? 0u : uint32_t(warp - 5);
+    const uint32_t pid = warp == 0 ? 0u : 1u;
     uint32_t gk = 0;
     int stage = 0;
     uint32_t phase = 0;
@@ -294,7 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
     const uint64_t pol_keep = policy_evict_last(), pol_norm = policy_evict_normal();
     // the ring slot of the next k-block, when it is this warp's
     auto claim = [&]() -> int {
-      const int s = (gk++ % kProducers) == pid ? stage : -1;
+      const int s = (gk++ % 2u) == pid ? stage : -1;
       if (s >= 0) {
         if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.err)) {
           ok = false;
@@ -436,12 +420,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
     while (!mbar_try(su32(drain), 0)) {
       if (now_ns() - t0 > kTimeoutNs) { flag_error(p.err, kErrTimeout); break; }
     }
-  } else if (warp >= 2 && warp < 6) {
+  } else if ((warp >= 2 && warp < 6) || warp >= 8) {
     // ---------------------------------------------------------------- epilogue (both CTAs)
     const int quad = warp % 4;
     const uint32_t tempty0 = mapa(su32(&tempty[0]), 0), conv0 = mapa(su32(&conv[0]), 0);
-    const uint32_t obuf = su32(stage_out) + uint32_t(warp - 2) * 4096u;
-    uint32_t slices = 0;
+    const int ew = warp < 6 ? warp - 2 : warp - 4;        // 0..7
+    const int first = ew < 4 ? 0 : kQ8EpiCols, end = first + kQ8EpiCols;  // this warp's columns of a tile
+    const uint32_t obuf = su32(stage_out) + uint32_t(ew) * 2048u;
+    float* cs = cols + ew * 2 * kQ8EpiCols;
+    const uint32_t cs32 = su32(cs) - uint32_t(first) * 4u;
     int acc = 0;
     uint32_t acc_phase = 0;
     uint32_t x_phase[2] = {0, 0};
@@ -450,18 +437,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
       const Q8Item it = q8_item(p, item);
       // the tile's column scales and biases, fetched while its sums are formed
       // (a copy per warp: no warp waits for another)
-      float* cs = cols + (warp - 2) * 512;
       if (!BWD) {
         __syncwarp();
 #pragma unroll
-        for (int c = lane; c < 256; c += 32) {
-          const int n = it.nb * 256 + c;
+        for (int c = lane; c < kQ8EpiCols; c += 32) {
+          const int n = it.nb * 256 + first + c;
           cs[c] = n < p.N ? __ldg(p.w_scale + n) : 0.f;
-          cs[256 + c] = n < p.N && p.bias ? q8_bias(p, n) : 0.f;
+          cs[kQ8EpiCols + c] = n < p.N && p.bias ? q8_bias(p, n) : 0.f;
         }
         __syncwarp();
       }
-      const uint32_t cs32 = su32(cs);
       const int64_t row_w0 = int64_t(it.t) * kTileRows + int(crank) * kHalfRows + quad * 32;
       const int n0 = it.nb * 256;
       const float sa = row_w0 + lane < p.M ? __ldg(p.a_scale + row_w0 + lane) : 0.f;
@@ -483,7 +468,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
       };
       const bool expanded = it.nc > 0;
       if (expanded) {
-        for (int col = 0; col < kAccCols && n0 + col < p.N; col += 32) {
+        for (int col = first; col < end && n0 + col < p.N; col += 32) {
           float f[32];
           scaled(col, f);
           tc_st32(tbase + col, f);
@@ -496,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
         x_phase[acc] ^= 1;
         tc_fence_after();
       }
-      for (int col = 0; col < kAccCols && n0 + col < p.N; col += 32) {
+      for (int col = first; col < end && n0 + col < p.N; col += 32) {
         float f[32];
         if (expanded) {
           uint32_t v[32];
@@ -509,11 +494,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_q8(co
         if (!BWD && p.bias) {
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            const float4 s = lds_f4(cs32 + 1024u + uint32_t(col + 4 * q) * 4u);
+            const float4 s = lds_f4(cs32 + uint32_t(kQ8EpiCols + col + 4 * q) * 4u);
             f[4 * q] += s.x; f[4 * q + 1] += s.y; f[4 * q + 2] += s.z; f[4 * q + 3] += s.w;
           }
         }
-        q8_store_slice(p, f, row_w0, n0 + col, obuf, slices++, lane);
+        q8_store_slice(p, f, row_w0, n0 + col, obuf, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -598,7 +583,7 @@ int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
   prm.pdl_z = pdl ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kQ8Threads);
   cfg.dynamicSmemBytes = kQ8Smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
