@@ -52,6 +52,8 @@ struct Q8Params {
   int N;
   int n_tiles, n_nblk, group, n_items;
   int nk;              // 128-byte k-blocks of the integer product
+  int a_rows;          // at most 128 rows in all: they are the A box, and the odd CTA loads no A (0: 128-row
+                       // boxes in both); the tile's other rows are whatever the ring held, and are not stored
   int expand;
   int dtype;
   int pdl_rows, pdl_z;  // launched to overlap the kernel before it, which makes the 8-bit rows / the
@@ -277,14 +279,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8Threads, 1) k_q8(
     bool ok = true;
     const uint64_t pol_keep = policy_evict_last(), pol_norm = policy_evict_normal();
     // the ring slot of the next k-block, when it is this warp's
-    auto claim = [&]() -> int {
+    auto claim = [&](uint32_t bytes) -> int {
       const int s = (gk++ % 2u) == pid ? stage : -1;
       if (s >= 0) {
         if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.err)) {
           ok = false;
           return -1;
         }
-        if (leader) mbar_expect_tx(&full[stage], 2 * kQ8StageBytes);
+        if (leader) mbar_expect_tx(&full[stage], bytes);
         issued |= 1u << stage;
         issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
       }
@@ -292,13 +294,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8Threads, 1) k_q8(
       return s;
     };
     bool rows_ready = !p.pdl_rows, z_ready = !p.pdl_z;
+    const uint32_t main_bytes = p.a_rows ? uint32_t(p.a_rows) * kQ8K + kQ8StageBytes : 2 * kQ8StageBytes;
     auto expand = [&](const Q8Item& it) {
       if (it.nc > 0 && !z_ready) {
         grid_dep_wait();
         z_ready = true;
       }
       for (int i = 0; i < it.nc && ok; ++i) {
-        const int s = claim();
+        const int s = claim(2 * kQ8StageBytes);
         if (s < 0) continue;
         uint8_t* sA = smem + s * kQ8StageBytes;
         uint8_t* sB = sA + kA2Bytes;
@@ -322,7 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8Threads, 1) k_q8(
       for (int kb = 0; kb < p.nk && ok; ++kb) {
         if (kb == defer) expand(last);
         if (!ok) break;
-        const int s = claim();
+        const int s = claim(main_bytes);
         if (s < 0) continue;
         uint8_t* sA = smem + s * kQ8StageBytes;
         uint8_t* sB = sA + kA2Bytes;
@@ -333,7 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8Threads, 1) k_q8(
           grid_dep_wait();
           rows_ready = true;
         }
-        tma_load_pair(sA, &p.mA, bar, kb * kQ8K, row0, pol_norm);
+        if (p.a_rows == 0 || leader) tma_load_pair(sA, &p.mA, bar, kb * kQ8K, row0, pol_norm);
       }
       if (ok && defer == p.nk) expand(last);
       last = it;
@@ -545,7 +548,10 @@ int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
   Q8Params prm;
   memset(&prm, 0, sizeof(prm));
   const int K = a.bwd ? a.d_out : a.d_in, N = a.bwd ? a.d_in : a.d_out;
-  if (!make_map8(&prm.mA, a.Aq, a.M, q8_ld(K)) || !make_map8(&prm.mB, a.Wq, a.d_out, q8_ld(a.d_in)))
+  // up to 128 rows: a box of just these (17 rows of 4096 -> 11008 took 41 us with
+  // 128-row boxes, whose reads past a tensor of fewer than 32 rows are slow)
+  prm.a_rows = a.M <= 128 ? int(a.M) : 0;
+  if (!make_map8(&prm.mA, a.Aq, a.M, q8_ld(K), prm.a_rows ? prm.a_rows : 128) || !make_map8(&prm.mB, a.Wq, a.d_out, q8_ld(a.d_in)))
     return MLORA_ERR_UNSUPPORTED;
   if (a.expand) {
     const int64_t zrows = int64_t(a.plan.n_chunks) * kTileRows;
