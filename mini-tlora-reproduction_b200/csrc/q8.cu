@@ -250,7 +250,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
 // out per 16-bit element, if the work around each row is spread over enough
 // elements of a thread: NV up to 16 (8 with column scales).
 template <class T, bool VEC, bool CS, int NV>
-__global__ void __launch_bounds__(512) k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
+__global__ void __launch_bounds__(NV == 6 ? 256 : 512, NV == 6 ? 3 : 0) k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
                                                    const float* __restrict__ col_scale, int8_t* __restrict__ q,
                                                    float* __restrict__ scale, int sh) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product after it may start
@@ -359,14 +359,14 @@ int launch_quantize(const T* src, int64_t rows, int64_t cols, int64_t ld, const 
                     cudaStream_t st) {
   const int64_t groups = q8_ld(cols) / 8;  // the zero bytes past `cols` included
   constexpr bool kWide = CS || sizeof(T) == 4;  // held as float32
-  const RowGrid g = row_grid(rows, groups, kWide ? 4 : 16);
+  const RowGrid g = row_grid(rows, groups, !kWide ? 16 : CS && sizeof(T) == 4 ? 4 : 6);
 #define MLORA_QUANT(NV) \
   k_quantize<T, VEC, CS, NV><<<g.grid, g.block, 0, st>>>(src, rows, int(cols), ld, cs, q, scale, g.sh)
   if (g.nv <= 1) MLORA_QUANT(1);
   else if (g.nv <= 2) MLORA_QUANT(2);
   else if (g.nv <= 3) MLORA_QUANT(3);
   else if (g.nv <= 4) MLORA_QUANT(4);
-  else if (g.nv <= 6) MLORA_QUANT(6);
+  else if (g.nv <= 6 && g.block <= 256) MLORA_QUANT(6);  // three blocks an SM: 65,536 x 11,008 554 -> 499 us
   else if (g.nv <= 8) MLORA_QUANT(8);
   else if (!kWide && g.nv <= 12) MLORA_QUANT((kWide ? 0 : 12));
   else if (!kWide && g.nv <= 16) MLORA_QUANT((kWide ? 0 : 16));

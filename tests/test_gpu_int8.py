@@ -41,7 +41,10 @@ def assert_rows8(r8, x, col_scale=None):
 
 @pytest.mark.parametrize("dt", [BF, FP, F32])
 @pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (2, 8), (5, 16), (33, 17), (9, 255), (7, 1000), (64, 1024),
-                                         (5, 4096), (3, 11008), (2, 16384), (2, 20000), (2, 16390), (300, 64)])
+                                         (5, 4096), (3, 11008), (2, 16384), (2, 20000), (2, 16390), (300, 64),
+                                         # rows enough to fill the GPU: other splits of a row over threads
+                                         (1200, 4096), (700, 8200), (600, 11008), (400, 14000), (300, 24000),
+                                         (200, 40000), (40, 70000), (5000, 520), (9000, 40)])
 def test_rows_are_exact(dt, rows, cols):
     x = randn((rows, cols), dt, rows * 7 + cols)
     assert_rows8(ops.quantize_rows(x), x)
@@ -104,7 +107,8 @@ def test_rows_of_views():
     (1, 64, 64, True), (1, 1, 1, True), (2, 4096, 129, False), (7, 1000, 1531, True), (16, 256, 4096, True),
     (17, 2048, 260, False), (33, 100, 72, True), (64, 512, 512, False), (128, 128, 256, True),
     (255, 333, 777, True), (256, 4096, 256, False), (300, 1040, 520, True), (513, 72, 1288, True),
-    (1500, 640, 2056, True)])
+    (1500, 640, 2056, True), (20, 520, 2100, True), (100, 200, 300, False), (128, 4096, 520, True),
+    (129, 264, 520, True), (5000, 136, 1288, True), (300, 4112, 3, True)])
 def test_product(dt, rows, d_in, d_out, bias):
     x, w = randn((rows, d_in), dt, 1), randn((d_out, d_in), dt, 2, d_in ** -0.5)
     b = randn((d_out,), dt, 3) if bias else None
