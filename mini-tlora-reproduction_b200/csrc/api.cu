@@ -4,6 +4,7 @@
 #include <cstring>
 #include <initializer_list>
 #include <memory>
+#include <new>
 
 #include "common.cuh"
 #include "q8.cuh"
@@ -48,18 +49,25 @@ const Plan* plan_of(const mlora_problem* prob, const mlora_routing* route, int* 
       return &kept[0]->plan;
     }
   }
-  auto k = std::make_unique<Kept>();
-  *status = build_plan(prob, route, &k->plan);
-  if (*status != MLORA_OK) return nullptr;
-  k->rows = prob->rows; k->d_in = prob->d_in; k->d_out = prob->d_out; k->r_pack = route->r_pack;
-  k->seg_start.assign(route->seg_start, route->seg_start + nb);
-  k->seg_adapter.assign(route->seg_adapter, route->seg_adapter + ns);
-  k->rank.assign(route->rank, route->rank + na);
-  k->pack_off.assign(route->pack_off, route->pack_off + na);
-  k->scaling.assign(route->scaling, route->scaling + na);
-  kept.insert(kept.begin(), std::move(k));
-  if (kept.size() > kKept) kept.pop_back();
-  return &kept[0]->plan;
+  // no exception may leave a C entry point: without host memory for the plan
+  // the call is refused
+  try {
+    auto k = std::make_unique<Kept>();
+    *status = build_plan(prob, route, &k->plan);
+    if (*status != MLORA_OK) return nullptr;
+    k->rows = prob->rows; k->d_in = prob->d_in; k->d_out = prob->d_out; k->r_pack = route->r_pack;
+    k->seg_start.assign(route->seg_start, route->seg_start + nb);
+    k->seg_adapter.assign(route->seg_adapter, route->seg_adapter + ns);
+    k->rank.assign(route->rank, route->rank + na);
+    k->pack_off.assign(route->pack_off, route->pack_off + na);
+    k->scaling.assign(route->scaling, route->scaling + na);
+    kept.insert(kept.begin(), std::move(k));
+    if (kept.size() > kKept) kept.pop_back();
+    return &kept[0]->plan;
+  } catch (const std::bad_alloc&) {
+    *status = MLORA_ERR_WORKSPACE;
+    return nullptr;
+  }
 }
 
 // layout of the caller's workspace: [plan tables | dZt scratch]
@@ -69,7 +77,11 @@ size_t ws_bytes(const Plan& p, int dtype) { return align_up(p.bytes, 1024) + zt_
 // staged before return) and return the device view.
 int upload_plan(const Plan& p, void* ws, cudaStream_t st, PlanDev* dev) {
   thread_local std::vector<uint8_t> host;
-  host.assign(p.bytes, 0);
+  try {
+    host.assign(p.bytes, 0);
+  } catch (const std::bad_alloc&) {
+    return MLORA_ERR_WORKSPACE;
+  }
   auto put = [&](size_t off, const void* src, size_t n) {
     if (n) std::memcpy(host.data() + off, src, n);
   };
@@ -714,7 +726,8 @@ extern "C" int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* 
                                 const void* B_pack, void* Y, void* zsave, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   if (!prob || !route || !q8) return MLORA_ERR_INVALID_ARG;
-  if ((q8->Wq && (W || !q8->w_scale || !q8->Xq)) || (q8->Xq && !q8->x_scale)) return MLORA_ERR_INVALID_ARG;
+  if (prob->rows != 0 && ((q8->Wq && (W || !q8->w_scale || !q8->Xq)) || (q8->Xq && !q8->x_scale)))
+    return MLORA_ERR_INVALID_ARG;
   if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
   int st = check_q8({q8->Wq, q8->Xq}, {q8->w_scale, q8->x_scale});
   if (st != MLORA_OK) return st;
@@ -727,7 +740,8 @@ extern "C" int mlora_backward_q8(const mlora_problem* prob, const mlora_routing*
                                  const void* B_pack, const void* zsave, void* dX, void* dA_pack, void* dB_pack,
                                  void* workspace, size_t workspace_bytes, void* stream) {
   if (!prob || !route || !q8) return MLORA_ERR_INVALID_ARG;
-  if ((q8->Wq && (W || !q8->w_scale || (dX && (!q8->Gq || !q8->g_scale)))) || (q8->Xq && !q8->x_scale))
+  if (prob->rows != 0 &&
+      ((q8->Wq && (W || !q8->w_scale || (dX && (!q8->Gq || !q8->g_scale)))) || (q8->Xq && !q8->x_scale)))
     return MLORA_ERR_INVALID_ARG;
   if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
   int st = check_q8({q8->Wq, q8->Xq, q8->Gq}, {q8->w_scale, q8->x_scale, q8->g_scale});

@@ -24,7 +24,8 @@ from typing import Optional
 
 import torch
 
-from .multi_lora_linear import MultiLoRALinear
+from . import ops
+from .multi_lora_linear import MultiLoRALinear, _save8
 
 
 class GraphedTrainStep:
@@ -51,14 +52,27 @@ class GraphedTrainStep:
             self.y = self._step()
 
     def _step(self) -> torch.Tensor:
+        """The calls of one step, without autograd: its nodes for the adapters'
+        parameters may belong to a graph that still lives on another stream,
+        and a capture must not meet that stream."""
         m = self.model
-        for ad in m.adapters.values():
-            ad.A.grad = None
-            ad.B.grad = None
-        self.x.grad = None
-        y = m(self.x, self.ids, plan=self.plan)
-        y.backward(self.dy)
-        m.sgd_step(self.lr)
+        pk = m._pack()
+        W, base8, bias = m._base_operands()
+        params = pk.params()
+        x, W, bias = pk.operands(self.x.detach(), W, bias, base8, params)
+        st = pk.state(self.plan, m.impl, base8, _save8(m.save_input))
+        want_A, want_B = any(p.requires_grad for p in params[0::2]), any(p.requires_grad for p in params[1::2])
+        with torch.no_grad(), ops._on(x.device):
+            rows8 = ops._new_rows8(x.shape[0], x.shape[1], x.device) if st.save8 and want_A else None
+            y, z, xs, _ = ops.forward_raw(x, W, bias, st, rows8=rows8)
+            dx, dA, dB = ops.backward_raw(self.dy.contiguous(), xs if rows8 is None else None, W, z, st, self.x.requires_grad,
+                                          want_A, want_B, rows8)
+            self.x.grad = dx
+            for i, ((o, r), act) in enumerate(zip(st.table.spans(), self.plan.active.tolist())):
+                A, B = params[2 * i], params[2 * i + 1]
+                A.grad = dA.narrow(0, o, r) if act and A.requires_grad else None
+                B.grad = dB.narrow(1, o, r) if act and B.requires_grad else None
+            m.sgd_step(self.lr)
         return y
 
     def __call__(self, x: Optional[torch.Tensor] = None, dy: Optional[torch.Tensor] = None) -> torch.Tensor:

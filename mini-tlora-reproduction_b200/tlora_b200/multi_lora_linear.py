@@ -237,33 +237,46 @@ class _PackedAdapters:
             self._scaling = (s, np.array([float(v) for v in s], dtype=np.float32))
         return self._scaling[1]
 
-    def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
-              base8: Optional[ops.Int8Rows] = None, save8: bool = False):
+    def state(self, plan: ops.RoutePlan, impl: str, base8: Optional[ops.Int8Rows] = None,
+              save8: bool = False) -> ops.LayerState:
+        return ops.LayerState(self.table, self.scaling(), plan, self.A_pack, self.B_pack, impl, base8=base8,
+                              save8=save8)
+
+    def operands(self, x, W, bias, base8: Optional[ops.Int8Rows], params: list):
+        """(x, W, bias) as the native calls take them, after the checks."""
         if x.device.type != "cuda":
             raise RuntimeError(
                 "tlora_b200 computes on CUDA devices only (sm_100a); move the module and inputs to a "
                 "B200 with .cuda() -- there is no CPU path")
-        params = self.params()
         self.sync(params)
-        if self.A_pack.device != x.device:
-            raise RuntimeError(f"input on {x.device} but adapters on {self.A_pack.device}")
-        if x.dtype != self.A_pack.dtype or (W is not None and W.dtype != x.dtype):
-            raise RuntimeError(f"dtype mismatch: input {x.dtype}, weights {self.A_pack.dtype}")
-        if base8 is not None and base8.device != x.device:
-            raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
-        if base8 is not None and bias is not None and (bias.dtype != x.dtype or bias.device != x.device):
-            raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
+        A, B = self.A_pack, self.B_pack
+        if A.device != x.device:
+            raise RuntimeError(f"input on {x.device} but adapters on {A.device}")
+        if x.dtype != A.dtype or (W is not None and W.dtype != x.dtype):
+            raise RuntimeError(f"dtype mismatch: input {x.dtype}, weights {A.dtype}")
+        if x.shape[1] != A.shape[1]:
+            raise ValueError(f"x has {x.shape[1]} features, the layer {A.shape[1]}")
+        if base8 is not None:
+            if base8.device != x.device:
+                raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
+            if base8.shape != (B.shape[0], A.shape[1]):
+                raise ValueError(f"8-bit backbone {base8.shape} in a layer of {(B.shape[0], A.shape[1])}")
+            if bias is not None and (bias.dtype != x.dtype or bias.device != x.device):
+                raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
         if W is not None and W.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the backbone is frozen: no dW (tlora/multi_lora_linear.py:78-80)")
-        x = x.contiguous()
+        return (x.contiguous(), W.contiguous() if W is not None else None,
+                bias.contiguous() if bias is not None else None)
+
+    def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
+              base8: Optional[ops.Int8Rows] = None, save8: bool = False):
+        params = self.params()
+        x, Wc, bc = self.operands(x, W, bias, base8, params)
         if plan is None:
             plan = ops.route(ids, self.table, x.device)
         train = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params))
         # nothing is kept for a backward that cannot follow
-        st = ops.LayerState(self.table, self.scaling(), plan, self.A_pack, self.B_pack, impl, base8=base8,
-                            save8=save8 and train)
-        Wc = W.contiguous() if W is not None else None
-        bc = bias.contiguous() if bias is not None else None
+        st = self.state(plan, impl, base8, save8 and train)
         with ops._on(x.device):
             if not train:
                 return ops.forward_raw(x.detach(), Wc, bc, st)[0]
@@ -324,7 +337,9 @@ class MultiLoRALinear(_Int8BaseMixin, nn.Module):
         plan; calls with ``plan=plan`` then issue no host-to-device copy, so a
         training step with fixed routing can be captured into a CUDA graph
         (tlora_b200.graphs.GraphedTrainStep).  The adapters' ranks and
-        scalings must not change afterwards."""
+        scalings must not change afterwards.  Calls with one plan share its
+        workspace: they must follow one another (one stream, or streams that
+        wait for each other)."""
         pk = self._pack()
         pk.sync()
         st = ops.LayerState(pk.table, pk.scaling(), plan, pk.A_pack, pk.B_pack, self.impl)

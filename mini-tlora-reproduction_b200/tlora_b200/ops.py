@@ -578,6 +578,8 @@ def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8
     With an 8-bit backbone (st.base8) or ``rows8`` the call is
     mlora_forward_q8; ``rows8`` receives the 8-bit rows of the sorted x."""
     rows, d_in = x.shape
+    if st.plan.rows != rows:
+        raise ValueError(f"the routing plan is of {st.plan.rows} rows, x has {rows}")
     d_out = st.B_pack.shape[0]
     xs = x_sorted if x_sorted is not None else (gather_rows(x, st.plan.perm) if st.plan.perm is not None else x)
     args = _Call(rows, d_in, d_out, mlora_dtype(x.dtype), st)

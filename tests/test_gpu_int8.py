@@ -541,3 +541,170 @@ def test_loading_an_8bit_checkpoint():
     c = b.cpu().cuda()
     assert torch.equal(c(x, ids), a(x, ids))
     assert np.isfinite(float(c(x, ids).detach().float().sum()))
+
+
+# ------------------------------------------------------------------ edges of the layer
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_layer_without_rows(dt):
+    m = layer(64, 96, {0: 8}, dt).quantize_base()
+    for how in ("full", "int8"):
+        m.save_input = how
+        x = torch.empty(0, 64, device="cuda", dtype=dt, requires_grad=True)
+        y = m(x, torch.empty(0, dtype=torch.int64))
+        y.backward(torch.empty_like(y))
+        assert y.shape == (0, 96) and x.grad.shape == (0, 64)
+        assert m.adapters["0"].A.grad is None and m.adapters["0"].B.grad is None
+
+
+@pytest.mark.parametrize("base8", [False, True])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_cuda_core_kernels_on_request(dt, base8):
+    d_in, d_out, ranks, ids = LAYERS["ranks"]
+    m = layer(d_in, d_out, ranks, dt)
+    m.impl = "simt"
+    m.save_input = "int8"
+    w = m.base.weight.detach().clone()
+    if base8:
+        m.quantize_base()
+    x, dy = randn((len(ids), d_in), dt, 1), randn((len(ids), d_out), dt, 2, 0.1)
+    check_layer(m, w, x, ids, dy, base8, True)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_delta_with_saved_inputs(dt):
+    d_in, d_out, ranks, ids = LAYERS["four_jobs"]
+    m = layer(d_in, d_out, ranks, dt)
+    x, dy = randn((len(ids), d_in), dt, 1), randn((len(ids), d_out), dt, 2, 0.1)
+    plain = step(m, x, ids, dy, add_base=False)
+    m.save_input = "int8"
+    with_base = step(m, x, ids, dy)
+    delta = step(m, x, ids, dy, add_base=False)
+    assert torch.equal(delta[0], plain[0])
+    if dt == BF:  # (float32: other kernels of the low-rank terms, other roundings)
+        assert torch.equal(delta[1], plain[1])
+    for a, b in zip(delta[2] + delta[3], with_base[2] + with_base[3]):
+        assert torch.equal(a, b)
+
+
+def test_layer_refusals():
+    m = layer(64, 96, {0: 8}, BF).quantize_base()
+    ids = torch.zeros(4, dtype=torch.int64)
+    x = randn((4, 64), BF, 1)
+    with pytest.raises(ValueError, match="features"):
+        m(randn((4, 72), BF, 1), ids)
+    with pytest.raises(RuntimeError, match="dtype"):
+        m(x.half(), ids)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        m(x.cpu(), ids)
+    with pytest.raises(ValueError, match="plan"):
+        m(x, ids, plan=m.route(torch.zeros(5, dtype=torch.int64)))
+    m.impl = "tc"
+    odd = layer(100, 96, {0: 8}, BF).quantize_base()
+    odd.impl = "tc"  # 16-bit rows of 100 columns are not a tensor-core operand
+    with pytest.raises(NotImplementedError):
+        odd(randn((4, 100), BF, 1), ids)
+
+
+def test_copies_of_an_8bit_layer():
+    import copy
+
+    m = layer(128, 96, {0: 8}, BF).quantize_base()
+    x, ids = randn((40, 128), BF, 1), torch.zeros(40, dtype=torch.int64)
+    want = m(x, ids)
+    twin = copy.deepcopy(m)
+    assert torch.equal(twin(x, ids), want)
+    with torch.no_grad():
+        m.base.weight_q8.zero_()
+    assert torch.equal(twin(x, ids), want)
+    plan = twin.route(ids)
+    twin(x, ids, plan=plan)
+    again = copy.deepcopy(plan)  # a plan that has been used
+    assert torch.equal(twin(x, ids, plan=again), want)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_capture_while_an_eager_graph_of_the_adapters_lives(eight):
+    d_in, d_out, ranks, ids = LAYERS["four_jobs"]
+    m = layer(d_in, d_out, ranks, BF)
+    if eight:
+        m.quantize_base()
+        m.save_input = "int8"
+    x, dy = randn((len(ids), d_in), BF, 1), randn((len(ids), d_out), BF, 2, 0.1)
+    alive = m(x.clone().requires_grad_(True), ids)  # its nodes for the adapters are not released
+    g = GraphedTrainStep(m, x, ids, dy, lr=0.0)
+    y = g(x, dy)
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive.detach())
+    alive.backward(dy)
+    assert m.adapters["0"].A.grad is not None
+
+
+@pytest.mark.parametrize("dt", [BF, FP, F32])
+def test_fused_sgd_of_the_native_call(dt):
+    """MLORA_FUSED_SGD: the gradients of the call, and the weights that the
+    separate step would give, bit by bit."""
+    import ctypes
+
+    d_in, d_out, ranks, ids = LAYERS["long_jobs"]
+    m = layer(d_in, d_out, ranks, dt).quantize_base()
+    m.save_input = "int8"
+    x, dy = randn((len(ids), d_in), dt, 1), randn((len(ids), d_out), dt, 2, 0.1)
+    want = step(m, x, ids, dy)
+    pk = m._pack()
+    plan = m.route(ids)
+    st = pk.state(plan, "auto", m.base.rows8, True)
+    r8 = ops._new_rows8(len(ids), d_in, x.device)
+    y, z, _, _ = ops.forward_raw(x, None, m.base.bias, st, rows8=r8)
+    call = ops._Call(len(ids), d_in, d_out, ops.mlora_dtype(dt), st)
+    call.prob.flags, call.prob.lr = _lib.FUSED_SGD, 0.5
+    ws = torch.empty(call.wbytes, dtype=torch.uint8, device="cuda")
+    g8 = ops._Scratch8(len(ids), d_out, x.device)
+    q8 = ops._q8_struct(m.base.rows8, r8, g8)
+    scratch = torch.empty(max(1, call.scratch8()), dtype=torch.uint8, device="cuda")
+    q8.scratch, q8.scratch_bytes = scratch.data_ptr(), call.scratch8()
+    dx, dA, dB = torch.empty_like(x), torch.empty_like(pk.A_pack), torch.empty_like(pk.B_pack)
+    old = [p.detach().clone() for p in pk.params()]
+    _lib.call("mlora_backward_q8", ctypes.byref(call.prob), ctypes.byref(call.route), ctypes.byref(q8),
+              dy.data_ptr(), None, None, pk.A_pack.data_ptr(), pk.B_pack.data_ptr(), z.data_ptr(), dx.data_ptr(),
+              dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), call.wbytes, ops._stream(x.device))
+    torch.cuda.synchronize()
+    assert torch.equal(dx, want[1])
+    for i, (o, r) in enumerate(pk.table.spans()):
+        assert torch.equal(dA[o:o + r], want[2][i]) and torch.equal(dB[:, o:o + r], want[3][i])
+        for p, was, g in ((pk.params()[2 * i], old[2 * i], want[2][i]), (pk.params()[2 * i + 1], old[2 * i + 1],
+                                                                       want[3][i])):
+            ref_p = was.clone()
+            ops.sgd_step_([(ref_p, g.contiguous())], 0.5)
+            assert torch.equal(p, ref_p)
+    # too little scratch is refused before anything runs
+    if dt != F32:
+        q8.scratch_bytes -= 1
+        with pytest.raises(_lib.MloraError):
+            _lib.call("mlora_backward_q8", ctypes.byref(call.prob), ctypes.byref(call.route), ctypes.byref(q8),
+                      dy.data_ptr(), None, None, pk.A_pack.data_ptr(), pk.B_pack.data_ptr(), z.data_ptr(),
+                      dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), call.wbytes, ops._stream(x.device))
+
+
+# ------------------------------------------------------------------ large
+
+def test_offsets_past_32_bits():
+    rows, cols = 70000, 32768  # 2.3e9 elements
+    x = torch.empty(rows, cols, device="cuda", dtype=BF).normal_(generator=gen(1))
+    r8 = ops.quantize_rows(x)
+    back = ops.dequantize_rows(r8, BF)
+    for s in (slice(0, 3), slice(rows - 3, rows), slice(65534, 65539)):
+        part = ops.quantize_rows(x[s].contiguous())
+        assert torch.equal(r8.q[s], part.q) and torch.equal(r8.scale[s], part.scale)
+        assert torch.equal(back[s], ops.dequantize_rows(part, BF))
+    del x, back
+    # a product that reads and writes past them
+    w8 = ops.quantize_rows(randn((40000, 32768), BF, 2))
+    y = ops.int8_linear(r8, w8, dtype=BF)
+    assert y.numel() > 2 ** 31
+    for s in (slice(0, 2), slice(rows - 2, rows), slice(53700, 53702)):
+        part = ops.Int8Rows(r8.q[s].contiguous(), r8.scale[s].contiguous(), cols)
+        acc = ints(part) @ ints(w8).t()
+        want = acc * part.scale.double()[:, None] * w8.scale.double()
+        ref.assert_within(y[s], want, 1.01 * (3 * ref.U + ref.half_step(BF)) * want.abs() + ref.tiny(BF), "y")
+    assert _lib.device_error() == 0
