@@ -411,7 +411,7 @@ int mlora_scatter_rows(const void* src, const int32_t* perm, int64_t rows, int32
  * fl32(x[i, k] col_scale[k]) instead.  A row of zeros has s = 0; a row with an
  * infinity or a NaN has s = NaN and q = 0, so that every value computed from
  * that row, and from no other, is NaN.  mlora_q8_dequantize writes the dense
- * matrix of s[i] q[i, k], each rounded once to dtype. */
+ * matrix of s[i] q[i, k], each rounded once to dtype.  cols <= 2^30. */
 int64_t mlora_q8_ld(int64_t cols);
 int mlora_q8_quantize(const void* src, int64_t rows, int64_t cols, int64_t ld_src, int32_t dtype,
                       const float* col_scale, int8_t* q, float* scale, void* stream);

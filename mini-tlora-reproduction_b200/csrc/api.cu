@@ -245,9 +245,9 @@ extern "C" int32_t mlora_num_tiles(int64_t rows) {
 
 namespace {
 
-// Kernel family of the 8-bit product of a layer call whose 16-bit kernels run
-// as `impl`: a call without LoRA rows has no operand that needs the 16-bit
-// family's alignment.
+// Kernel family of the 8-bit product of a layer call whose other kernels run as
+// `impl`: left open by MLORA_IMPL_AUTO, since the 8-bit operands are always
+// aligned, whatever the 16-bit ones are.
 int q8_impl(const mlora_problem* prob, int impl) {
   return prob->impl == MLORA_IMPL_AUTO ? MLORA_IMPL_AUTO : impl;
 }
@@ -255,8 +255,8 @@ int q8_impl(const mlora_problem* prob, int impl) {
 // The 8-bit backbone product of mlora_forward_q8, with the LoRA expand of the
 // intermediate that the shrink before it left in zsave.
 int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8, const PlanDev& dev,
-                    int impl, Q8After after, const void* bias, const void* B_pack, void* Y, const void* zsave, int32_t stages,
-                    cudaStream_t s) {
+                    int impl, Q8After after, const void* bias, const void* B_pack, void* Y, const void* zsave,
+                    int32_t stages, cudaStream_t s) {
   Q8Main m;
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
   m.Aq = q8->Xq; m.a_scale = q8->x_scale;
@@ -310,7 +310,8 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   if (few) {
     st = q8_few_prep(X, prob->rows, prob->d_in, prob->dtype, q8->Xq, q8->x_scale, dev, A_pack, zsave, s);
     if (st != MLORA_OK) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
+                           s);
   }
   if (q8 && q8->Xq) {  // operand of the 8-bit product, the saved form of X, or both
     st = q8_quantize(X, prob->rows, prob->d_in, prob->d_in, prob->dtype, nullptr, (int8_t*)q8->Xq,
@@ -336,13 +337,15 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     st = tc_forward(a, s);
     if (st != MLORA_OK || !q8_base) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
+                           s);
   }
   if (q8_base && prob->dtype == MLORA_F32) {
     st = q8_low32(false, dev, (const float*)X, (const float*)A_pack, (float*)zsave, prob->rows, prob->d_in,
                   prob->d_out, route->r_pack, s);
     if (st != MLORA_OK) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
+                           s);
   }
   SimtCall a;
   a.plan = dev;
@@ -527,10 +530,6 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
                           dB_pack, stages & of_b, 0, p.n_tiles, 0, nb_out, nullptr, s);
 }
 
-}  // namespace
-
-namespace {
-
 // mlora_backward_staged, or with `q8` mlora_backward_q8 over all ranges.
 int backward_staged(const mlora_problem* prob, const mlora_routing* route, const void* dY, const void* X,
                     const void* W, const void* A_pack, const void* B_pack, const void* zsave, void* dzsave, void* dX,
@@ -633,8 +632,8 @@ extern "C" int64_t mlora_q8_ld(int64_t cols) { return cols <= 0 ? 0 : q8_ld(cols
 namespace {
 
 int check_rows_cols(int64_t rows, int64_t cols, int32_t dtype) {
-  if (rows < 0 || rows > (int64_t(1) << 31) - kTileRows || cols < 1 || cols > INT32_MAX - 64)
-    return MLORA_ERR_INVALID_ARG;
+  if (rows < 0 || rows > (int64_t(1) << 31) - kTileRows || cols < 1) return MLORA_ERR_INVALID_ARG;
+  if (cols > (int64_t(1) << 30)) return MLORA_ERR_UNSUPPORTED;  // column indices and their steps are 32-bit
   if (dtype != MLORA_F32 && dtype != MLORA_BF16 && dtype != MLORA_F16) return MLORA_ERR_UNSUPPORTED;
   return MLORA_OK;
 }

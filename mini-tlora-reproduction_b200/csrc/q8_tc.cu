@@ -20,9 +20,13 @@
 // accumulator: its expand k-blocks sit in the ring after the first kDefer
 // k-blocks of the next tile, by which time the rewrite has finished.
 //
-// Bound by the integer tensor rate for large tiles; the tile order keeps a
-// group of weight blocks in L2 while the rows stream, as in the 16-bit
-// mainloops.  Tiles are dealt round-robin to the resident pairs: all tiles of
+// Bound by what an SM takes in: at the full tensor rate a 256 x 256 tile needs 64
+// bytes a cycle per SM, 57 are reached, with the tensor pipe active 72 to 82 %
+// (65,536 x 4096 -> 11008: 1.97 ms, 3.0 P op/s, the library's integer product
+// 1.88 ms; a 256 x 512 tile would need 48 but fills TMEM with one accumulator).
+// The tile order keeps a group of weight blocks in L2 while the rows stream, as
+// in the 16-bit mainloops (groups of 4, 8 or 32 blocks instead of 16: 2 to 15 %
+// slower, within noise, 1 % faster).  Tiles are dealt round-robin to the resident pairs: all tiles of
 // a launch are equal up to a few expand k-blocks.
 #include "q8.cuh"
 
@@ -617,7 +621,9 @@ int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
 //
 // Per 64 rows of a block the shared memory moves 32 KB in by TMA, 48 KB
 // through the conversion and 48 KB into the MMAs, about 1000 cycles, against
-// 700 cycles of the SM's share of HBM for the 16 KB of new bytes.
+// 700 cycles of the SM's share of HBM for the 16 KB of new bytes.  Measured:
+// 65,536 x 4096, 8 jobs 111 us (the saved bytes: 41; loads alone 61, without
+// the conversion 80), 18,432 rows of 16 jobs 35 us (12).
 //
 // Long sums are split over several items (SavedItem): each stores its fp32
 // block, and the last to finish adds the blocks in their order, so the result

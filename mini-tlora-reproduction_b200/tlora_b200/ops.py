@@ -498,6 +498,8 @@ class _Call:
         if kept is None:
             args = _CallArgs(rows, d_in, d_out, dtype, st.impl, plan, table, st.scaling, out_rows=plan.perm)
             kept = (args, args.sizes(), {})
+            if len(plan.calls) >= 8:  # scalings that change from call to call
+                plan.calls.clear()
             plan.calls[key] = kept
         self.args, (self.zbytes, self.wbytes), self._scratch = kept
         word = st.err_word
