@@ -243,16 +243,24 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
   return r;
 }
 
+// Largest block of the kernel that holds NV groups a thread, and the blocks that
+// an SM should hold of it (a cap on the registers; 0 = none): with 24 to 32
+// warps an SM enough rows are in flight while others are rounded.
+template <int NV> constexpr int kQuantThreads = NV == 6 ? 256 : NV == 8 || NV == 12 ? 128 : 512;
+template <int NV> constexpr int kQuantBlocks = NV == 6 ? 3 : NV == 8 ? 8 : NV == 12 ? 6 : 0;
+
 // 2^sh threads (32..512) per row, several rows per block; thread t of a row
 // takes the 8-column groups t, t + 2^sh, ...  NV > 0: the row (CS: its products
 // with the column scales) is held in registers between the maximum and the
 // rounding, so it is read once; NV = 0: twice.  Bound by HBM, 2 bytes in and 1
 // out per 16-bit element, if the work around each row is spread over enough
-// elements of a thread: NV up to 16, or 6 where the values are float32 (three
-// blocks an SM then).  65,536 x 4096 bf16: 139 to 148 us (its bytes: 123); with
-// column scales 65,536 x 11,008: 499 us (331).
+// elements of a thread and enough rows are in flight (kQuantBlocks).  65,536 x
+// 4096 bf16: 122 us (its bytes: 123; 148 with twice the registers and half the
+// warps); with column scales 4096 columns 148 us, 11,008 columns 499 (331): two
+// more loads and a product an element, and values held in float32.
 template <class T, bool VEC, bool CS, int NV>
-__global__ void __launch_bounds__(NV == 6 ? 256 : 512, NV == 6 ? 3 : 0) k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
+__global__ void __launch_bounds__(kQuantThreads<NV>, kQuantBlocks<NV>)
+    k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
                                                    const float* __restrict__ col_scale, int8_t* __restrict__ q,
                                                    float* __restrict__ scale, int sh) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product after it may start
@@ -361,17 +369,18 @@ int launch_quantize(const T* src, int64_t rows, int64_t cols, int64_t ld, const 
                     cudaStream_t st) {
   const int64_t groups = q8_ld(cols) / 8;  // the zero bytes past `cols` included
   constexpr bool kWide = CS || sizeof(T) == 4;  // held as float32
-  const RowGrid g = row_grid(rows, groups, !kWide ? 16 : CS && sizeof(T) == 4 ? 4 : 6);
+  const RowGrid g = row_grid(rows, groups, !kWide ? 12 : CS && sizeof(T) == 4 ? 4 : 6);
 #define MLORA_QUANT(NV) \
   k_quantize<T, VEC, CS, NV><<<g.grid, g.block, 0, st>>>(src, rows, int(cols), ld, cs, q, scale, g.sh)
   if (g.nv <= 1) MLORA_QUANT(1);
   else if (g.nv <= 2) MLORA_QUANT(2);
   else if (g.nv <= 3) MLORA_QUANT(3);
   else if (g.nv <= 4) MLORA_QUANT(4);
-  else if (g.nv <= 6 && g.block <= 256) MLORA_QUANT(6);  // three blocks an SM: 65,536 x 11,008 554 -> 499 us
-  else if (g.nv <= 8) MLORA_QUANT(8);
-  else if (!kWide && g.nv <= 12) MLORA_QUANT((kWide ? 0 : 12));
-  else if (!kWide && g.nv <= 16) MLORA_QUANT((kWide ? 0 : 16));
+  else if (g.nv <= 6 && g.block <= kQuantThreads<6>) MLORA_QUANT(6);
+  else if (g.nv <= 8 && g.block <= kQuantThreads<8>) MLORA_QUANT(8);
+  else if (!kWide && g.nv <= 12 && g.block <= kQuantThreads<12>) MLORA_QUANT((kWide ? 0 : 12));
+  else if (!kWide && g.nv <= 16) MLORA_QUANT((kWide ? 0 : 16));  // rows over larger blocks
+  else if (kWide && g.nv <= 10) MLORA_QUANT((kWide ? 10 : 0));
   else MLORA_QUANT(0);
 #undef MLORA_QUANT
   count_launch();

@@ -108,6 +108,7 @@ def problem(rows=4, d_in=64, d_out=32, dtype=_lib.BF16, max_ctas=0):
     ((P, 4, 0, 16, _lib.BF16, None, P, P), _lib.ERR_INVALID_ARG),
     ((P, 4, 16, 15, _lib.BF16, None, P, P), _lib.ERR_INVALID_ARG),   # rows overlap
     ((P, 4, 16, 16, 7, None, P, P), _lib.ERR_UNSUPPORTED),
+    ((P, 4, (1 << 30) + 1, 1 << 31, _lib.BF16, None, P, P), _lib.ERR_UNSUPPORTED),
     ((None, 4, 16, 16, _lib.BF16, None, P, P), _lib.ERR_INVALID_ARG),
     ((P, 4, 16, 16, _lib.BF16, None, None, P), _lib.ERR_INVALID_ARG),
     ((P, 4, 16, 16, _lib.BF16, None, ODD, P), _lib.ERR_UNSUPPORTED),  # 8-bit rows start on 16 bytes
