@@ -74,6 +74,7 @@ class AdapterTable:
     r_pack: int
     _dev_keys: dict = field(default_factory=dict, repr=False)
     _spans: Optional[list] = field(default=None, repr=False)
+    _pieces: Optional[list] = field(default=None, repr=False)
 
     @staticmethod
     def build(ids: Sequence[int], ranks: Sequence[int]) -> "AdapterTable":
@@ -93,6 +94,13 @@ class AdapterTable:
         if self._spans is None:
             self._spans = [(int(o), int(r)) for o, r in zip(self.pack_off, self.rank)]
         return self._spans
+
+    def pieces(self) -> list:
+        """Lengths that cut the packed ranks into rank, padding, rank, padding, ..."""
+        if self._pieces is None:
+            ends = [o for o, _ in self.spans()[1:]] + [self.r_pack]
+            self._pieces = [n for (o, r), e in zip(self.spans(), ends) for n in (r, e - o - r)]
+        return self._pieces
 
     def slot_of(self) -> dict:
         return {a: i for i, a in enumerate(self.ids)}
@@ -826,14 +834,18 @@ class MultiLoRAFunction(torch.autograd.Function):
         rows8 = _wrap8(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
         need = ctx.needs_input_grad
         dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
+        # one call cuts a pack into all adapters' gradients
+        cut = st.table.pieces()
+        pa = torch.unsafe_split_with_sizes(dA, cut, 0) if dA is not None else None
+        pb = torch.unsafe_split_with_sizes(dB, cut, 1) if dB is not None else None
         grads = [None] * (2 * st.table.n)
-        for i, ((o, r), act) in enumerate(zip(st.table.spans(), st.plan.active.tolist())):
+        for i, act in enumerate(st.plan.active.tolist()):
             if not act:
                 continue
             if need[4 + 2 * i]:
-                grads[2 * i] = dA.narrow(0, o, r)
+                grads[2 * i] = pa[2 * i]
             if need[5 + 2 * i]:
-                grads[2 * i + 1] = dB.narrow(1, o, r)
+                grads[2 * i + 1] = pb[2 * i]
         return (dx, None, None, None, *grads)
 
 
