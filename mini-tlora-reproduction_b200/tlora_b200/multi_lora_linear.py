@@ -72,7 +72,8 @@ class Int8Base(nn.Module):
         self.in_features, self.out_features = rows8.cols, rows8.rows
         self.register_buffer("weight_q8", rows8.q)
         self.register_buffer("weight_scale", rows8.scale)
-        self.bias = nn.Parameter(bias.detach().clone(), requires_grad=False) if bias is not None else None
+        self.register_parameter(
+            "bias", nn.Parameter(bias.detach().clone(), requires_grad=False) if bias is not None else None)
 
     @classmethod
     def from_linear(cls, base: nn.Linear) -> "Int8Base":
@@ -135,8 +136,8 @@ class _Int8BaseMixin:
 
     def _base_operands(self):
         """(W or None, 8-bit rows or None, bias)."""
-        b = self.base
-        return (None, b.rows8, b.bias) if isinstance(b, Int8Base) else (b.weight, None, b.bias)
+        b = self._modules["base"]
+        return (None, b.rows8, b._parameters["bias"]) if isinstance(b, Int8Base) else (b.weight, None, b.bias)
 
 
 _SAVE_INPUT = ("full", "int8")
@@ -195,12 +196,7 @@ class _PackedAdapters:
 
     def params(self) -> list:
         """A_0, B_0, A_1, ... as the adapters hold them now."""
-        out = []
-        for ad in self.adapters:
-            p = ad._parameters
-            out.append(p["A"])
-            out.append(p["B"])
-        return out
+        return [p[k] for p in [ad._parameters for ad in self.adapters] for k in ("A", "B")]
 
     def _in_sync(self, params) -> bool:
         # a parameter that no longer views the packs has another address: the
@@ -317,7 +313,7 @@ class MultiLoRALinear(_Int8BaseMixin, nn.Module):
         return self.adapters[str(adapter_id)].parameters()
 
     def _pack(self) -> _PackedAdapters:
-        ads = self.adapters._modules
+        ads = self._modules["adapters"]._modules
         if self._packed is None or not self._packed.owns(ads):
             self._packed = _PackedAdapters(ads)
         return self._packed

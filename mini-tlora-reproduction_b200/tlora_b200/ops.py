@@ -75,6 +75,7 @@ class AdapterTable:
     _dev_keys: dict = field(default_factory=dict, repr=False)
     _spans: Optional[list] = field(default=None, repr=False)
     _pieces: Optional[list] = field(default=None, repr=False)
+    _layout: Optional[bytes] = field(default=None, repr=False)
 
     @staticmethod
     def build(ids: Sequence[int], ranks: Sequence[int]) -> "AdapterTable":
@@ -94,6 +95,12 @@ class AdapterTable:
         if self._spans is None:
             self._spans = [(int(o), int(r)) for o, r in zip(self.pack_off, self.rank)]
         return self._spans
+
+    def layout(self) -> bytes:
+        """The ranks and packed offsets, as a key."""
+        if self._layout is None:
+            self._layout = self.rank.tobytes() + self.pack_off.tobytes()
+        return self._layout
 
     def pieces(self) -> list:
         """Lengths that cut the packed ranks into rank, padding, rank, padding, ..."""
@@ -501,7 +508,7 @@ class _Call:
 
     def __init__(self, rows, d_in, d_out, dtype, st: "LayerState"):
         plan, table = st.plan, st.table
-        key = (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.rank.tobytes(), st.scaling.tobytes())
+        key = (rows, d_in, d_out, dtype, st.impl, table.layout(), st.scaling.tobytes())
         kept = plan.calls.get(key)
         if kept is None:
             args = _CallArgs(rows, d_in, d_out, dtype, st.impl, plan, table, st.scaling, out_rows=plan.perm)
