@@ -292,9 +292,11 @@ int launch_q8_few(const Q8Main& a, Q8After after, cudaStream_t st) {
 
 }  // namespace
 
-// The weight-streaming kernel takes up to 16 rows of the forward; above, the
-// tensor-memory tiles read the weight as often (once) and do the products
-// faster.
+// The weight-streaming kernel takes up to 16 rows of the forward.  Measured at 16
+// rows against the tensor-memory tiles (17 rows): 4096 -> 4096 8.7 and 17.3 us,
+// 4096 -> 11008 17.5 and 18.3, 8192 -> 8192 19.7 and 27.5.  With four groups of
+// eight rows it took 13 to 16, 32 to 34 and 38 to 42 us for 17 to 31 rows: the
+// tiles are faster there on all but the smallest layers.
 bool q8_few_ok(const Q8Main& a) {
   return !a.bwd && a.M <= kQ8Few &&
          (!a.expand || (aligned(a.zt, 16) && aligned(a.pack, 16)));  // 16-byte loads of the expand

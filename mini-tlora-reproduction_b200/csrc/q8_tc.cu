@@ -20,14 +20,16 @@
 // accumulator: its expand k-blocks sit in the ring after the first kDefer
 // k-blocks of the next tile, by which time the rewrite has finished.
 //
-// Bound by what an SM takes in: at the full tensor rate a 256 x 256 tile needs 64
-// bytes a cycle per SM, 57 are reached, with the tensor pipe active 72 to 82 %
-// (65,536 x 4096 -> 11008: 1.97 ms, 3.0 P op/s, the library's integer product
-// 1.88 ms; a 256 x 512 tile would need 48 but fills TMEM with one accumulator).
+// Bound by power on large shapes: the tensor pipe is active 70 to 82 % at 1.6 to
+// 1.65 GHz under the cap (65,536 x 4096 -> 11008: 1.97 ms, 3.0 P op/s; the
+// library's integer product 1.88 ms).  At the full rate a 256 x 256 tile also
+// takes 64 bytes a cycle into each SM, of which 57 are reached; tiles of 256 x
+// 512, which need 48, were built and timed in turn with these: 1 to 3 % faster
+// from K = 8192 on, none at K = 4096, slower with few tiles, and not kept.
 // The tile order keeps a group of weight blocks in L2 while the rows stream, as
 // in the 16-bit mainloops (groups of 4, 8 or 32 blocks instead of 16: 2 to 15 %
-// slower, within noise, 1 % faster).  Tiles are dealt round-robin to the resident pairs: all tiles of
-// a launch are equal up to a few expand k-blocks.
+// slower, within noise, 1 % faster).  Tiles are dealt round-robin to the
+// resident pairs: all tiles of a launch are equal up to a few expand k-blocks.
 #include "q8.cuh"
 
 namespace mlora {

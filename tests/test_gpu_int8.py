@@ -264,6 +264,9 @@ LAYERS = {
     # several tiles per pair of SMs, with fewer and with more k-blocks than a tile's expand waits for
     "many_tiles_short": (264, 2312, {0: 24, 1: 64, 2: 100}, grouped((0, 2100), (-1, 300), (1, 1200), (2, 1500))),
     "many_tiles": (2048, 2312, {i: 16 for i in range(9)}, torch.arange(9).repeat_interleave(563)),
+    # long contractions over many tiles, forward and backward
+    "long_rows": (8200, 3000, {0: 16, 1: 130}, grouped((0, 2500), (-1, 500), (1, 2700))),
+    "long_columns": (2560, 8448, {i: 8 for i in range(4)}, torch.arange(4).repeat_interleave(1700)),
     # sums over rows long enough to be split
     "long_jobs": (520, 72, {0: 100, 1: 8}, grouped((0, 6000), (1, 4500))),
     "wide": (72, 2056, {0: 24, 1: 64}, grouped((0, 400), (1, 200))),
