@@ -33,13 +33,17 @@ class GraphedTrainStep:
                  lr: float, warmup: int = 3, need_dx: bool = True):
         if x.device.type != "cuda":
             raise RuntimeError("CUDA graphs need CUDA tensors")
+        if dy.shape != (x.shape[0], model.base.out_features):
+            raise ValueError(f"dy has shape {tuple(dy.shape)}, the output {(x.shape[0], model.base.out_features)}")
+        if dy.device != x.device:
+            raise RuntimeError(f"input on {x.device} but dy on {dy.device}")
         self.model = model
         self.lr = float(lr)
         self.plan = model.route(adapter_ids.cpu(), device=x.device)
         model.make_resident(self.plan)
         self.ids = adapter_ids.cpu()
         self.x = x.detach().clone().requires_grad_(need_dx)
-        self.dy = dy.detach().clone()
+        self.dy = dy.detach().to(x.dtype, copy=True)  # the output's type, as autograd casts it
         side = torch.cuda.Stream(x.device)
         side.wait_stream(torch.cuda.current_stream(x.device))
         with torch.cuda.stream(side):  # warm-up off the default stream, as capture requires

@@ -689,12 +689,22 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     dX rows are written straight to their original positions.  With an 8-bit
     backbone or ``rows8`` (the 8-bit rows of the sorted input, in place of
     ``xs``) the call is mlora_backward_q8."""
-    rows = dy.shape[0]
-    d_in = st.A_pack.shape[1]
-    d_out = st.B_pack.shape[0]
-    dev = dy.device
+    rows, d_in, d_out = st.plan.rows, st.A_pack.shape[1], st.B_pack.shape[0]
+    dev, dt = st.B_pack.device, st.B_pack.dtype
+    # the kernels take their strides and types from the layer: nothing else may differ
+    if dy.shape != (rows, d_out):
+        raise ValueError(f"dy has shape {tuple(dy.shape)}, the output {(rows, d_out)}")
+    if dy.dtype != dt or dy.device != dev:
+        raise RuntimeError(f"dy is {dy.dtype} on {dy.device}, the layer {dt} on {dev}")
+    if (xs is not None and (xs.shape != (rows, d_in) or xs.dtype != dt or xs.device != dev)) or (
+            rows8 is not None and (rows8.shape != (rows, d_in) or rows8.device != dev)):
+        raise ValueError(f"the saved input is not that of a call of {rows} rows and {d_in} features")
+    args = _Call(rows, d_in, d_out, mlora_dtype(dt), st)
+    if z.numel() * z.element_size() < args.zbytes:
+        raise ValueError(f"the saved intermediate has {z.numel() * z.element_size()} bytes, the call {args.zbytes}")
+    dy = dy.contiguous()
+    xs = xs.contiguous() if xs is not None else None
     dys = gather_rows(dy, st.plan.perm) if st.plan.perm is not None else dy
-    args = _Call(rows, d_in, d_out, mlora_dtype(dy.dtype), st)
     wb = args.wbytes
     ws, args.prob.flags = _workspace(st, args, wb, dev)
     dx = torch.empty(rows, d_in, dtype=dy.dtype, device=dev) if want_dx else None
