@@ -508,6 +508,13 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
       if (st != MLORA_OK) return st;
     }
     if (!dB_pack || !(stages & MLORA_BWD_DB)) return MLORA_OK;
+    // q8_sum32 reads the low-rank blocks 16 bytes at a time.  dZ lies in the
+    // workspace, zsave where the caller has it: off such a boundary the
+    // reduction that reads single elements takes its place
+    if (!aligned(zsave, 16))
+      return backward_kernels(prob, route, p, dev, MLORA_IMPL_SIMT, dY, nullptr, W, A_pack, B_pack, zsave, dzsave,
+                              nullptr, nullptr, dB_pack, stages & (MLORA_BWD_DB | MLORA_BWD_SGD_B), 0, p.n_tiles, 0,
+                              nb_out, nullptr, s);
     float* upd = (stages & MLORA_BWD_SGD_B) ? (float*)const_cast<void*>(B_pack) : nullptr;
     return q8_sum32(1, dev, nullptr, nullptr, (const float*)dY, (const float*)zsave, (float*)dB_pack, prob->rows,
                     prob->d_out, route->r_pack, upd, prob->lr, s);

@@ -2,6 +2,8 @@
 besides the values of test_gpu_int8.py: graphed steps, shared plans, hooks,
 unusual types and buffers."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -79,3 +81,78 @@ def test_graphed_step_refuses_other_gradients():
             GraphedTrainStep(m, x, IDS, bad, lr=0.0)
     with pytest.raises(RuntimeError, match="dy"):
         GraphedTrainStep(m, x, IDS, torch.zeros(rows, 192, dtype=BF), lr=0.0)
+
+
+# ------------------------------------------------------------------ buffers of a native caller
+
+def odd(t):
+    """A copy of t that starts one element past a 256-byte boundary."""
+    if t is None:
+        return None
+    buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    out = buf[1:].view(t.shape)
+    out.copy_(t)
+    assert out.data_ptr() % 16 == t.element_size()
+    return out
+
+
+def native_step(m, x, ids, dy, where, save8=True):
+    """One forward and backward through the C entry points; ``where`` places
+    every tensor of the caller's that has the layer's type."""
+    dt, (rows, d_in), d_out = x.dtype, x.shape, dy.shape[1]
+    pk, plan, b8 = m._pack(), m.route(ids), m.base.rows8
+    pk.sync()
+    st = pk.state(plan, m.impl, b8, save8)
+    call = ops._Call(rows, d_in, d_out, ops.mlora_dtype(dt), st)
+    A, B, bias = where(pk.A_pack), where(pk.B_pack), where(m.base.bias.detach())
+    x, dy = where(x), where(dy)
+    y, dx = where(torch.zeros(rows, d_out, device="cuda", dtype=dt)), where(torch.zeros_like(x))
+    dA, dB = where(torch.zeros_like(A)), where(torch.zeros_like(B))
+    z = where(torch.zeros(max(1, call.zbytes // x.element_size()), device="cuda", dtype=dt))
+    ws = torch.empty(call.wbytes, dtype=torch.uint8, device="cuda")
+    r8, g8 = ops._new_rows8(rows, d_in, x.device), ops._Scratch8(rows, d_out, x.device)
+    q8 = ops._q8_struct(b8, r8, g8)
+    s, p, r = ops._stream(x.device), ctypes.byref(call.prob), ctypes.byref(call.route)
+    ptr = ops._ptr
+    _lib.call("mlora_forward_q8", p, r, ctypes.byref(q8), ptr(x), None, ptr(bias), ptr(A), ptr(B), ptr(y), ptr(z),
+              ptr(ws), call.wbytes, s)
+    scratch = torch.empty(max(1, call.scratch8()), dtype=torch.uint8, device="cuda")
+    q8.scratch, q8.scratch_bytes = scratch.data_ptr(), call.scratch8()
+    if not save8:
+        q8.Xq = q8.x_scale = None
+    _lib.call("mlora_backward_q8", p, r, ctypes.byref(q8), ptr(dy), None if save8 else ptr(x), None, ptr(A), ptr(B),
+              ptr(z), ptr(dx), ptr(dA), ptr(dB), ptr(ws), call.wbytes, s)
+    torch.cuda.synchronize()
+    act = plan.active
+    return (y, dx, [dA[o:o + k] if act[i] else None for i, (o, k) in enumerate(pk.table.spans())],
+            [dB[:, o:o + k] if act[i] else None for i, (o, k) in enumerate(pk.table.spans())])
+
+
+def check(m, w, x, ids, dy, got, base8=True, save8=True):
+    ads = [(a.A.detach(), a.B.detach(), a.scaling) for a in m.adapters.values()]
+    slot = torch.full_like(ids, -1).cuda()
+    for i, k in enumerate(m.adapters):
+        slot[ids.cuda() == int(k)] = i
+    y, dx, dA, dB = ref.lora(x, slot, w, m.base.bias, ads, dy, base8, save8)
+    ref.assert_within(got[0], *y, what="y")
+    ref.assert_within(got[1], *dx, what="dx")
+    for i in range(len(ads)):
+        if dA[i] is None:
+            assert got[2][i] is None and got[3][i] is None
+            continue
+        ref.assert_within(got[2][i], *dA[i], what=f"dA{i}")
+        ref.assert_within(got[3][i], *dB[i], what=f"dB{i}")
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("rows", [5, 262])
+@pytest.mark.parametrize("dt", [F32, BF, FP])
+def test_buffers_aligned_to_their_elements_only(dt, rows, save8):
+    m = layer(256, 192, RANKS, dt)
+    w = m.base.weight.detach().clone()
+    m.quantize_base()
+    ids = IDS[torch.linspace(0, len(IDS) - 1, rows).long()]
+    x, dy = randn((rows, 256), dt, 1), randn((rows, 192), dt, 2, 0.1)
+    for where in (odd, lambda t: t.clone()):
+        check(m, w, x, ids, dy, native_step(m, x, ids, dy, where, save8), save8=save8)
