@@ -73,9 +73,7 @@ class AdapterTable:
     pack_off: np.ndarray  # int32 [n]
     r_pack: int
     _dev_keys: dict = field(default_factory=dict, repr=False)
-    _spans: Optional[list] = field(default=None, repr=False)
-    _pieces: Optional[list] = field(default=None, repr=False)
-    _layout: Optional[bytes] = field(default=None, repr=False)
+    _cuts: Optional[tuple] = field(default=None, init=False, repr=False)
 
     @staticmethod
     def build(ids: Sequence[int], ranks: Sequence[int]) -> "AdapterTable":
@@ -90,24 +88,32 @@ class AdapterTable:
     def n(self) -> int:
         return len(self.ids)
 
-    def spans(self) -> list:
-        """(first packed row, rank) of every slot, as plain integers."""
-        if self._spans is None:
-            self._spans = [(int(o), int(r)) for o, r in zip(self.pack_off, self.rank)]
-        return self._spans
-
     def layout(self) -> bytes:
         """The ranks and packed offsets, as a key."""
-        if self._layout is None:
-            self._layout = self.rank.tobytes() + self.pack_off.tobytes()
-        return self._layout
+        return self.rank.tobytes() + self.pack_off.tobytes()
 
-    def pieces(self) -> list:
-        """Lengths that cut the packed ranks into rank, padding, rank, padding, ..."""
-        if self._pieces is None:
-            ends = [o for o, _ in self.spans()[1:]] + [self.r_pack]
-            self._pieces = [n for (o, r), e in zip(self.spans(), ends) for n in (r, e - o - r)]
-        return self._pieces
+    def _cut(self) -> tuple:
+        """(layout, spans, pieces, their places), computed once per layout."""
+        key = self.layout()
+        if self._cuts is None or self._cuts[0] != key:
+            spans = [(int(o), int(r)) for o, r in zip(self.pack_off, self.rank)]
+            pieces, place, end = [], [0] * self.n, 0
+            for i in sorted(range(self.n), key=lambda i: spans[i]):
+                o, r = spans[i]
+                place[i] = len(pieces) + 1
+                pieces += [o - end, r]
+                end = o + r
+            self._cuts = (key, spans, pieces + [self.r_pack - end], place)
+        return self._cuts
+
+    def spans(self) -> list:
+        """(first packed row, rank) of every slot, as plain integers."""
+        return self._cut()[1]
+
+    def pieces(self) -> tuple:
+        """Lengths that cut the packed ranks into gaps and adapters, and the
+        place of every slot's among them."""
+        return self._cut()[2:]
 
     def slot_of(self) -> dict:
         return {a: i for i, a in enumerate(self.ids)}
@@ -137,9 +143,9 @@ class RoutePlan:
     # workspaces that already hold this plan on the device (make_resident),
     # keyed by the call shape; calls with such a key upload nothing
     resident: dict = field(default_factory=dict)
-    # the C descriptions of calls made with this plan, by call shape and
-    # adapter layout (built once)
-    calls: dict = field(default_factory=dict, repr=False)
+    # the C descriptions of calls made with this plan, by all that they hold
+    # (its segments among it: a plan that changes gets new ones)
+    calls: dict = field(default_factory=dict, init=False, repr=False)
 
     def __getstate__(self):
         return {**self.__dict__, "calls": {}}  # C structures are neither copied nor pickled
@@ -501,19 +507,25 @@ class _CallArgs:
 
 
 class _Call:
-    """One call made with a routing plan: a fresh mlora_problem over the plan's
-    kept mlora_routing and buffer sizes."""
+    """One call made with a routing plan: a fresh mlora_problem over a
+    mlora_routing and buffer sizes kept for the plan's present content."""
 
     __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "_scratch")
 
     def __init__(self, rows, d_in, d_out, dtype, st: "LayerState"):
         plan, table = st.plan, st.table
-        key = (rows, d_in, d_out, dtype, st.impl, table.layout(), st.scaling.tobytes())
+        perm = plan.perm
+        key = (rows, d_in, d_out, dtype, st.impl, table.layout(), st.scaling.tobytes(), plan.seg_start.tobytes(),
+               plan.seg_adapter.tobytes(), None if perm is None else perm.data_ptr())
         kept = plan.calls.get(key)
         if kept is None:
-            args = _CallArgs(rows, d_in, d_out, dtype, st.impl, plan, table, st.scaling, out_rows=plan.perm)
+            # copies: what is kept must not change with the caller's arrays
+            args = _CallArgs(rows, d_in, d_out, dtype, st.impl,
+                             RoutePlan(plan.rows, plan.seg_start.copy(), plan.seg_adapter.copy()),
+                             AdapterTable(table.ids, table.rank.copy(), table.pack_off.copy(), table.r_pack),
+                             st.scaling.copy(), out_rows=perm)
             kept = (args, args.sizes(), {})
-            if len(plan.calls) >= 8:  # scalings that change from call to call
+            if len(plan.calls) >= 8:  # plans or scalings that change from call to call
                 plan.calls.clear()
             plan.calls[key] = kept
         self.args, (self.zbytes, self.wbytes), self._scratch = kept
@@ -852,7 +864,7 @@ class MultiLoRAFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
         # one call cuts a pack into all adapters' gradients
-        cut = st.table.pieces()
+        cut, place = st.table.pieces()
         pa = torch.unsafe_split_with_sizes(dA, cut, 0) if dA is not None else None
         pb = torch.unsafe_split_with_sizes(dB, cut, 1) if dB is not None else None
         grads = [None] * (2 * st.table.n)
@@ -860,9 +872,9 @@ class MultiLoRAFunction(torch.autograd.Function):
             if not act:
                 continue
             if need[4 + 2 * i]:
-                grads[2 * i] = pa[2 * i]
+                grads[2 * i] = pa[place[i]]
             if need[5 + 2 * i]:
-                grads[2 * i + 1] = pb[2 * i]
+                grads[2 * i + 1] = pb[place[i]]
         return (dx, None, None, None, *grads)
 
 

@@ -49,3 +49,79 @@ def test_saved_tensors_of_another_call():
         backward(state(), dy, None, rows8=ops.Int8Rows(torch.zeros(40, 64, dtype=torch.int8), torch.ones(40), 63))
     with pytest.raises(ValueError, match="saved intermediate"):
         backward(state(), dy, z=torch.zeros(16, dtype=torch.uint8))
+
+
+# ------------------------------------------------------------------ plans that change between calls
+
+def call_of(st, rows=40):
+    return ops._Call(rows, 64, 48, ops.mlora_dtype(BF), st)
+
+
+def segments(call):
+    r = call.route
+    return [r.seg_start[i] for i in range(r.n_seg + 1)], [r.seg_adapter[i] for i in range(r.n_seg)]
+
+
+def test_calls_follow_a_plan_whose_arrays_are_replaced():
+    st = state()
+    assert segments(call_of(st)) == ([0, 20, 40], [0, 1])
+    st.plan.seg_start = np.array([0, 5, 40], np.int32)
+    assert segments(call_of(st)) == ([0, 5, 40], [0, 1])
+    st.plan.seg_adapter = np.array([1, -1], np.int32)
+    assert segments(call_of(st)) == ([0, 5, 40], [1, -1])
+    st.plan.perm = torch.arange(40, dtype=torch.int32)
+    assert call_of(st).route.out_rows == st.plan.perm.data_ptr()
+    st.plan.perm = None
+    assert call_of(st).route.out_rows is None
+
+
+def test_calls_follow_a_plan_edited_in_place():
+    st = state(rows=600)
+    st.plan.seg_start[:] = [0, 100, 600]   # the tiles of adapter 1: 0 to 2 instead of 1 to 2
+    assert segments(call_of(st, 600)) == ([0, 100, 600], [0, 1])
+    before = call_of(st, 600).zbytes
+    st.plan.seg_start[:] = [0, 600, 600]   # one adapter, one chunk a tile
+    after = call_of(st, 600)
+    assert segments(after) == ([0, 600, 600], [0, 1])
+    assert after.zbytes == 3 * 256 * 64 * 2 and before == 4 * 256 * 64 * 2
+    st.plan.seg_start[:] = [0, 300, 600]
+    assert call_of(st, 600).zbytes == 4 * 256 * 64 * 2
+
+
+def test_calls_follow_a_replaced_plan():
+    import dataclasses
+
+    st = state()
+    call_of(st)
+    st.plan = dataclasses.replace(st.plan, seg_start=np.array([0, 7, 40], np.int32))
+    assert segments(call_of(st)) == ([0, 7, 40], [0, 1])
+
+
+def test_kept_descriptions_are_copies():
+    st = state()
+    kept = st.plan.seg_start
+    call_of(st)
+    kept[:] = [0, 9, 40]
+    call_of(st)
+    st.plan.seg_start = np.array([0, 20, 40], np.int32)  # as it was, in another array
+    assert segments(call_of(st)) == ([0, 20, 40], [0, 1])
+    st.scaling[1] = 3.0
+    assert call_of(st).route.scaling[1] == 3.0
+    st.scaling = np.array([0.5, 0.75], np.float32)
+    assert call_of(st).route.scaling[1] == 0.75
+
+
+def test_tables_follow_their_ranks():
+    import dataclasses
+
+    table = ops.AdapterTable.build([0, 1], [8, 16])
+    first = table.layout()
+    assert table.spans() == [(0, 8), (64, 16)] and table.pieces() == ([0, 8, 56, 16, 48], [1, 3])
+    other = dataclasses.replace(table, rank=np.array([4, 20], np.int32))
+    assert other.spans() == [(0, 4), (64, 20)] and other.pieces() == ([0, 4, 60, 20, 44], [1, 3])
+    table.rank[0] = 2
+    assert table.spans() == [(0, 2), (64, 16)] and table.pieces() == ([0, 2, 62, 16, 48], [1, 3])
+    assert len({first, other.layout(), table.layout()}) == 3
+    # packed in another order, with a gap before the first
+    third = ops.AdapterTable([5, 7], np.array([8, 64], np.int32), np.array([128, 64], np.int32), 192)
+    assert third.pieces() == ([64, 64, 0, 8, 56], [3, 1])
