@@ -332,10 +332,12 @@ class MultiLoRALinear(_Int8BaseMixin, nn.Module):
         """Upload the routing ``plan`` once into a device workspace kept on the
         plan; calls with ``plan=plan`` then issue no host-to-device copy, so a
         training step with fixed routing can be captured into a CUDA graph
-        (tlora_b200.graphs.GraphedTrainStep).  The adapters' ranks and
-        scalings must not change afterwards.  Calls with one plan share its
-        workspace: they must follow one another (one stream, or streams that
-        wait for each other)."""
+        (tlora_b200.graphs.GraphedTrainStep).  Every layer that uses the plan
+        calls this; layers of one shape with the same ranks and scalings share
+        a workspace, whose calls must follow one another (one stream, or
+        streams that wait for each other).  After a change of the plan or of
+        the adapters' ranks or scalings call it again (until then calls upload
+        what changed; a captured graph keeps what it was captured with)."""
         pk = self._pack()
         pk.sync()
         st = ops.LayerState(pk.table, pk.scaling(), plan, pk.A_pack, pk.B_pack, self.impl)

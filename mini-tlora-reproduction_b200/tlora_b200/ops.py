@@ -141,7 +141,7 @@ class RoutePlan:
     perm: Optional[torch.Tensor] = None  # int32 [rows] on device: sorted position -> source row
     active: np.ndarray = None            # bool [n_adapters]: adapter owns >= 1 row
     # workspaces that already hold this plan on the device (make_resident),
-    # keyed by the call shape; calls with such a key upload nothing
+    # keyed by all that its tables hold; calls with such a key upload nothing
     resident: dict = field(default_factory=dict)
     # the C descriptions of calls made with this plan, by all that they hold
     # (its segments among it: a plan that changes gets new ones)
@@ -506,17 +506,24 @@ class _CallArgs:
         return int(z.value), int(w.value)
 
 
+def _call_key(rows, d_in, d_out, dtype, st: "LayerState") -> tuple:
+    """All that the routing tables of a call are made from."""
+    plan, table = st.plan, st.table
+    return (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.layout(), st.scaling.tobytes(),
+            plan.seg_start.tobytes(), plan.seg_adapter.tobytes())
+
+
 class _Call:
     """One call made with a routing plan: a fresh mlora_problem over a
     mlora_routing and buffer sizes kept for the plan's present content."""
 
-    __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "_scratch")
+    __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "key", "_scratch")
 
     def __init__(self, rows, d_in, d_out, dtype, st: "LayerState"):
         plan, table = st.plan, st.table
         perm = plan.perm
-        key = (rows, d_in, d_out, dtype, st.impl, table.layout(), st.scaling.tobytes(), plan.seg_start.tobytes(),
-               plan.seg_adapter.tobytes(), None if perm is None else perm.data_ptr())
+        self.key = _call_key(rows, d_in, d_out, dtype, st)
+        key = (self.key, None if perm is None else perm.data_ptr())
         kept = plan.calls.get(key)
         if kept is None:
             # copies: what is kept must not change with the caller's arrays
@@ -566,19 +573,16 @@ class LayerState:
     save8: bool = False
 
 
-def _resident_key(rows, d_in, d_out, dtype, st: LayerState):
-    return (int(rows), int(d_in), int(d_out), int(dtype), st.impl, int(st.table.r_pack))
-
-
 def make_resident(st: LayerState, rows: int, d_in: int, d_out: int, dtype: torch.dtype, device) -> torch.Tensor:
     """Upload the routing plan of ``st`` for calls of this shape into a
     workspace kept on the plan (mlora_plan_upload); later forward / backward
     calls with the same plan and shape then issue no host-to-device copy
     (MLORA_PLAN_RESIDENT), which lets a training step be captured into a
-    CUDA graph.  The plan must not change afterwards (same ids, ranks and
-    scalings)."""
+    CUDA graph.  Ranks, scalings and segments are part of the uploaded tables:
+    layers that differ in them get a workspace each, and a captured graph keeps
+    to those it was captured with."""
     code = mlora_dtype(dtype)
-    key = _resident_key(rows, d_in, d_out, code, st)
+    key = _call_key(rows, d_in, d_out, code, st)
     if key in st.plan.resident:
         return st.plan.resident[key]
     args = _CallArgs(rows, d_in, d_out, code, st.impl, st.plan, st.table, st.scaling)
@@ -592,8 +596,11 @@ def make_resident(st: LayerState, rows: int, d_in: int, d_out: int, dtype: torch
 def _workspace(st: LayerState, args, wb, device):
     """(workspace, flags) of a call: the plan's resident workspace when there
     is one for this shape, else a fresh one the call uploads the plan into."""
-    p = args.prob
-    ws = st.plan.resident.get(_resident_key(p.rows, p.d_in, p.d_out, p.dtype, st))
+    ws = None
+    if st.plan.resident:
+        p = args.prob
+        ws = st.plan.resident.get(args.key if isinstance(args, _Call) else
+                                  _call_key(p.rows, p.d_in, p.d_out, p.dtype, st))
     if ws is not None and ws.numel() >= wb and ws.device == device:
         return ws, _lib.PLAN_RESIDENT
     return torch.empty(max(wb, 1), dtype=torch.uint8, device=device), 0

@@ -83,6 +83,46 @@ def test_graphed_step_refuses_other_gradients():
         GraphedTrainStep(m, x, IDS, torch.zeros(rows, 192, dtype=BF), lr=0.0)
 
 
+# ------------------------------------------------------------------ plans
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_layers_share_a_resident_plan(dt, eight):
+    # one shape and one packed size, other scalings or ranks
+    layers = [layer(256, 192, r, dt, seed=i) for i, r in enumerate((RANKS, RANKS, {0: 72, 1: 3, 2: 64}))]
+    for ad in layers[1].adapters.values():
+        ad.scaling *= 3
+    x, dy = randn((len(IDS), 256), dt, 1), randn((len(IDS), 192), dt, 2, 0.1)
+    for m in layers:
+        if eight:
+            m.quantize_base()
+            m.save_input = "int8"
+    want = [step(m, x, IDS, dy) for m in layers]
+    plan = layers[0].route(IDS)
+    for m in layers:
+        m.make_resident(plan)
+    for _ in range(2):
+        for m, (y, dx, dA, dB) in zip(layers, want):
+            got = step(m, x, IDS, dy, plan)
+            assert torch.equal(got[0], y) and torch.equal(got[1], dx)
+            for a, b in zip(got[2] + got[3], dA + dB):
+                assert torch.equal(a, b)
+    layers[0].adapters["1"].scaling *= 2  # no longer what was uploaded
+    assert torch.equal(step(layers[0], x, IDS, dy, plan)[0], step(layers[0], x, IDS, dy)[0])
+    assert _lib.device_error() == 0
+
+
+def test_a_plan_that_changes_between_calls():
+    m = layer(256, 192, RANKS, BF).quantize_base()
+    x, dy = randn((len(IDS), 256), BF, 1), randn((len(IDS), 192), BF, 2, 0.1)
+    plan = m.route(IDS)
+    for ids in (IDS, IDS.flip(0).contiguous(), IDS):
+        new = m.route(ids)
+        plan.seg_start, plan.seg_adapter, plan.perm = new.seg_start, new.seg_adapter, new.perm
+        for a, b in zip(step(m, x, ids, dy, plan), step(m, x, ids, dy)):
+            assert all(torch.equal(u, v) for u, v in zip(a, b)) if isinstance(a, list) else torch.equal(a, b)
+
+
 # ------------------------------------------------------------------ buffers of a native caller
 
 def odd(t):

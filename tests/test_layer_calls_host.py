@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tlora_b200 import ops
+from tlora_b200 import _lib, ops
 
 BF = torch.bfloat16
 
@@ -125,3 +125,53 @@ def test_tables_follow_their_ranks():
     # packed in another order, with a gap before the first
     third = ops.AdapterTable([5, 7], np.array([8, 64], np.int32), np.array([128, 64], np.int32), 192)
     assert third.pieces() == ([64, 64, 0, 8, 56], [3, 1])
+
+
+# ------------------------------------------------------------------ resident plans
+
+def resident(st, rows=40, d_in=64, d_out=48):
+    """The workspace that a call with this state finds, or None."""
+    call = ops._Call(rows, d_in, d_out, ops.mlora_dtype(BF), st)
+    ws, flags = ops._workspace(st, call, call.wbytes, torch.device("cpu"))
+    return ws if flags & _lib.PLAN_RESIDENT else None
+
+
+@pytest.fixture
+def uploads(monkeypatch):
+    """mlora_plan_upload without a GPU: what it was called for."""
+    seen, call = [], _lib.call
+
+    def fake(name, *args):
+        if name != "mlora_plan_upload":
+            return call(name, *args)
+        seen.append(args)
+    monkeypatch.setattr(_lib, "call", fake)
+    monkeypatch.setattr(ops, "_stream", lambda device: 0)
+    return seen
+
+
+def make(st):
+    return ops.make_resident(st, 40, 64, 48, BF, torch.device("cpu"))
+
+
+def test_layers_of_one_shape_share_a_resident_plan(uploads):
+    # scalings and ranks are part of the uploaded tables
+    one = state(ranks=(64, 128))
+    assert make(one) is make(one) and len(uploads) == 1
+    for other in (state(ranks=(64, 128), scaling=(0.5, 1.0)), state(ranks=(128, 64)), state(ranks=(60, 128))):
+        other.plan = one.plan
+        assert other.table.r_pack == one.table.r_pack
+        assert resident(other) is None
+        ws = make(other)
+        assert ws is not make(one) and resident(other) is ws
+    assert len(uploads) == 4 and resident(one) is make(one)
+
+
+def test_a_changed_plan_is_not_resident(uploads):
+    st = state()
+    make(st)
+    assert resident(st) is not None
+    st.plan.seg_start[:] = [0, 3, 40]
+    assert resident(st) is None
+    make(st)
+    assert resident(st) is not None and len(uploads) == 2
