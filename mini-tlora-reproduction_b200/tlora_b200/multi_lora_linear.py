@@ -267,6 +267,7 @@ class _PackedAdapters:
     def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
               base8: Optional[ops.Int8Rows] = None, save8: bool = False):
         params = self.params()
+        ops._no_tangents(x, W, bias, *params)
         x, Wc, bc = self.operands(x, W, bias, base8, params)
         if plan is None:
             plan = ops.route(ids, self.table, x.device)

@@ -16,6 +16,7 @@ from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import BF16, F16, F32, RANK_CHUNK, TILE_ROWS
@@ -56,6 +57,16 @@ class _on:
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+def _no_tangents(*tensors) -> None:
+    """Forward-mode derivatives are not computed: a tensor that carries one is
+    refused, so that none is lost unseen."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives (jvp) are not computed")
 
 
 # ---------------------------------------------------------------------------
@@ -438,6 +449,7 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
     frozen, like the backbone of ``MultiLoRALinear``."""
     if not isinstance(weight, Int8Rows):
         raise TypeError("int8_linear expects weight as Int8Rows (quantize_rows(W))")
+    _no_tangents(None if isinstance(x, Int8Rows) else x, bias)
     dev = weight.q.device
     if dev.type != "cuda":
         _check_cuda(weight.q, "int8_linear")

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tlora_b200 import _lib, ops
+from tlora_b200 import MultiLoRALinear, _lib, ops
 
 BF = torch.bfloat16
 
@@ -175,3 +175,33 @@ def test_a_changed_plan_is_not_resident(uploads):
     assert resident(st) is None
     make(st)
     assert resident(st) is not None and len(uploads) == 2
+
+
+# ------------------------------------------------------------------ forward-mode derivatives
+
+def test_tensors_with_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    m = MultiLoRALinear(64, 48, {0: 4})
+    ids, x = torch.zeros(3, dtype=torch.int64), torch.ones(3, 64)
+    w8 = ops.Int8Rows(torch.zeros(48, 64, dtype=torch.int8), torch.ones(48), 64)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    m(dual, ids)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    ops.int8_linear(dual, w8)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    ops.int8_linear(x, w8, fw.make_dual(torch.zeros(48), torch.ones(48)))
+        with pytest.raises(RuntimeError, match="CUDA"):  # without a tangent: the usual check
+            m(x, ids)
+    m = MultiLoRALinear(64, 48, {0: 4})
+    for p in (m.adapters["0"].A, m.adapters["0"].B, m.base.weight, m.base.bias):
+        p.requires_grad_(False)
+    with fw.dual_level():
+        for name in ("adapters.0.A", "adapters.0.B", "base.weight", "base.bias"):
+            p = dict(m.named_parameters())[name]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.func.functional_call(m, {name: fw.make_dual(p.detach(), torch.ones_like(p))}, (x, ids))
