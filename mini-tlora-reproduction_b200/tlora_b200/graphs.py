@@ -13,6 +13,11 @@ costs one launch.
     for batch in batches:          # same rows per adapter each step
         y = step(batch.x, batch.dy)
 
+The step is the module's own call and autograd, so its forward and backward
+hooks, the gradient hooks of its parameters and an overridden forward are
+captured with it (what they run on the GPU is replayed; the hooks themselves
+are called while the step is captured, not at each replay).
+
 Inputs are copied into the graph's static buffers before each replay; the
 returned Y, the adapters' .grad and the updated weights live in the graph's
 memory and are overwritten by the next replay.
@@ -23,9 +28,38 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch import nn
 
-from . import ops
-from .multi_lora_linear import MultiLoRALinear, _save8
+from .multi_lora_linear import MultiLoRALinear
+
+
+class _Leaves:
+    """Stands in for a module's trainable parameters while it is called: leaves
+    of their own over the same memory, with the parameters' gradient hooks.
+    Autograd's nodes for the parameters themselves may belong to a graph that
+    still lives on another stream, which a capture must not meet."""
+
+    def __init__(self, module: nn.Module):
+        self.places, self.pairs, made = [], [], {}
+        for mod in module.modules():
+            for name, p in mod._parameters.items():
+                if p is None or not p.requires_grad:
+                    continue
+                if id(p) not in made:
+                    made[id(p)] = leaf = nn.Parameter(p.detach())
+                    if p._backward_hooks:
+                        leaf._backward_hooks = p._backward_hooks
+                    self.pairs.append((p, leaf))
+                self.places.append((mod, name, p, made[id(p)]))
+
+    def __enter__(self) -> "_Leaves":
+        for mod, name, _, leaf in self.places:
+            mod._parameters[name] = leaf
+        return self
+
+    def __exit__(self, *exc) -> None:
+        for mod, name, p, _ in self.places:
+            mod._parameters[name] = p
 
 
 class GraphedTrainStep:
@@ -33,8 +67,6 @@ class GraphedTrainStep:
                  lr: float, warmup: int = 3, need_dx: bool = True):
         if x.device.type != "cuda":
             raise RuntimeError("CUDA graphs need CUDA tensors")
-        if dy.shape != (x.shape[0], model.base.out_features):
-            raise ValueError(f"dy has shape {tuple(dy.shape)}, the output {(x.shape[0], model.base.out_features)}")
         if dy.device != x.device:
             raise RuntimeError(f"input on {x.device} but dy on {dy.device}")
         self.model = model
@@ -56,28 +88,34 @@ class GraphedTrainStep:
             self.y = self._step()
 
     def _step(self) -> torch.Tensor:
-        """The calls of one step, without autograd: its nodes for the adapters'
-        parameters may belong to a graph that still lives on another stream,
-        and a capture must not meet that stream."""
+        """One step as a user writes it: the module's call (with its hooks and
+        an overridden forward), autograd, the gradients' hooks, the update."""
         m = self.model
-        pk = m._pack()
-        W, base8, bias = m._base_operands()
-        params = pk.params()
-        x, W, bias = pk.operands(self.x.detach(), W, bias, base8, params)
-        st = pk.state(self.plan, m.impl, base8, _save8(m.save_input))
-        want_A, want_B = any(p.requires_grad for p in params[0::2]), any(p.requires_grad for p in params[1::2])
-        with torch.no_grad(), ops._on(x.device):
-            rows8 = ops._new_rows8(x.shape[0], x.shape[1], x.device) if st.save8 and want_A else None
-            y, z, xs, _ = ops.forward_raw(x, W, bias, st, rows8=rows8)
-            dx, dA, dB = ops.backward_raw(self.dy.contiguous(), xs if rows8 is None else None, W, z, st, self.x.requires_grad,
-                                          want_A, want_B, rows8)
-            self.x.grad = dx
-            for i, ((o, r), act) in enumerate(zip(st.table.spans(), self.plan.active.tolist())):
-                A, B = params[2 * i], params[2 * i + 1]
-                A.grad = dA.narrow(0, o, r) if act and A.requires_grad else None
-                B.grad = dB.narrow(1, o, r) if act and B.requires_grad else None
-            m.sgd_step(self.lr)
-        return y
+        m._pack().sync()
+        x = self.x.detach().requires_grad_(self.x.requires_grad)
+        with _Leaves(m) as leaves:
+            y = m(x, self.ids, plan=self.plan)
+        if self.dy.shape != y.shape:
+            raise ValueError(f"dy has shape {tuple(self.dy.shape)}, the output {tuple(y.shape)}")
+        wanted = ([x] if x.requires_grad else []) + [leaf for _, leaf in leaves.pairs]
+        grads = [None] * len(wanted)
+        if y.requires_grad:
+            grads = list(torch.autograd.grad(y, wanted, self.dy, allow_unused=True))
+        self.x.grad = grads.pop(0) if x.requires_grad else None
+        adapters = {id(p) for ad in m.adapters.values() for p in ad.parameters()}
+        for ad in m.adapters.values():
+            ad.A.grad = ad.B.grad = None
+        for (p, _), g in zip(leaves.pairs, grads):
+            if g is None:
+                continue
+            if id(p) in adapters or p.grad is None:
+                p.grad = g
+            else:
+                p.grad.add_(g)  # a parameter of the user's own: gradients add up, as ever
+            for hook in tuple((p._post_accumulate_grad_hooks or {}).values()):
+                hook(p)
+        m.sgd_step(self.lr)
+        return y.detach()
 
     def __call__(self, x: Optional[torch.Tensor] = None, dy: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Copy new inputs (same shapes) into the static buffers and replay

@@ -83,6 +83,75 @@ def test_graphed_step_refuses_other_gradients():
         GraphedTrainStep(m, x, IDS, torch.zeros(rows, 192, dtype=BF), lr=0.0)
 
 
+def test_graphed_step_keeps_the_modules_hooks():
+    """Hooks and an overridden forward do in a graphed step what they do in an
+    eager one."""
+    class Doubled(MultiLoRALinear):
+        def forward(self, x, adapter_ids, **kw):
+            return 2 * super().forward(x + self.shift, adapter_ids, **kw)
+
+    def make():
+        torch.manual_seed(0)
+        m = Doubled(256, 192, RANKS)
+        with torch.no_grad():
+            for ad in m.adapters.values():
+                ad.B.normal_(0, 0.05)
+        m = m.cuda().bfloat16()
+        m.shift = torch.nn.Parameter(torch.full((256,), 0.25, device="cuda", dtype=BF))
+        m.seen = torch.zeros(3, device="cuda")
+
+        def forward_hook(mod, args, out):
+            mod.seen[0] += out.detach().float().abs().sum()
+            return out * 0.5
+
+        def backward_hook(mod, gi, go):
+            mod.seen[1] += go[0].float().abs().sum()
+
+        def after(p):
+            m.seen[2] += p.grad.float().abs().sum()
+        m.register_forward_hook(forward_hook)
+        m.register_full_backward_hook(backward_hook)
+        m.adapters["0"].A.register_hook(lambda g: g * 3)
+        m.adapters["1"].B.register_hook(lambda g: g.clamp(-0.5, 0.5))
+        m.adapters["2"].A.register_post_accumulate_grad_hook(after)
+        return m
+
+    x, dy = randn((len(IDS), 256), BF, 1), randn((len(IDS), 192), BF, 2, 0.1)
+    eager, m = make(), make()
+    alive = m(x.clone().requires_grad_(True), IDS)  # an eager graph of the same leaves
+    g = GraphedTrainStep(m, x, IDS, dy, lr=0.0)
+    for k in range(2):
+        eager.seen.zero_()
+        m.seen.zero_()
+        eager.shift.grad = None
+        want = step(eager, x, IDS, dy)
+        m.shift.grad.zero_()
+        y = g(x, dy)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(g.dx, want[1]) and torch.equal(m.seen, eager.seen)
+        assert torch.equal(m.shift.grad, eager.shift.grad) and bool((m.seen > 0).all())
+        for ad, da, db in zip(m.adapters.values(), want[2], want[3]):
+            assert torch.equal(ad.A.grad, da) and torch.equal(ad.B.grad, db)
+        x, dy = randn((len(IDS), 256), BF, 3), randn((len(IDS), 192), BF, 4, 0.1)
+    assert alive.requires_grad
+    # the module has its own parameters back
+    assert all(p.is_leaf and p.requires_grad for ad in m.adapters.values() for p in ad.parameters())
+
+
+def test_graphed_step_of_frozen_parts():
+    m = layer(256, 192, RANKS, BF).quantize_base()
+    m.save_input = "int8"
+    x, dy = randn((len(IDS), 256), BF, 1), randn((len(IDS), 192), BF, 2, 0.1)
+    want = step(m, x, IDS, dy)
+    for ad in m.adapters.values():
+        ad.A.requires_grad_(False)
+        ad.A.grad = None
+    g = GraphedTrainStep(m, x, IDS, dy, lr=0.0, need_dx=False)
+    assert torch.equal(g(), want[0]) and g.dx is None
+    for ad, db in zip(m.adapters.values(), want[3]):
+        assert ad.A.grad is None and torch.equal(ad.B.grad, db)
+
+
 # ------------------------------------------------------------------ plans
 
 @pytest.mark.parametrize("eight", [False, True])
