@@ -426,12 +426,13 @@ def _int8_product(x, weight: Int8Rows, bias, dtype):
     if isinstance(x, Int8Rows):
         src, ld, (xq, xs) = None, 0, _ptrs8(x)
     else:
+        # rows and their 8-bit form stay alive until the launch: y must not take their memory
         src, ld = _row_major(x.detach() if x.requires_grad else x)
-        kept = _Scratch8(rows, d_in, dev)  # noqa: F841  (alive until the launch)
-        src, (xq, xs) = src.data_ptr(), kept.ptrs
+        kept = _Scratch8(rows, d_in, dev)
+        xq, xs = kept.ptrs
     y = torch.empty((rows, d_out), dtype=dtype, device=dev)
     prob = _lib.Problem(rows, d_in, d_out, _DTYPES[dtype], _lib.IMPL_AUTO)
-    _lib.call("mlora_q8_linear", ctypes.byref(prob), src, ld, xq, xs, q.data_ptr(), weight.scale.data_ptr(),
+    _lib.call("mlora_q8_linear", ctypes.byref(prob), _ptr(src), ld, xq, xs, q.data_ptr(), weight.scale.data_ptr(),
               _ptr(bias), y.data_ptr(), _stream(dev))
     return y
 

@@ -265,3 +265,22 @@ def test_buffers_aligned_to_their_elements_only(dt, rows, save8):
     x, dy = randn((rows, 256), dt, 1), randn((rows, 192), dt, 2, 0.1)
     for where in (odd, lambda t: t.clone()):
         check(m, w, x, ids, dy, native_step(m, x, ids, dy, where, save8), save8=save8)
+
+
+# ------------------------------------------------------------------ product
+
+@pytest.mark.parametrize("rows", [4, 300])
+def test_copied_input_lives_until_the_launch(rows):
+    # with filled new memory a copy of x that is released early would be overwritten by y's
+    w8 = ops.quantize_rows(randn((256, 256), BF, 2))  # y is as large as the copy
+    x = randn((256, rows), BF, 1).t()
+    want = ops.int8_linear(x.contiguous(), w8)
+    torch.cuda.synchronize()
+    was = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)
+    try:
+        torch.cuda.empty_cache()
+        got = [ops.int8_linear(x, w8) for _ in range(3)]
+    finally:
+        torch.use_deterministic_algorithms(was)
+    assert all(torch.equal(y, want) for y in got)
