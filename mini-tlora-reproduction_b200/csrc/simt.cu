@@ -11,6 +11,8 @@
 //            dX = dY W + sum_c dZt[c] A_chunk              (bwd)
 //   reduce   dA_chunk = sum_tiles dZt[c]^T X_tile, dB_chunk = sum_tiles dY_tile^T Zt[c]
 //   sgd      P <- P - lr dP on the listed adapter tensors
+#include <algorithm>
+
 #include "common.cuh"
 #include "q8.cuh"
 #include "simt.cuh"
@@ -332,14 +334,20 @@ int simt_backward(const SimtCall& a, cudaStream_t st) {
 
 int simt_expand_add32(bool bwd, const PlanDev& plan, const float* pack, const float* zt, float* out,
                       const int32_t* out_rows, int64_t M, int d_in, int d_out, int R, cudaStream_t st) {
-  const dim3 grid(unsigned(((bwd ? d_in : d_out) + BN - 1) / BN), unsigned((M + BM - 1) / BM));
-  if (bwd)
-    k_main<float, true><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in, d_out,
-                                             R, 0, 0, 1);
-  else
-    k_main<float, false><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in,
-                                              d_out, R, 0, 0, 1);
-  count_launch();
+  // the row blocks are the grid's second dimension, which holds 65,535: whole
+  // tiles of them a launch
+  const int tiles = mlora_num_tiles(M), most = 65535 * BM / kTileRows;
+  for (int t0 = 0; t0 < tiles; t0 += most) {
+    const int64_t rows = std::min<int64_t>(M - int64_t(t0) * kTileRows, int64_t(most) * kTileRows);
+    const dim3 grid(unsigned(((bwd ? d_in : d_out) + BN - 1) / BN), unsigned((rows + BM - 1) / BM));
+    if (bwd)
+      k_main<float, true><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in,
+                                               d_out, R, t0, 0, 1);
+    else
+      k_main<float, false><<<grid, NT, 0, st>>>(plan, nullptr, nullptr, nullptr, pack, zt, out, out_rows, M, d_in,
+                                                d_out, R, t0, 0, 1);
+    count_launch();
+  }
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
 

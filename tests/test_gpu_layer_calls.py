@@ -284,3 +284,16 @@ def test_copied_input_lives_until_the_launch(rows):
     finally:
         torch.use_deterministic_algorithms(was)
     assert all(torch.equal(y, want) for y in got)
+
+
+def test_more_rows_than_one_launch_of_the_float32_expand():
+    rows = 64 * 65535 + 300  # blocks of 64 rows; a grid holds 65,535 in its second dimension
+    m = layer(16, 16, {0: 4, 1: 8}, F32).quantize_base()
+    ids = torch.cat([torch.zeros(rows - 200, dtype=torch.int64), torch.ones(200, dtype=torch.int64)])
+    x, dy = randn((rows, 16), F32, 1), randn((rows, 16), F32, 2)
+    y, dx, dA, dB = step(m, x, ids, dy)
+    for lo in (0, rows // 2, 64 * 65535 - 150, rows - 300):
+        part = slice(lo, lo + 300)
+        yp, dxp, _, _ = step(m, x[part], ids[part], dy[part])
+        assert torch.equal(y[part], yp) and torch.equal(dx[part], dxp)
+    assert _lib.device_error() == 0
