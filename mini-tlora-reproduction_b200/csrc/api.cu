@@ -645,14 +645,14 @@ int check_rows_cols(int64_t rows, int64_t cols, int32_t dtype) {
   return MLORA_OK;
 }
 
-// shape of an 8-bit product
-int check_q8_problem(const mlora_problem* prob) {
+// shape of an 8-bit product whose sums run over d_in (the forward) or d_out (dX)
+int check_q8_problem(const mlora_problem* prob, bool over_d_out) {
   if (!prob) return MLORA_ERR_INVALID_ARG;
   int st = check_rows_cols(prob->rows, prob->d_in, prob->dtype);
   if (st == MLORA_OK) st = check_rows_cols(prob->rows, prob->d_out, prob->dtype);
   if (st != MLORA_OK) return st;
   if (prob->max_ctas < 0) return MLORA_ERR_INVALID_ARG;
-  return prob->d_in > kQ8MaxK || prob->d_out > kQ8MaxK ? MLORA_ERR_UNSUPPORTED : MLORA_OK;
+  return (over_d_out ? prob->d_out : prob->d_in) > kQ8MaxK ? MLORA_ERR_UNSUPPORTED : MLORA_OK;
 }
 
 }  // namespace
@@ -691,7 +691,7 @@ extern "C" int mlora_q8_dequantize(const int8_t* q, const float* scale, int64_t 
 
 extern "C" int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t ld_x, int8_t* Xq, float* x_scale,
                                const int8_t* Wq, const float* w_scale, const void* bias, void* Y, void* stream) {
-  int st = check_q8_problem(prob);
+  int st = check_q8_problem(prob, false);
   if (st != MLORA_OK) return st;
   if (X && ld_x < prob->d_in) return MLORA_ERR_INVALID_ARG;
   if (prob->rows == 0) return MLORA_OK;
@@ -710,7 +710,7 @@ extern "C" int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t
 
 extern "C" int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale,
                                   const int8_t* Wq, const float* w_scale, void* dX, void* stream) {
-  int st = check_q8_problem(prob);
+  int st = check_q8_problem(prob, true);
   if (st != MLORA_OK) return st;
   if (prob->rows == 0) return MLORA_OK;
   if (!dY || !Gq || !g_scale || !Wq || !w_scale || !dX) return MLORA_ERR_INVALID_ARG;
@@ -734,7 +734,7 @@ extern "C" int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* 
   if (!prob || !route || !q8) return MLORA_ERR_INVALID_ARG;
   if (prob->rows != 0 && ((q8->Wq && (W || !q8->w_scale || !q8->Xq)) || (q8->Xq && !q8->x_scale)))
     return MLORA_ERR_INVALID_ARG;
-  if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
+  if (q8->Wq && check_q8_problem(prob, false) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
   int st = check_q8({q8->Wq, q8->Xq}, {q8->w_scale, q8->x_scale});
   if (st != MLORA_OK) return st;
   return forward_staged(prob, route, X, W, bias, A_pack, B_pack, Y, zsave, workspace, workspace_bytes,
@@ -749,7 +749,7 @@ extern "C" int mlora_backward_q8(const mlora_problem* prob, const mlora_routing*
   if (prob->rows != 0 &&
       ((q8->Wq && (W || !q8->w_scale || (dX && (!q8->Gq || !q8->g_scale)))) || (q8->Xq && !q8->x_scale)))
     return MLORA_ERR_INVALID_ARG;
-  if (q8->Wq && check_q8_problem(prob) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
+  if (q8->Wq && dX && check_q8_problem(prob, true) == MLORA_ERR_UNSUPPORTED) return MLORA_ERR_UNSUPPORTED;
   int st = check_q8({q8->Wq, q8->Xq, q8->Gq}, {q8->w_scale, q8->x_scale, q8->g_scale});
   if (st != MLORA_OK) return st;
   return backward_all(prob, route, dY, X, W, A_pack, B_pack, zsave, dX, dA_pack, dB_pack, workspace,

@@ -462,10 +462,10 @@ int dequantize_t(const int8_t* q, const float* scale, int64_t rows, int64_t cols
 constexpr int QK = 16;  // words of K per step
 
 template <class T, bool BWD>
-__global__ void __launch_bounds__(NT) k_q8_main(Q8Main a) {
+__global__ void __launch_bounds__(NT) k_q8_main(Q8Main a, int nb0) {
   __shared__ int Aw[QK][LD], Bw[QK][LD];
   __shared__ float As[BK][LD], Bs[BK][LD];
-  const int n0 = blockIdx.y * BN;
+  const int n0 = (nb0 + int(blockIdx.y)) * BN;
   const int64_t m0 = int64_t(blockIdx.x) * BM;
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
   const int N = BWD ? a.d_in : a.d_out, K = BWD ? a.d_out : a.d_in;
@@ -713,10 +713,14 @@ __global__ void __launch_bounds__(256) k_sum32(PlanDev plan, const int8_t* __res
 template <class T>
 int launch_q8_main(const Q8Main& a, cudaStream_t st) {
   const int N = a.bwd ? a.d_in : a.d_out;
-  const dim3 grid(unsigned((a.M + BM - 1) / BM), unsigned((N + BN - 1) / BN));
-  if (a.bwd) k_q8_main<T, true><<<grid, NT, 0, st>>>(a);
-  else k_q8_main<T, false><<<grid, NT, 0, st>>>(a);
-  count_launch();
+  // the column blocks are the grid's second dimension, which holds 65,535
+  const int blocks = (N + BN - 1) / BN;
+  for (int nb0 = 0; nb0 < blocks; nb0 += 65535) {
+    const dim3 grid(unsigned((a.M + BM - 1) / BM), unsigned(std::min(blocks - nb0, 65535)));
+    if (a.bwd) k_q8_main<T, true><<<grid, NT, 0, st>>>(a, nb0);
+    else k_q8_main<T, false><<<grid, NT, 0, st>>>(a, nb0);
+    count_launch();
+  }
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
 }
 

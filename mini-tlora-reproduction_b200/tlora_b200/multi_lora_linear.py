@@ -272,6 +272,8 @@ class _PackedAdapters:
         if plan is None:
             plan = ops.route(ids, self.table, x.device)
         train = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params))
+        if base8 is not None and train and x.requires_grad:
+            ops._check_dx8(base8)
         # nothing is kept for a backward that cannot follow
         st = self.state(plan, impl, base8, save8 and train)
         with ops._on(x.device):

@@ -437,6 +437,13 @@ def _int8_product(x, weight: Int8Rows, bias, dtype):
     return y
 
 
+def _check_dx8(weight: Int8Rows) -> None:
+    """Before a forward whose input wants a gradient."""
+    if weight.q.shape[0] > _lib.Q8_MAX_K:
+        raise NotImplementedError(f"the input's gradient is a contraction over {weight.q.shape[0]} outputs: an 8-bit "
+                                  f"product sums up to {_lib.Q8_MAX_K}")
+
+
 def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Matrix product in 8-bit integers with a scale per token and per output
@@ -447,7 +454,8 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
     to it) or an :class:`Int8Rows` (rows quantized once for several products;
     then ``dtype``, or the bias's type, is the type of ``y``).  ``weight`` holds the
     8-bit rows of W [out_features, in_features] (``quantize_rows(W)``) and is
-    frozen, like the backbone of ``MultiLoRALinear``."""
+    frozen, like the backbone of ``MultiLoRALinear``.  Sums run over at most
+    131,072 terms: in_features, and out_features where x wants a gradient."""
     if not isinstance(weight, Int8Rows):
         raise TypeError("int8_linear expects weight as Int8Rows (quantize_rows(W))")
     _no_tangents(None if isinstance(x, Int8Rows) else x, bias)
@@ -479,6 +487,7 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
         if not bias.is_contiguous():
             bias = bias.contiguous()
     if grad and not eight and x.requires_grad:
+        _check_dx8(weight)
         return Int8LinearFunction.apply(x, weight.q, weight.scale, bias, weight.cols)
     return _int8_product(x, weight, bias, dtype)
 

@@ -297,3 +297,37 @@ def test_more_rows_than_one_launch_of_the_float32_expand():
         yp, dxp, _, _ = step(m, x[part], ids[part], dy[part])
         assert torch.equal(y[part], yp) and torch.equal(dx[part], dxp)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_more_outputs_than_a_contraction_may_have(dt, rows):
+    # d_out is no contraction of the forward, only of dx
+    d_in, d_out = 80, _lib.Q8_MAX_K + 200
+    x, w = randn((rows, d_in), dt, 1), randn((d_out, d_in), dt, 2, 0.1)
+    b = randn((d_out,), dt, 3)
+    w8 = ops.quantize_rows(w)
+    ref.assert_within(ops.int8_linear(x, w8, b), *ref.linear(x, w, b), what="y")
+    prob = _lib.Problem(rows, d_in, d_out, ops.mlora_dtype(dt), _lib.IMPL_SIMT)
+    y, r8 = torch.empty(rows, d_out, device="cuda", dtype=dt), ops.quantize_rows(x)
+    _lib.call("mlora_q8_linear", ctypes.byref(prob), None, 0, r8.q.data_ptr(), r8.scale.data_ptr(), w8.q.data_ptr(),
+              w8.scale.data_ptr(), b.data_ptr(), y.data_ptr(), ops._stream(x.device))
+    ref.assert_within(y, *ref.linear(x, w, b), what="y")
+    with pytest.raises(NotImplementedError, match="contraction"):
+        ops.int8_linear(x.requires_grad_(True), w8, b)
+    m = layer(d_in, d_out, {0: 8}, dt)
+    x, ids = x.detach(), torch.zeros(rows, dtype=torch.int64)
+    w = m.base.weight.detach().clone()
+    m.quantize_base()
+    # without dx the layer trains its adapters
+    dy = randn((rows, d_out), dt, 4, 0.1)
+    y = m(x, ids)
+    y.backward(dy)
+    ad = m.adapters["0"]
+    slot = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    (yw, by), _, dA, dB = ref.lora(x, slot, w, m.base.bias, [(ad.A.detach(), ad.B.detach(), ad.scaling)], dy, True, False)
+    ref.assert_within(y, yw, by, what="y")
+    ref.assert_within(ad.A.grad, *dA[0], what="dA")
+    ref.assert_within(ad.B.grad, *dB[0], what="dB")
+    with pytest.raises(NotImplementedError, match="contraction"):
+        m(x.requires_grad_(True), ids)

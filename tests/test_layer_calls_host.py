@@ -1,6 +1,8 @@
 """Calls of the layer's raw entry points that must be refused on the host,
 before anything reaches a GPU (so they run on CPU tensors)."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -205,3 +207,30 @@ def test_tensors_with_tangents_are_refused():
             p = dict(m.named_parameters())[name]
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.func.functional_call(m, {name: fw.make_dual(p.detach(), torch.ones_like(p))}, (x, ids))
+
+
+# ------------------------------------------------------------------ limits of a native call
+
+def test_contraction_limits():
+    """Each call is limited by the length of its own sums: d_in of the forward,
+    d_out of dX.  No rows: nothing is launched."""
+    lib, none, over = _lib.lib(), ctypes.c_void_p(None), _lib.Q8_MAX_K + 8
+
+    def linear(d_in, d_out):
+        p = _lib.Problem(0, d_in, d_out, _lib.BF16, _lib.IMPL_AUTO)
+        return (lib.mlora_q8_linear(ctypes.byref(p), none, 0, *[none] * 7),
+                lib.mlora_q8_linear_dx(ctypes.byref(p), *[none] * 7))
+    assert linear(64, over) == (_lib.OK, _lib.ERR_UNSUPPORTED)
+    assert linear(over, 64) == (_lib.ERR_UNSUPPORTED, _lib.OK)
+    assert linear(64, (1 << 30) + 1)[0] == _lib.ERR_UNSUPPORTED
+
+    def layer(d_in, d_out, dx):
+        p = _lib.Problem(0, d_in, d_out, _lib.BF16, _lib.IMPL_AUTO)
+        r, a = _lib.Routing(0, None, None, 0, None, None, None, 0, None), ctypes.c_void_p(4096)
+        q8 = _lib.Q8(4096, 4096, 4096, 4096, 4096, 4096)
+        return (lib.mlora_forward_q8(ctypes.byref(p), ctypes.byref(r), ctypes.byref(q8), a, *[none] * 7, 0, none),
+                lib.mlora_backward_q8(ctypes.byref(p), ctypes.byref(r), ctypes.byref(q8), a, none, none, none, none,
+                                      none, a if dx else none, none, none, none, 0, none))
+    assert layer(64, over, False) == (_lib.OK, _lib.OK)
+    assert layer(64, over, True) == (_lib.OK, _lib.ERR_UNSUPPORTED)
+    assert layer(over, 64, True) == (_lib.ERR_UNSUPPORTED, _lib.OK)
