@@ -427,7 +427,9 @@ int mlora_q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64
  * and the gradient of its input through the 8-bit rows of dY w_scale,
  *     dX[i, k] = g_scale[i] sum_j Gq[i, j] Wq[j, k].
  * prob gives rows, d_in, d_out, dtype (of X, bias, Y, dY, dX), max_ctas and
- * err_word.  X (rows ld_x elements apart) is quantized into Xq / x_scale
+ * err_word.  max_ctas caps the tensor-core kernel, which takes CTAs in pairs
+ * (with 1 the CUDA-core product serves); a forward of at most 16 rows streams
+ * the weight through short blocks and takes no cap.  X (rows ld_x elements apart) is quantized into Xq / x_scale
  * first; with X NULL they hold the 8-bit rows already.  dY is quantized into
  * the scratch Gq [rows, mlora_q8_ld(d_out)] / g_scale [rows].  The integer
  * sums are exact; one rounding to dtype at the end. */

@@ -191,13 +191,15 @@ int check_q8(std::initializer_list<const void*> mats, std::initializer_list<cons
 // cores, whatever their size, unless the call asks for the CUDA cores.
 int q8_main(const Q8Main& a, int impl, Q8After after, cudaStream_t st) {
   if (impl != MLORA_IMPL_SIMT && q8_few_ok(a)) return q8_main_few(a, after, st);
-  if (impl != MLORA_IMPL_SIMT && a.expand && a.dtype == MLORA_F32 && tc_available()) {
+  if (impl != MLORA_IMPL_SIMT && a.expand && a.dtype == MLORA_F32) {
     // float32: the expand is not a tensor-core operand; it is added after
     Q8Main product = a;
     product.expand = false;
-    const int s = q8_main_tc(product, after, st);
-    return s != MLORA_OK ? s : simt_expand_add32(a.bwd, a.plan, (const float*)a.pack, (const float*)a.zt,
-                                                 (float*)a.out, a.out_rows, a.M, a.d_in, a.d_out, a.R, st);
+    if (q8_tc_ok(product)) {
+      const int s = q8_main_tc(product, after, st);
+      return s != MLORA_OK ? s : simt_expand_add32(a.bwd, a.plan, (const float*)a.pack, (const float*)a.zt,
+                                                   (float*)a.out, a.out_rows, a.M, a.d_in, a.d_out, a.R, st);
+    }
   }
   const bool tc = impl != MLORA_IMPL_SIMT && q8_tc_ok(a);
   return tc ? q8_main_tc(a, after, st) : q8_main_simt(a, st);

@@ -543,11 +543,12 @@ bool make_map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t ld, int
 }  // namespace
 
 // Any sizes, alignments and types, except that the expand reads 16-bit
-// operands by TMA (a LoRA call of the tensor-core family).
+// operands by TMA (a LoRA call of the tensor-core family), and that a tile
+// takes two CTAs.
 bool q8_tc_ok(const Q8Main& a) {
   if (a.expand && (a.dtype == MLORA_F32 || (a.bwd && a.d_in % 8) || !aligned(a.pack, 16) || !aligned(a.zt, 16)))
     return false;
-  return tc_available();
+  return tc_available() && cta_budget(a.max_ctas) >= 2;
 }
 
 int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
@@ -585,11 +586,9 @@ int q8_main_tc(const Q8Main& a, Q8After after, cudaStream_t st) {
   prm.out = a.out;
   prm.out_rows = a.out_rows;
   prm.err = a.err;
-  const int sms = cta_budget(a.max_ctas);
-  if (sms < 2) return MLORA_ERR_UNSUPPORTED;
   const void* fn = a.bwd ? reinterpret_cast<const void*>(&k_q8<true>) : reinterpret_cast<const void*>(&k_q8<false>);
   MLORA_CUDA_TRY(set_smem_once(fn, kQ8Smem));
-  const unsigned grid = 2u * unsigned(std::min(prm.n_items, sms / 2));
+  const unsigned grid = 2u * unsigned(std::min(prm.n_items, cta_budget(a.max_ctas) / 2));
   const bool pdl = after != kAfterOther && pdl_enabled();
   prm.pdl_rows = pdl && after == kAfterRows ? 1 : 0;
   prm.pdl_z = pdl ? 1 : 0;

@@ -331,3 +331,22 @@ def test_more_outputs_than_a_contraction_may_have(dt, rows):
     ref.assert_within(ad.B.grad, *dB[0], what="dB")
     with pytest.raises(NotImplementedError, match="contraction"):
         m(x.requires_grad_(True), ids)
+
+
+@pytest.mark.parametrize("rows", [5, 40, 300])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_one_cta(dt, rows):
+    """max_ctas = 1 leaves no pair of SMs: the CUDA-core product."""
+    x, w, b = randn((rows, 200), dt, 1), randn((136, 200), dt, 2, 0.1), randn((136,), dt, 3)
+    dy = randn((rows, 136), dt, 4, 0.1)
+    w8 = ops.quantize_rows(w)
+    prob = _lib.Problem(rows, 200, 136, ops.mlora_dtype(dt), _lib.IMPL_AUTO, 1)
+    y, dx = torch.empty(rows, 136, device="cuda", dtype=dt), torch.empty_like(x)
+    r8, g8 = ops._Scratch8(rows, 200, x.device), ops._Scratch8(rows, 136, x.device)
+    s = ops._stream(x.device)
+    _lib.call("mlora_q8_linear", ctypes.byref(prob), x.data_ptr(), 200, *r8.ptrs, w8.q.data_ptr(), w8.scale.data_ptr(),
+              b.data_ptr(), y.data_ptr(), s)
+    _lib.call("mlora_q8_linear_dx", ctypes.byref(prob), dy.data_ptr(), *g8.ptrs, w8.q.data_ptr(), w8.scale.data_ptr(),
+              dx.data_ptr(), s)
+    ref.assert_within(y, *ref.linear(x, w, b), what="y")
+    ref.assert_within(dx, *ref.linear_dx(dy, w), what="dx")
