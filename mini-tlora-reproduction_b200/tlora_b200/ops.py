@@ -17,6 +17,7 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import BF16, F16, F32, RANK_CHUNK, TILE_ROWS
@@ -402,6 +403,7 @@ class Int8LinearFunction(torch.autograd.Function):
         return _int8_product(x, _wrap8(wq, w_scale, d_in), bias, x.dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         wq, w_scale = ctx.saved_tensors
         rows, d_out, d_in = dy.shape[0], wq.shape[0], ctx.d_in

@@ -350,3 +350,14 @@ def test_one_cta(dt, rows):
               dx.data_ptr(), s)
     ref.assert_within(y, *ref.linear(x, w, b), what="y")
     ref.assert_within(dx, *ref.linear_dx(dy, w), what="dx")
+
+
+def test_second_derivatives_are_refused():
+    w8 = ops.quantize_rows(randn((48, 64), BF, 2))
+    x = randn((5, 64), BF, 1).requires_grad_(True)
+    dy = randn((5, 48), BF, 3).requires_grad_(True)
+    dx, = torch.autograd.grad(ops.int8_linear(x, w8), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="not have been used"):  # not a zero
+        torch.autograd.grad(dx.float().sum(), dy, retain_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.float().sum().backward()
