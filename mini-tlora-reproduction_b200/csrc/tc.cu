@@ -966,14 +966,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
             if (MODE == SHRINK_BWD && p.dz8) {
               // the product with the saved integers has no rounding of its
               // own: 16 bits of x_scale dZ in two bf16 numbers (the exponent
-              // of fp16 would not hold it), so dA is rounded once, at the end
+              // of fp16 would not hold it), so dA is rounded once, at the end.
+              // An infinite high part has no rest (inf - inf would make it NaN)
               const float sx = in ? p.x_scale[int64_t(it.t) * kTileRows + rt] : 0.f;
               float lo[32];
 #pragma unroll
               for (int q = 0; q < 32; ++q) {
                 const float w = in ? ch.scale * __uint_as_float(v[q]) * sx : 0.f;
                 f[q] = __bfloat162float(__float2bfloat16_rn(w));
-                lo[q] = w - f[q];
+                lo[q] = isinf(f[q]) ? 0.f : w - f[q];
               }
               __nv_bfloat16* d8 = p.dz8 + (dst + col - p.out);
               store32(d8, f, false);

@@ -361,3 +361,45 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(dx.float().sum(), dy, retain_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.float().sum().backward()
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("base8", [False, True])
+@pytest.mark.parametrize("dt", [BF, FP, F32])
+def test_infinite_upstream_gradients(dt, base8):
+    m = layer(256, 192, RANKS, dt)
+    if base8:
+        m.quantize_base()
+    m.save_input = "int8"
+    x, dy = randn((len(IDS), 256), dt, 1), randn((len(IDS), 192), dt, 2, 0.1)
+    _, dx0, dA0, dB0 = step(m, x, IDS, dy)
+    dy[100, 7] = float("inf")  # a row of adapter 1, in a tile with all three
+    _, dx, dA, dB = step(m, x, IDS, dy)
+    rest = [i for i in range(len(IDS)) if i != 100]
+    assert torch.equal(dx[rest], dx0[rest]) and not torch.isfinite(dx[100]).any()
+    for i in (0, 2):
+        assert torch.equal(dA[i], dA0[i]) and torch.equal(dB[i], dB0[i])
+    # dA = dZ^T (s q(x)): dZ of the row is infinite with the signs of B's row 7
+    q, _ = ref.quantize(x[100:101])
+    want = torch.sign(m.adapters["1"].B.detach()[7].double())[:, None] * q * float("inf")
+    assert bool((q == 0).any()) and torch.equal(torch.isnan(dA[1]), torch.isnan(want))
+    keep = ~torch.isnan(want)
+    assert torch.equal(dA[1].double()[keep], want[keep])
+    # dB = dY^T Z: only column 7 of dY is infinite
+    others = [k for k in range(192) if k != 7]
+    assert torch.equal(dB[1][others], dB0[1][others]) and not torch.isfinite(dB[1][7]).any()
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("rows", [4, 16])
+def test_infinite_inputs_of_a_few_rows(dt, rows):
+    m = layer(256, 192, {0: 8, 1: 64}, dt).quantize_base()
+    ids = torch.arange(rows) % 2
+    x = randn((rows, 256), dt, 1)
+    with torch.no_grad():
+        clean = m(x, ids)
+        x[1, 9], x[2, 0] = float("-inf"), float("nan")
+        y = m(x, ids)
+    rest = [i for i in range(rows) if i not in (1, 2)]
+    assert torch.equal(y[rest], clean[rest]) and torch.isnan(y[[1, 2]]).all()
