@@ -660,6 +660,11 @@ def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8
     return y, z, xs, args
 
 
+def _no_8_bits(st: LayerState) -> None:
+    if st.base8 is not None or st.save8:
+        raise NotImplementedError("staged calls have neither a backbone nor saved inputs in 8 bits")
+
+
 class StagedForward:
     """Forward of one routing plan split into stages and tile ranges (the
     nano-batch pipeline): ``shrink(t0, t1)`` writes the low-rank
@@ -668,6 +673,7 @@ class StagedForward:
     ``expand``)."""
 
     def __init__(self, x, W, bias, st: LayerState, y=None):
+        _no_8_bits(st)
         self.x, self.W, self.bias, self.st = x, W, bias, st
         rows, d_in = x.shape
         d_out = st.B_pack.shape[0]
@@ -781,6 +787,7 @@ class StagedBackward:
     summed in."""
 
     def __init__(self, dy, xs, W, z, st: LayerState):
+        _no_8_bits(st)
         self.dy, self.xs, self.W, self.z, self.st = dy, xs, W, z, st
         rows = dy.shape[0]
         d_in = st.A_pack.shape[1]

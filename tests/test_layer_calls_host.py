@@ -234,3 +234,18 @@ def test_contraction_limits():
     assert layer(64, over, False) == (_lib.OK, _lib.OK)
     assert layer(64, over, True) == (_lib.OK, _lib.ERR_UNSUPPORTED)
     assert layer(over, 64, True) == (_lib.ERR_UNSUPPORTED, _lib.OK)
+
+
+# ------------------------------------------------------------------ settings that a path does not have
+
+def test_staged_calls_refuse_8_bits():
+    base8 = ops.Int8Rows(torch.zeros(48, 64, dtype=torch.int8), torch.ones(48), 64)
+    x, dy = torch.zeros(40, 64, dtype=BF), torch.zeros(40, 48, dtype=BF)
+    for changed in ({"base8": base8}, {"save8": True}):
+        st = state()
+        for k, v in changed.items():
+            setattr(st, k, v)
+        with pytest.raises(NotImplementedError, match="8 bits"):
+            ops.StagedForward(x, None, None, st)
+        with pytest.raises(NotImplementedError, match="8 bits"):
+            ops.StagedBackward(dy, x, None, torch.zeros(1), st)
