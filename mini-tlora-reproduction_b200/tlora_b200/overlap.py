@@ -58,6 +58,7 @@ import torch.distributed as dist
 
 from . import _lib, ops, peer
 from ._lib import TILE_ROWS
+from .multi_lora_linear import _save8
 from .nano import ramp_ranges, split_ranges
 
 COMMS = ("nccl", "peer", "mc")
@@ -245,6 +246,8 @@ class ShardedLayer:
             raise ValueError(f"dz must be 'split' or 'replicated', not {dz!r}")
         if not hasattr(model.base, "weight"):
             raise NotImplementedError("a backbone in 8 bits is not sharded: call model.dequantize_base() first")
+        if _save8(getattr(model, "save_input", "full")):
+            raise NotImplementedError("a sharded layer keeps its input as it is: set model.save_input = 'full'")
         self.dz = dz
         # nano-batch ranges over the plan tiles: "even" (the reference's
         # split_ranges) or "ramp" (the first nano-batch half as long, so that

@@ -249,3 +249,15 @@ def test_staged_calls_refuse_8_bits():
             ops.StagedForward(x, None, None, st)
         with pytest.raises(NotImplementedError, match="8 bits"):
             ops.StagedBackward(dy, x, None, torch.zeros(1), st)
+
+
+def test_sharded_layers_refuse_inputs_saved_in_8_bits():
+    from tlora_b200.overlap import ShardedLayer
+
+    m = MultiLoRALinear(256, 64, {0: 4})
+    m.save_input = "int8"
+    with pytest.raises(NotImplementedError, match="save_input"):
+        ShardedLayer(m, 0, 1)
+    m.save_input = "eight"
+    with pytest.raises(ValueError, match="save_input"):
+        ShardedLayer(m, 0, 1)
