@@ -69,6 +69,8 @@ class Int8Base(nn.Module):
 
     def __init__(self, rows8: ops.Int8Rows, bias: Optional[torch.Tensor]):
         super().__init__()
+        if bias is not None and bias.shape != (rows8.rows,):
+            raise ValueError(f"bias of shape {tuple(bias.shape)} for {rows8.rows} output channels")
         self.in_features, self.out_features = rows8.cols, rows8.rows
         self.register_buffer("weight_q8", rows8.q)
         self.register_buffer("weight_scale", rows8.scale)
@@ -252,13 +254,7 @@ class _PackedAdapters:
             raise RuntimeError(f"dtype mismatch: input {x.dtype}, weights {A.dtype}")
         if x.shape[1] != A.shape[1]:
             raise ValueError(f"x has {x.shape[1]} features, the layer {A.shape[1]}")
-        if base8 is not None:
-            if base8.device != x.device:
-                raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
-            if base8.shape != (B.shape[0], A.shape[1]):
-                raise ValueError(f"8-bit backbone {base8.shape} in a layer of {(B.shape[0], A.shape[1])}")
-            if bias is not None and (bias.dtype != x.dtype or bias.device != x.device):
-                raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
+        ops.check_base(x, A, B, W, bias, base8)
         if W is not None and W.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the backbone is frozen: no dW (tlora/multi_lora_linear.py:78-80)")
         return (x.contiguous(), W.contiguous() if W is not None else None,

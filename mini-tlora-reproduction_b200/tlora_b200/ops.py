@@ -630,6 +630,24 @@ def _workspace(st: LayerState, args, wb, device):
     return torch.empty(max(wb, 1), dtype=torch.uint8, device=device), 0
 
 
+def check_base(x, A, B, W, bias, base8: Optional["Int8Rows"]) -> None:
+    """The backbone's operands against the layer's packs: the kernels take all
+    sizes from the packs."""
+    shape = (B.shape[0], A.shape[1])
+    if W is not None and W.shape != shape:
+        raise ValueError(f"backbone {tuple(W.shape)} in a layer of {shape}")
+    if bias is not None:
+        if bias.shape != shape[:1]:
+            raise ValueError(f"bias of shape {tuple(bias.shape)} in a layer of {shape[0]} outputs")
+        if bias.dtype != x.dtype or bias.device != x.device:
+            raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
+    if base8 is not None:
+        if base8.device != x.device:
+            raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
+        if base8.shape != shape:
+            raise ValueError(f"8-bit backbone {base8.shape} in a layer of {shape}")
+
+
 def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8Rows"] = None):
     """Run mlora_forward; returns (Y in the caller's row order, zsave, x in
     sorted order, call args).  With interleaved ids the rows of X are

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from tlora_b200 import MultiLoRALinear, _lib, ops
+from tlora_b200.multi_lora_linear import Int8Base
 
 BF = torch.bfloat16
 
@@ -261,3 +262,25 @@ def test_sharded_layers_refuse_inputs_saved_in_8_bits():
     m.save_input = "eight"
     with pytest.raises(ValueError, match="save_input"):
         ShardedLayer(m, 0, 1)
+
+
+# ------------------------------------------------------------------ modules that were changed by hand
+
+def test_bias_of_another_length():
+    base8 = ops.Int8Rows(torch.zeros(48, 64, dtype=torch.int8), torch.ones(48), 64)
+    for bad in (torch.zeros(47), torch.zeros(49), torch.zeros(1, 48)):
+        with pytest.raises(ValueError, match="bias"):
+            Int8Base(base8, bad)
+    m = MultiLoRALinear(64, 48, {0: 4})
+    pk = m._pack()
+    pk.sync()
+    x, A, B = torch.zeros(3, 64), pk.A_pack, pk.B_pack
+    ops.check_base(x, A, B, m.base.weight, m.base.bias, None)
+    ops.check_base(x, A, B, None, None, base8)
+    for W, bias, b8 in ((m.base.weight[:, 1:], None, None), (m.base.weight[1:], None, None),
+                        (m.base.weight, torch.zeros(47), None), (None, torch.zeros(47), base8),
+                        (None, None, ops.Int8Rows(torch.zeros(47, 64, dtype=torch.int8), torch.ones(47), 64))):
+        with pytest.raises(ValueError):
+            ops.check_base(x, A, B, W, bias, b8)
+    with pytest.raises(RuntimeError, match="bias"):
+        ops.check_base(x, A, B, None, torch.zeros(48, dtype=BF), base8)
