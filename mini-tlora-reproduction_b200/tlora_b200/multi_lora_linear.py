@@ -198,7 +198,8 @@ class _PackedAdapters:
 
     def params(self) -> list:
         """A_0, B_0, A_1, ... as the adapters hold them now."""
-        return [p[k] for p in [ad._parameters for ad in self.adapters] for k in ("A", "B")]
+        # (the parameters' dict is read directly: attribute lookups cost several times as much)
+        return [ad._parameters[k] if k in ad._parameters else getattr(ad, k) for ad in self.adapters for k in "AB"]
 
     def _in_sync(self, params) -> bool:
         # a parameter that no longer views the packs has another address: the

@@ -284,3 +284,16 @@ def test_bias_of_another_length():
             ops.check_base(x, A, B, W, bias, b8)
     with pytest.raises(RuntimeError, match="bias"):
         ops.check_base(x, A, B, None, torch.zeros(48, dtype=BF), base8)
+
+
+def test_adapter_weights_that_are_plain_tensors():
+    # as functional training loops set them: no longer parameters, still the weights
+    m = MultiLoRALinear(64, 48, {0: 4, 1: 8})
+    ad, pk = m.adapters["0"], m._pack()
+    pk.sync()
+    new = torch.randn(4, 64, requires_grad=True)
+    del ad.A
+    ad.A = new
+    assert pk.params()[0] is new and pk.params()[1] is ad.B
+    pk.sync()
+    assert torch.equal(pk.A_pack[:4], new.detach())
