@@ -258,13 +258,13 @@ int q8_impl(const mlora_problem* prob, int impl) {
 // intermediate that the shrink before it left in zsave.
 int q8_forward_main(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8, const PlanDev& dev,
                     int impl, Q8After after, const void* bias, const void* B_pack, void* Y, const void* zsave,
-                    int32_t stages, cudaStream_t s) {
+                    cudaStream_t s) {
   Q8Main m;
   m.M = prob->rows; m.d_in = prob->d_in; m.d_out = prob->d_out; m.R = route->r_pack; m.dtype = prob->dtype;
   m.Aq = q8->Xq; m.a_scale = q8->x_scale;
   m.Wq = q8->Wq; m.w_scale = q8->w_scale;
   m.bias = bias; m.out = Y; m.out_rows = route->out_rows;
-  m.expand = dev.n_chunks > 0 && !(stages & MLORA_STAGE_NO_EXPAND);
+  m.expand = dev.n_chunks > 0;
   m.plan = dev; m.zt = zsave; m.pack = B_pack;
   m.max_ctas = prob->max_ctas;
   m.err = prob->err_word;
@@ -299,10 +299,8 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   if (impl < 0) return MLORA_ERR_UNSUPPORTED;
   if (ar && (impl != MLORA_IMPL_TC || route->out_rows)) return MLORA_ERR_UNSUPPORTED;
   const bool q8_base = q8 && q8->Wq;
-  const int32_t all_stages = stages;
   // a few rows in 16 bits: rows and shrink in one launch
-  const bool few = q8_base && impl == MLORA_IMPL_TC && prob->rows <= kQ8Few && !p.chunks.empty() &&
-                   (stages & MLORA_STAGE_SHRINK);
+  const bool few = q8_base && impl == MLORA_IMPL_TC && prob->rows <= kQ8Few && !p.chunks.empty();
   cudaStream_t s = (cudaStream_t)stream;
   PlanDev dev;
   st = stage_plan(prob, p, workspace, s, &dev, !few);
@@ -312,8 +310,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   if (few) {
     st = q8_few_prep(X, prob->rows, prob->d_in, prob->dtype, q8->Xq, q8->x_scale, dev, A_pack, zsave, s);
     if (st != MLORA_OK) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
-                           s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, s);
   }
   if (q8 && q8->Xq) {  // operand of the 8-bit product, the saved form of X, or both
     st = q8_quantize(X, prob->rows, prob->d_in, prob->d_in, prob->dtype, nullptr, (int8_t*)q8->Xq,
@@ -339,15 +336,13 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     st = tc_forward(a, s);
     if (st != MLORA_OK || !q8_base) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
-                           s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, s);
   }
   if (q8_base && prob->dtype == MLORA_F32) {
     st = q8_low32(false, dev, (const float*)X, (const float*)A_pack, (float*)zsave, prob->rows, prob->d_in,
                   prob->d_out, route->r_pack, s);
     if (st != MLORA_OK) return st;
-    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages,
-                           s);
+    return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, s);
   }
   SimtCall a;
   a.plan = dev;
@@ -362,7 +357,7 @@ int forward_staged(const mlora_problem* prob, const mlora_routing* route, const 
   a.c_end = p.tile_chunk_begin[tile_end];
   st = simt_forward(a, s);
   if (st != MLORA_OK || !q8_base) return st;
-  return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, all_stages, s);
+  return q8_forward_main(prob, route, q8, dev, q8_impl(prob, impl), after, bias, B_pack, Y, zsave, s);
 }
 
 }  // namespace
