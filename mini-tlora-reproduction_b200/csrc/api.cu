@@ -401,12 +401,13 @@ extern "C" int mlora_forward(const mlora_problem* prob, const mlora_routing* rou
 namespace {
 
 // The kernels of a backward call on a staged plan; with `q8`, dA reads the
-// saved 8-bit rows of X.
+// saved 8-bit rows of X.  `isolate`: the reductions keep what is not finite in a
+// row out of other segments' gradients (8-bit calls).
 int backward_kernels(const mlora_problem* prob, const mlora_routing* route, const Plan& p, const PlanDev& dev,
                      int impl, const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
                      const void* zsave, void* dzsave, void* dX, void* dA_pack, void* dB_pack, int32_t stages,
-                     int32_t tile_begin, int32_t tile_end, int32_t db_begin, int32_t db_end, const mlora_q8* q8,
-                     cudaStream_t s) {
+                     int32_t tile_begin, int32_t tile_end, int32_t db_begin, int32_t db_end, bool isolate,
+                     const mlora_q8* q8, cudaStream_t s) {
   if (impl == MLORA_IMPL_TC) {
     TcCall a;
     a.plan = dev;
@@ -421,6 +422,7 @@ int backward_kernels(const mlora_problem* prob, const mlora_routing* route, cons
     a.wide = prob->impl == MLORA_IMPL_TC_WIDE;
     a.bwd_stages = stages; a.t0 = tile_begin; a.t1 = tile_end; a.db0 = db_begin; a.db1 = db_end;
     a.lr = prob->lr;
+    a.isolate = isolate;
     if (q8) { a.x_scale = q8->x_scale; a.dz8 = q8->scratch; }
     return tc_backward(a, s);
   }
@@ -435,6 +437,7 @@ int backward_kernels(const mlora_problem* prob, const mlora_routing* route, cons
   a.out_rows = route->out_rows;
   a.bwd_stages = stages; a.db0 = db_begin; a.db1 = db_end;
   a.lr = prob->lr;
+  a.isolate = isolate;
   if (q8) { a.Xq = q8->Xq; a.x_scale = q8->x_scale; }
   a.c_begin = p.tile_chunk_begin[tile_begin];
   a.c_end = p.tile_chunk_begin[tile_end];
@@ -467,7 +470,7 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
   const int32_t reduce = MLORA_BWD_DA | MLORA_BWD_DB | MLORA_BWD_SGD_A | MLORA_BWD_SGD_B;
   if (!q8_dx && !saved8 && prob->dtype != MLORA_F32)
     return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack,
-                            dB_pack, stages, 0, p.n_tiles, 0, nb_out, nullptr, s);
+                            dB_pack, stages, 0, p.n_tiles, 0, nb_out, true, nullptr, s);
   // dZ (and the 16-bit dX), then the 8-bit dX, then the reductions
   const bool f32 = prob->dtype == MLORA_F32;
   int32_t first = stages & ~reduce;
@@ -479,7 +482,8 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     first &= ~MLORA_BWD_DZ;
   }
   st = backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, q8_dx ? nullptr : dX,
-                        dA_pack, dB_pack, first, 0, p.n_tiles, 0, nb_out, saved8 && dA_pack ? q8 : nullptr, s);
+                        dA_pack, dB_pack, first, 0, p.n_tiles, 0, nb_out, true,
+                        saved8 && dA_pack ? q8 : nullptr, s);
   if (st != MLORA_OK) return st;
   if (q8_dx) {
     st = q8_quantize(dY, prob->rows, prob->d_out, prob->d_out, prob->dtype, q8->w_scale, q8->Gq, q8->g_scale, s);
@@ -511,14 +515,14 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     if (!aligned(zsave, 16))
       return backward_kernels(prob, route, p, dev, MLORA_IMPL_SIMT, dY, nullptr, W, A_pack, B_pack, zsave, dzsave,
                               nullptr, nullptr, dB_pack, stages & (MLORA_BWD_DB | MLORA_BWD_SGD_B), 0, p.n_tiles, 0,
-                              nb_out, nullptr, s);
+                              nb_out, true, nullptr, s);
     float* upd = (stages & MLORA_BWD_SGD_B) ? (float*)const_cast<void*>(B_pack) : nullptr;
     return q8_sum32(1, dev, nullptr, nullptr, (const float*)dY, (const float*)zsave, (float*)dB_pack, prob->rows,
                     prob->d_out, route->r_pack, upd, prob->lr, s);
   }
   if (!saved8)
     return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, nullptr, dA_pack,
-                            dB_pack, stages & reduce, 0, p.n_tiles, 0, nb_out, nullptr, s);
+                            dB_pack, stages & reduce, 0, p.n_tiles, 0, nb_out, true, nullptr, s);
   // dA from the saved 8-bit rows, dB as ever
   const int32_t of_a = MLORA_BWD_DA | MLORA_BWD_SGD_A, of_b = MLORA_BWD_DB | MLORA_BWD_SGD_B;
   if (dA_pack && (stages & MLORA_BWD_DA) && impl == MLORA_IMPL_TC) {
@@ -526,12 +530,12 @@ int q8_backward(const mlora_problem* prob, const mlora_routing* route, const Pla
     if (st != MLORA_OK) return st;
   } else if (dA_pack && (stages & MLORA_BWD_DA)) {
     st = backward_kernels(prob, route, p, dev, MLORA_IMPL_SIMT, dY, nullptr, W, A_pack, B_pack, zsave, dzsave,
-                          nullptr, dA_pack, nullptr, stages & of_a, 0, p.n_tiles, 0, nb_out, q8, s);
+                          nullptr, dA_pack, nullptr, stages & of_a, 0, p.n_tiles, 0, nb_out, true, q8, s);
     if (st != MLORA_OK) return st;
   }
   if (!dB_pack || !(stages & MLORA_BWD_DB)) return MLORA_OK;
   return backward_kernels(prob, route, p, dev, impl, dY, nullptr, W, A_pack, B_pack, zsave, dzsave, nullptr, nullptr,
-                          dB_pack, stages & of_b, 0, p.n_tiles, 0, nb_out, nullptr, s);
+                          dB_pack, stages & of_b, 0, p.n_tiles, 0, nb_out, true, nullptr, s);
 }
 
 // mlora_backward_staged, or with `q8` mlora_backward_q8 over all ranges.
@@ -581,7 +585,7 @@ int backward_staged(const mlora_problem* prob, const mlora_routing* route, const
   if (q8) return q8_backward(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack,
                              dB_pack, stages, q8, s);
   return backward_kernels(prob, route, p, dev, impl, dY, X, W, A_pack, B_pack, zsave, dzsave, dX, dA_pack, dB_pack,
-                          stages, tile_begin, tile_end, db_begin, db_end, nullptr, s);
+                          stages, tile_begin, tile_end, db_begin, db_end, false, nullptr, s);
 }
 
 }  // namespace

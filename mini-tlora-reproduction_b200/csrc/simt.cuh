@@ -25,6 +25,8 @@ struct SimtCall {
   int bwd_stages = MLORA_BWD_DZ | MLORA_BWD_DX | MLORA_BWD_DA | MLORA_BWD_DB;
   int db0 = 0, db1 = 0;
   float lr = 0.f;  // fused SGD step (MLORA_BWD_SGD_A / _B)
+  // reductions: what is not finite in a row reaches no other segment's gradients
+  bool isolate = false;
   // dA from inputs saved in 8 bits: rows Xq [M, q8_ld(d_in)] with scales
   // x_scale stand for X, which may then be nullptr
   const int8_t* Xq = nullptr;

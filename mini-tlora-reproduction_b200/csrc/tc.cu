@@ -134,6 +134,7 @@ struct TcParams {
   int stage_bytes;  // 1-SM kernel: bytes per stage (multiple of 8 KB)
   int da_on;        // reduce: compute dA items
   int db0, db1;     // reduce: dB items of d_out blocks [db0, db1)
+  int isolate;      // reduce: rows of other segments in a slice are cleared, not multiplied by zero
   int f16;             // 16-bit elements are fp16 (else bf16)
   const __nv_bfloat16* bias;  // 16-bit elements (bf16 or fp16, see f16)
   __nv_bfloat16* out;  // Y, dX, Zt or dZt
@@ -530,6 +531,25 @@ __device__ __forceinline__ int4 reduce_entry(const TcParams& p, int e) {
   return d;
 }
 
+// REDUCE: the rows [x, y) of its tile that entry `d`'s segment owns
+__device__ __forceinline__ int2 reduce_rows(const TcParams& p, const int4& d) {
+  const Chunk& ch = p.plan.chunks[d.x];
+  return make_int2(ch.lo, ch.hi);
+}
+
+// REDUCE: clear the rows of a 64-row slice (two 64 x 64 boxes at `sA`, 128 bytes
+// a row) outside [lo, hi), for the MMAs that follow.  Warp-collective.
+__device__ __forceinline__ void clear_rows(uint32_t sA, int lo, int hi, int lane) {
+  if (lo <= 0 && hi >= 64) return;
+#pragma unroll 4
+  for (int e = lane; e < 2 * 64 * 8; e += 32) {
+    const int row = (e >> 3) & 63;
+    if (row < lo || row >= hi) sts128(sA + uint32_t(e >> 9) * kBox64 + uint32_t(row) * 128u + uint32_t(e & 7) * 16u, 0, 0, 0, 0);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
 // ------------------------------------------------------------------ tile scheduler
 // Work items are handed out dynamically: the producer thread of a CTA (of
 // the even CTA of a pair) takes the next item index from the launch's global
@@ -877,8 +897,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
         }
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && (lane == 0 || (MODE == REDUCE && p.isolate))) {
     // ---------------------------------------------------------------- MMA issuer
+    // One lane.  REDUCE with isolate: the whole warp, which clears the rows of
+    // other segments in a slice before its MMAs (their zero in the low-rank
+    // block would make a NaN of an infinity); lane 0 issues.
+    const bool whole = MODE == REDUCE && p.isolate;
+    auto all = [&](bool v) { return whole ? __all_sync(0xffffffffu, v) != 0 : v; };
     int stage = 0;
     uint32_t phase = 0;
     int acc = 0;
@@ -889,38 +914,63 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
     const uint32_t b_step = B_MN ? (16 * 128) >> 4 : 32 >> 4;
     SchedQ sq{sched_item, sched_full, sched_empty, 0, 0};
     for (int item = 0; ok;) {
-      if (!sched_take(sq, false, abort_flag, p.plan.err, item)) { ok = false; break; }
-      mbar_arrive(&sq.empty[sq.q]);
+      if (!all(sched_take(sq, false, abort_flag, p.plan.err, item))) { ok = false; break; }
+      if (whole) __syncwarp();  // every lane has the item
+      if (lane == 0) mbar_arrive(&sq.empty[sq.q]);
       sq.advance();
       if (item < 0) break;
       const Item it = decode<MODE>(p, item, kUnits);
       if (it.skip) continue;
-      if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err)) { ok = false; break; }
+      if (!all(mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err))) { ok = false; break; }
       tc_fence_after();
       const uint32_t d = tmem + uint32_t(acc * kAccCols);
       const uint32_t idesc = idesc_16(128, it.n, A_MN, B_MN, p.f16 != 0);
+      // isolate: the walk over the item's entries, as the producers' (m_r: own rows)
+      int m_e = 0, m_q = 0;
+      int4 m_d = make_int4(0, 0, 0, 0), m_n = m_d;
+      int2 m_r = make_int2(0, 0), m_s = m_r;
+      if (whole && it.nk > 0) {
+        m_e = it.ri.lb;
+        m_d = reduce_entry(p, m_e);
+        m_r = reduce_rows(p, m_d);
+        m_q = m_d.z;
+        if (m_e + 1 < it.ri.le) { m_n = reduce_entry(p, m_e + 1); m_s = reduce_rows(p, m_n); }
+      }
       for (int kb = 0; kb < it.nk; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, p.plan.err)) { ok = false; break; }
+        if (!all(mbar_wait(&full[stage], phase, abort_flag, p.plan.err))) { ok = false; break; }
         tc_fence_after();
         const uint32_t sA = su32(smem + stage * stage_bytes);
+        if (whole) {
+          clear_rows(sA, m_r.x - 64 * m_q, m_r.y - 64 * m_q, lane);
+          if (++m_q >= m_d.w && ++m_e < it.ri.le) {
+            m_d = m_n;
+            m_r = m_s;
+            m_q = m_d.z;
+            if (m_e + 1 < it.ri.le) { m_n = reduce_entry(p, m_e + 1); m_s = reduce_rows(p, m_n); }
+          }
+        }
         const uint64_t ad = sdesc(sA, a_lbo, 1024);
         const uint64_t bd = sdesc(sA + kA1Bytes, b_lbo, 1024);
+        if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc_mma(d, ad + uint64_t(k * a_step), bd + uint64_t(k * b_step), idesc, (kb | k) != 0);
-        tc_commit(&empty[stage]);
+          for (int k = 0; k < 4; ++k)
+            tc_mma(d, ad + uint64_t(k * a_step), bd + uint64_t(k * b_step), idesc, (kb | k) != 0);
+          tc_commit(&empty[stage]);
+        }
         if (++stage == n_stages) { stage = 0; phase ^= 1; }
       }
       if (!ok) break;
-      tc_commit(&tfull[acc]);
+      if (lane == 0) tc_commit(&tfull[acc]);
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
     // every issued MMA has completed once this commit lands
-    tc_commit(drain);
-    const unsigned long long t0 = now_ns();
-    while (!mbar_try(su32(drain), 0)) {
-      if (now_ns() - t0 > kTimeoutNs) { flag_error(p.plan.err, kErrTimeout); break; }
+    if (lane == 0) {
+      tc_commit(drain);
+      const unsigned long long t0 = now_ns();
+      while (!mbar_try(su32(drain), 0)) {
+        if (now_ns() - t0 > kTimeoutNs) { flag_error(p.plan.err, kErrTimeout); break; }
+      }
     }
   } else if (warp >= 2 && warp < 6) {
     // ---------------------------------------------------------------- epilogue
@@ -1980,6 +2030,7 @@ int tc_backward(const TcCall& a, cudaStream_t st) {
     prm.B_upd = db && (a.bwd_stages & MLORA_BWD_SGD_B)
                     ? reinterpret_cast<__nv_bfloat16*>(const_cast<void*>(a.B_pack)) : nullptr;
     prm.lr = a.lr;
+    prm.isolate = a.isolate ? 1 : 0;
     int nc = 1;
     for (const ReduceItem& r : a.host->reduce) nc = std::max(nc, int(r.nc));
     set_ring(prm, kA1Bytes, nc * kBox64);  // A: two 64x64 boxes

@@ -30,6 +30,8 @@ struct TcCall {
   bool pair_fwd = false;  // forward mainloop on 2-SM pairs (tcgen05 cta_group::2)
   bool pair_dx = true;    // dX mainloop on 2-SM pairs
   bool wide = false;      // the pair mainloops on 256 x 512 tiles (k_tc2w) instead of 256 x 256
+  // reductions: what is not finite in a row reaches no other segment's gradients
+  bool isolate = false;
   // backward shrink: x_scale dZ as bf16 high and low parts too (dA from inputs saved in 8 bits)
   const float* x_scale = nullptr;
   void* dz8 = nullptr;

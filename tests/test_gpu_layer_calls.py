@@ -403,3 +403,37 @@ def test_infinite_inputs_of_a_few_rows(dt, rows):
         y = m(x, ids)
     rest = [i for i in range(rows) if i not in (1, 2)]
     assert torch.equal(y[rest], clean[rest]) and torch.isnan(y[[1, 2]]).all()
+
+
+ODD = torch.cat([torch.full((n,), a, dtype=torch.int64) for a, n in ((0, 50), (1, 1), (2, 330), (-1, 9), (3, 70), (4, 300))])
+
+
+@pytest.mark.parametrize("base8, save8", [(True, False), (True, True), (False, True)])
+@pytest.mark.parametrize("impl, dt, d_in, d_out", [("auto", BF, 264, 200), ("auto", FP, 264, 200), ("auto", F32, 264, 200),
+                                                   ("simt", BF, 264, 200), ("simt", F32, 264, 200),
+                                                   ("auto", BF, 100, 75)])
+def test_bad_rows_reach_no_other_adapter(impl, dt, d_in, d_out, base8, save8):
+    """Segments that end inside a slice of rows that the reductions take at a
+    time: what is not finite in one segment's rows stays out of the others'."""
+    m = layer(d_in, d_out, {0: 4, 1: 72, 2: 16, 3: 300, 4: 8}, dt)
+    m.impl = impl
+    if base8:
+        m.quantize_base()
+    m.save_input = "int8" if save8 else "full"
+    rows = len(ODD)
+    x, dy = randn((rows, d_in), dt, 1), randn((rows, d_out), dt, 2, 0.1)
+    clean = step(m, x, ODD, dy)
+    for row in (0, 49, 50, 51, 380, 381, 389, 390, 459, 460, rows - 1):
+        owner = int(ODD[row])
+        rest = [i for i in range(rows) if i != row]
+        for bad_x in (True, False):
+            xs, ds = x.clone(), dy.clone()
+            (xs if bad_x else ds)[row, 3:6] = torch.tensor([float("inf"), float("nan"), float("-inf")])
+            y, dx, dA, dB = step(m, xs, ODD, ds)
+            assert torch.equal(y[rest], clean[0][rest]) and torch.equal(dx[rest], clean[1][rest])
+            for i in range(5):
+                if i != owner:
+                    assert torch.equal(dA[i], clean[2][i]) and torch.equal(dB[i], clean[3][i]), (row, bad_x, i)
+            if owner >= 0:
+                assert not torch.isfinite(dA[owner]).all() and not torch.isfinite(dB[owner]).all()
+    assert _lib.device_error() == 0
