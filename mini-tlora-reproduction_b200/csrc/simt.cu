@@ -170,15 +170,16 @@ __global__ void __launch_bounds__(NT) k_main(PlanDev plan, const T* __restrict__
 }
 
 // ---------------------------------------------------------------- reduce
-// grid (n_reduce, 4 chunks, 2 halves of the 128-wide block)
-template <class T>
+// grid (n_reduce, 4 chunks, 2 halves of the 128-wide block).  Q8: a reduction of
+// an 8-bit call, which may read X in 8 bits (Xq), and in which a row of another
+// segment of the tile counts as zero whatever it holds
+template <class T, bool Q8>
 __global__ void __launch_bounds__(NT) k_reduce(PlanDev plan, const T* __restrict__ X,
                                                 const T* __restrict__ dY, const T* __restrict__ zt,
                                                 const T* __restrict__ dzt, T* __restrict__ dA,
                                                 T* __restrict__ dB, int64_t M, int d_in, int d_out,
                                                 int R, int db0, int db1, T* A_upd, T* B_upd, float lr,
-                                                const int8_t* __restrict__ Xq, const float* __restrict__ x_scale,
-                                                int isolate) {
+                                                const int8_t* __restrict__ Xq, const float* __restrict__ x_scale) {
   __shared__ float As[BK][LD], Bs[BK][LD];
   const ReduceItem it = plan.reduce[blockIdx.x];
   const int jc = blockIdx.y;
@@ -195,14 +196,12 @@ __global__ void __launch_bounds__(NT) k_reduce(PlanDev plan, const T* __restrict
   auto fa = [&](int i, int tok) -> float {
     const int c = plan.list[it.lb + tok / kTileRows] + j;
     const int64_t row = int64_t(plan.chunks[c].tile) * kTileRows + tok % kTileRows;
-    if (row >= M || b0 + i >= D) return 0.f;
-    if (isolate) {
-      // a row of another segment of the tile counts as zero, whatever it holds
+    if constexpr (Q8) {
       const int rt = tok % kTileRows;
-      if (rt < plan.chunks[c].lo || rt >= plan.chunks[c].hi) return 0.f;
+      if (row >= M || b0 + i >= D || rt < plan.chunks[c].lo || rt >= plan.chunks[c].hi) return 0.f;
+      if (!is_dB && Xq) return float(Xq[row * q8_ld(d_in) + b0 + i]) * x_scale[row];
     }
-    if (!is_dB && Xq) return float(Xq[row * q8_ld(d_in) + b0 + i]) * x_scale[row];
-    return to_f(mat[row * D + b0 + i]);
+    return (row < M && b0 + i < D) ? to_f(mat[row * D + b0 + i]) : 0.f;
   };
   auto fb = [&](int jj, int tok) -> float {
     const int c = plan.list[it.lb + tok / kTileRows] + j;
@@ -293,10 +292,10 @@ int launch_backward(const SimtCall& a, cudaStream_t st) {
   if (a.n_reduce > 0 && (dA || dB)) {
     T* A_upd = dA && (a.bwd_stages & MLORA_BWD_SGD_A) ? (T*)a.A_pack : nullptr;
     T* B_upd = dB && (a.bwd_stages & MLORA_BWD_SGD_B) ? (T*)a.B_pack : nullptr;
-    k_reduce<T><<<dim3(a.n_reduce, kMaxChunksPerItem, 2), NT, 0, st>>>(
+    auto reduce = a.isolate ? &k_reduce<T, true> : &k_reduce<T, false>;
+    reduce<<<dim3(a.n_reduce, kMaxChunksPerItem, 2), NT, 0, st>>>(
         a.plan, (const T*)a.X, (const T*)a.dY, (const T*)a.zsave, (const T*)a.dzt, (T*)dA,
-        (T*)dB, a.M, a.d_in, a.d_out, a.R, a.db0, a.db1, A_upd, B_upd, a.lr, a.Xq, a.x_scale,
-        a.isolate ? 1 : 0);
+        (T*)dB, a.M, a.d_in, a.d_out, a.R, a.db0, a.db1, A_upd, B_upd, a.lr, a.Xq, a.x_scale);
     count_launch();
   }
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;

@@ -198,8 +198,10 @@ class _PackedAdapters:
 
     def params(self) -> list:
         """A_0, B_0, A_1, ... as the adapters hold them now."""
-        # (the parameters' dict is read directly: attribute lookups cost several times as much)
-        return [ad._parameters[k] if k in ad._parameters else getattr(ad, k) for ad in self.adapters for k in "AB"]
+        try:  # the parameters' dicts, read directly: attribute lookups cost several times as much
+            return [p[k] for p in [ad._parameters for ad in self.adapters] for k in ("A", "B")]
+        except KeyError:  # a weight that is no parameter
+            return [getattr(ad, k) for ad in self.adapters for k in ("A", "B")]
 
     def _in_sync(self, params) -> bool:
         # a parameter that no longer views the packs has another address: the
@@ -264,7 +266,8 @@ class _PackedAdapters:
     def apply(self, x, ids, W, bias, impl="auto", plan: Optional[ops.RoutePlan] = None,
               base8: Optional[ops.Int8Rows] = None, save8: bool = False):
         params = self.params()
-        ops._no_tangents(x, W, bias, *params)
+        if ops.forward_ad._current_level >= 0:
+            ops._no_tangents(x, W, bias, *params)
         x, Wc, bc = self.operands(x, W, bias, base8, params)
         if plan is None:
             plan = ops.route(ids, self.table, x.device)

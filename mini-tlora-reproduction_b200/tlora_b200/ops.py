@@ -63,8 +63,6 @@ class _on:
 def _no_tangents(*tensors) -> None:
     """Forward-mode derivatives are not computed: a tensor that carries one is
     refused, so that none is lost unseen."""
-    if forward_ad._current_level < 0:
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("forward-mode derivatives (jvp) are not computed")
@@ -460,7 +458,8 @@ def int8_linear(x, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
     131,072 terms: in_features, and out_features where x wants a gradient."""
     if not isinstance(weight, Int8Rows):
         raise TypeError("int8_linear expects weight as Int8Rows (quantize_rows(W))")
-    _no_tangents(None if isinstance(x, Int8Rows) else x, bias)
+    if forward_ad._current_level >= 0:
+        _no_tangents(None if isinstance(x, Int8Rows) else x, bias)
     dev = weight.q.device
     if dev.type != "cuda":
         _check_cuda(weight.q, "int8_linear")
@@ -533,8 +532,8 @@ class _CallArgs:
 def _call_key(rows, d_in, d_out, dtype, st: "LayerState") -> tuple:
     """All that the routing tables of a call are made from."""
     plan, table = st.plan, st.table
-    return (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.layout(), st.scaling.tobytes(),
-            plan.seg_start.tobytes(), plan.seg_adapter.tobytes())
+    return (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.rank.tobytes(), table.pack_off.tobytes(),
+            st.scaling.tobytes(), plan.seg_start.tobytes(), plan.seg_adapter.tobytes())
 
 
 class _Call:
