@@ -83,6 +83,10 @@ class GraphedTrainStep:
                 self._step()
         torch.cuda.current_stream(x.device).wait_stream(side)
         torch.cuda.synchronize(x.device)
+        # what the captured kernels read and update stays, even if the module's
+        # weights move, change their type or are replaced (quantize_base)
+        pk = model._pack()
+        self._kept = [t.detach() for t in (pk.A_pack, pk.B_pack, *model.parameters(), *model.buffers())]
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.y = self._step()

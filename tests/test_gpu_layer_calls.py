@@ -437,3 +437,22 @@ def test_bad_rows_reach_no_other_adapter(impl, dt, d_in, d_out, base8, save8):
             if owner >= 0:
                 assert not torch.isfinite(dA[owner]).all() and not torch.isfinite(dB[owner]).all()
     assert _lib.device_error() == 0
+
+
+def test_graphed_step_outlives_what_it_captured():
+    """The graph's kernels keep reading the weights they were captured with,
+    wherever the module's own go afterwards."""
+    for change in (lambda m: m.quantize_base(), lambda m: m.cpu(), lambda m: m.half()):
+        m = layer(1024, 1024, RANKS, BF)
+        x, dy = randn((len(IDS), 1024), BF, 1), randn((len(IDS), 1024), BF, 2, 0.1)
+        g = GraphedTrainStep(m, x, IDS, dy, lr=0.0)
+        want = g(x, dy).clone(), g.dx.clone()
+        held = {t.untyped_storage().data_ptr() for t in g._kept}
+        pk = m._pack()
+        assert {pk.A_pack.data_ptr(), pk.B_pack.data_ptr(), m.base.weight.data_ptr(), m.base.bias.data_ptr()} <= held
+        change(m)
+        m._pack().sync()
+        torch.cuda.empty_cache()
+        y = g(x, dy)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(g.dx, want[1])
