@@ -917,7 +917,8 @@ class MultiLoRAFunction(torch.autograd.Function):
         st: LayerState = ctx.st
         rows8 = _wrap8(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
         need = ctx.needs_input_grad
-        dx, dA, dB = backward_raw(dy.contiguous(), xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
+        with _on(dy.device):
+            dx, dA, dB = backward_raw(dy, xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
         # one call cuts a pack into all adapters' gradients
         cut, place = st.table.pieces()
         pa = torch.unsafe_split_with_sizes(dA, cut, 0) if dA is not None else None
