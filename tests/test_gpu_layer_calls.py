@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import _int8_ref as ref
+import _saved_ref as saved
 from tlora_b200 import MultiLoRALinear, _lib, ops
 from tlora_b200.graphs import GraphedTrainStep
 
@@ -456,3 +457,23 @@ def test_graphed_step_outlives_what_it_captured():
         y = g(x, dy)
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(g.dx, want[1])
+
+
+# ------------------------------------------------------------------ bits kept
+
+@pytest.mark.parametrize("base8", [False, True])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("counts, ranks", [((1, 64, 200), (4, 16, 64)), ((40, 8, 0), (130, 1, 8)),
+                                           ((6000, 90, 4100), (8, 33, 100))])
+def test_dA_from_saved_rows_is_rounded_once(counts, ranks, dt, base8):
+    m = layer(264, 192, dict(enumerate(ranks)), dt)
+    if base8:
+        m.quantize_base()
+    m.save_input = "int8"
+    ids = torch.cat([torch.full((n,), i, dtype=torch.int64) for i, n in enumerate(counts)])
+    x, dy = randn((len(ids), 264), dt, 1), randn((len(ids), 192), dt, 2, 0.1)
+    dA = step(m, x, ids, dy)[2]
+    for i, ad in enumerate(m.adapters.values()):
+        mine = (ids == i).cuda()
+        if counts[i]:
+            ref.assert_within(dA[i], *saved.dA_saved(x[mine], ad.B.detach(), ad.scaling, dy[mine]), what=f"dA{i}")

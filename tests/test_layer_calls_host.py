@@ -297,3 +297,19 @@ def test_adapter_weights_that_are_plain_tensors():
     assert pk.params()[0] is new and pk.params()[1] is ad.B
     pk.sync()
     assert torch.equal(pk.A_pack[:4], new.detach())
+
+
+# ------------------------------------------------------------------ the oracle itself
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [8, 64, 200])
+def test_bound_of_saved_dA_sees_a_lost_low_part(dt, n):
+    import _saved_ref as saved
+
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, 256, generator=g).to(dt)
+    dy, B = (torch.randn(n, 192, generator=g) * 0.1).to(dt), (torch.randn(192, 16, generator=g) * 0.05).to(dt)
+    v, bound = saved.dA_saved(x, B, 0.75, dy)
+    assert bool(((saved.dA_both(x, B, 0.75, dy).double() - v).abs() <= bound).all())
+    lost = (saved.dA_high_only(x, B, 0.75, dy).double() - v).abs() > bound
+    assert int(lost.sum()) >= 16  # of 4096: elements whose terms nearly cancel
