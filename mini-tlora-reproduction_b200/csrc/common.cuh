@@ -70,7 +70,7 @@ struct PlanDev {
   const ShrinkItem* shrink;         // [n_shrink]
   const ReduceItem* reduce;         // [n_reduce]
   const int32_t* list;              // [n_list] base chunk ids, grouped by adapter
-  const int4* list_desc;            // [n_list] {base chunk, tile, first 64-row slice, one past the last}
+  const int4* list_desc;            // [n_list] {base chunk, tile, first row of the tile, one past the last}
   int32_t* counters;                // [16] work counters of the persistent kernels, one per role;
                                     // zeroed by every plan upload (one per API call)
   const SavedItem* saved;           // [n_saved]
@@ -78,6 +78,10 @@ struct PlanDev {
   int* err;                         // status word of this call (mlora_problem.err_word), or nullptr
                                     // for the library-wide word g_err_word
 };
+
+// The 64-row slices [first, end) of its tile that an entry's rows lie in.
+inline __host__ __device__ int first_slice(const int4& d) { return d.z / 64; }
+inline __host__ __device__ int end_slice(const int4& d) { return (d.w + 63) / 64; }
 
 // Host-side plan built from the routing description.
 struct Plan {
@@ -90,7 +94,7 @@ struct Plan {
   std::vector<SavedItem> saved;
   int32_t saved_groups = 0, saved_parts = 0;  // groups of several parts, and their parts
   std::vector<int32_t> list;
-  std::vector<int4> list_desc;      // per list entry: {base chunk, tile, first slice, end slice}
+  std::vector<int4> list_desc;      // per list entry: {base chunk, tile, first row, end row}
   std::vector<int32_t> list_begin;  // [n_adapters + 1]
   std::vector<uint8_t> adapter_active;
   // byte layout of the plan inside the workspace

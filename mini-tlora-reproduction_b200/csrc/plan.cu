@@ -115,7 +115,7 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
     p->list_desc.resize(p->list.size());
     for (size_t e = 0; e < p->list.size(); ++e) {
       const Chunk& ch = p->chunks[p->list[e]];
-      p->list_desc[e] = make_int4(p->list[e], ch.tile, ch.lo / 64, (ch.hi + 63) / 64);
+      p->list_desc[e] = make_int4(p->list[e], ch.tile, ch.lo, ch.hi);
     }
   }
 
@@ -165,7 +165,8 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
     std::vector<int32_t> nks(nad, 0);
     int64_t work = 0;
     for (int a = 0; a < nad; ++a) {
-      for (int e = p->list_begin[a]; e < p->list_begin[a + 1]; ++e) nks[a] += p->list_desc[e].w - p->list_desc[e].z;
+      for (int e = p->list_begin[a]; e < p->list_begin[a + 1]; ++e)
+        nks[a] += end_slice(p->list_desc[e]) - first_slice(p->list_desc[e]);
       work += int64_t(nks[a]) * nb * ((r->rank[a] + kChunk - 1) / kChunk);
     }
     const int64_t quota = std::max<int64_t>(kSavedMin, (work + kSavedItems - 1) / kSavedItems);
@@ -176,10 +177,10 @@ int build_plan(const mlora_problem* prob, const mlora_routing* r, Plan* p) {
       const int nch = (r->rank[a] + kChunk - 1) / kChunk;
       // the first entry and slice of every part
       std::vector<std::pair<int, int>> from;
-      for (int k = 0, e = lb, q = p->list_desc[lb].z, k0 = 0; k < parts; ++k) {
+      for (int k = 0, e = lb, q = first_slice(p->list_desc[lb]), k0 = 0; k < parts; ++k) {
         const int k1 = int(int64_t(nks[a]) * k / parts);
         for (; k0 < k1; ++k0)
-          if (++q >= p->list_desc[e].w && ++e < le) q = p->list_desc[e].z;
+          if (++q >= end_slice(p->list_desc[e]) && ++e < le) q = first_slice(p->list_desc[e]);
         from.push_back({e, q});
       }
       for (int b = 0; b < nb; ++b)

@@ -674,11 +674,12 @@ __device__ __forceinline__ int da_deal(int k, int n_items) {
 // if the plan is corrupted)
 __device__ __forceinline__ int4 da_entry(const DaParams& p, int e) {
   int4 d = p.plan.list_desc[e];
-  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > 4 || d.z >= d.w) {
+  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > kTileRows ||
+      d.z >= d.w) {
     flag_error(p.plan.err, kErrBounds);
     d = make_int4(0, 0, 0, 1);
   }
-  return d;
+  return make_int4(d.x, d.y, first_slice(d), end_slice(d));
 }
 
 // two bytes of `w` (selected into the low bytes of the halves) as bf16: a

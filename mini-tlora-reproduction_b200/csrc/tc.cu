@@ -134,7 +134,6 @@ struct TcParams {
   int stage_bytes;  // 1-SM kernel: bytes per stage (multiple of 8 KB)
   int da_on;        // reduce: compute dA items
   int db0, db1;     // reduce: dB items of d_out blocks [db0, db1)
-  int isolate;      // reduce: rows of other segments in a slice are cleared, not multiplied by zero
   int f16;             // 16-bit elements are fp16 (else bf16)
   const __nv_bfloat16* bias;  // 16-bit elements (bf16 or fp16, see f16)
   __nv_bfloat16* out;  // Y, dX, Zt or dZt
@@ -519,32 +518,26 @@ __device__ __forceinline__ Item decode(const TcParams& p, int item, int units) {
   return it;
 }
 
-// REDUCE: list entry e of a reduce item -> {base chunk, tile, first slice,
-// end slice} (the 64-row slices of the tile that hold the segment's rows), one
-// 16-byte load; out-of-range values (a corrupted plan) are flagged and clamped
+// REDUCE: list entry e of a reduce item -> {base chunk, tile, first row of the
+// tile that the segment owns, one past the last}, one 16-byte load;
+// out-of-range values (a corrupted plan) are flagged and clamped
 __device__ __forceinline__ int4 reduce_entry(const TcParams& p, int e) {
   int4 d = p.plan.list_desc[e];
-  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > 4 || d.z > d.w) {
+  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > kTileRows || d.z > d.w) {
     flag_error(p.plan.err, kErrBounds);
     d = make_int4(0, 0, 0, 0);
   }
   return d;
 }
 
-// REDUCE: the rows [x, y) of its tile that entry `d`'s segment owns
-__device__ __forceinline__ int2 reduce_rows(const TcParams& p, const int4& d) {
-  const Chunk& ch = p.plan.chunks[d.x];
-  return make_int2(ch.lo, ch.hi);
-}
-
 // REDUCE: clear the rows of a 64-row slice (two 64 x 64 boxes at `sA`, 128 bytes
 // a row) outside [lo, hi), for the MMAs that follow.  Warp-collective.
 __device__ __forceinline__ void clear_rows(uint32_t sA, int lo, int hi, int lane) {
-  if (lo <= 0 && hi >= 64) return;
 #pragma unroll 4
   for (int e = lane; e < 2 * 64 * 8; e += 32) {
     const int row = (e >> 3) & 63;
-    if (row < lo || row >= hi) sts128(sA + uint32_t(e >> 9) * kBox64 + uint32_t(row) * 128u + uint32_t(e & 7) * 16u, 0, 0, 0, 0);
+    if (row < lo || row >= hi)
+      sts128(sA + uint32_t(e >> 9) * kBox64 + uint32_t(row) * 128u + uint32_t(e & 7) * 16u, 0, 0, 0, 0);
   }
   fence_async_smem();
   __syncwarp();
@@ -731,8 +724,13 @@ __device__ __forceinline__ void epi_main_slice(const TcParams& p, int64_t row_w0
 }
 
 // ------------------------------------------------------------------ 1-SM kernel
-template <int MODE>
-__global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcParams p) {
+// ISO (REDUCE): rows of other segments in a slice are cleared, not multiplied by
+// zero, which would make a NaN of an infinity; by a warp more.
+constexpr int kClearWarp = kThreads / 32;
+constexpr int kWholeSlice = 64 << 8;  // rows_of: first | one past the last << 8, of the 64
+template <bool ISO> constexpr int kThreads1 = kThreads + (ISO ? 32 : 0);
+template <int MODE, bool ISO = false>
+__global__ void __launch_bounds__(kThreads1<ISO>, 1) k_tc(const __grid_constant__ TcParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage_out = smem + kRing1Bytes;
@@ -746,6 +744,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
   uint64_t* sched_full = reinterpret_cast<uint64_t*>(const_cast<int*>(abort_flag) + 1);  // [kSched]
   uint64_t* sched_empty = sched_full + kSched;                                          // [kSched]
   volatile int32_t* sched_item = reinterpret_cast<volatile int32_t*>(sched_empty + kSched);
+  // ISO, per stage: rows cleared; and which rows are the segment's own
+  uint64_t* cleared = reinterpret_cast<uint64_t*>(const_cast<int32_t*>(sched_item) + kSched);
+  volatile int32_t* rows_of = reinterpret_cast<volatile int32_t*>(cleared + kMaxStages1);
   const int n_stages = p.n_stages, stage_bytes = p.stage_bytes;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -756,7 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], ISO ? 2 : 1);  // the MMAs, and the clearing warp
+      if (ISO) mbar_init(&cleared[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
@@ -765,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
     mbar_init(drain, 1);
     for (int q = 0; q < kSched; ++q) {
       mbar_init(&sched_full[q], 1);
-      mbar_init(&sched_empty[q], 1 + 4 + kProducers - 1);  // the MMA thread, the epilogue warps, the other producers
+      mbar_init(&sched_empty[q], 1 + 4 + kProducers - 1 + (ISO ? 1 : 0));  // the MMA thread, the epilogue warps, the other producers
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -782,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
   const uint32_t tmem = *tmem_slot;
 
   if (MODE == SHRINK_FWD || MODE == SHRINK_BWD) grid_dep_launch();  // the mainloop after it may start
-  if ((warp == 0 || warp >= 6) && lane == 0) {
+  if ((warp == 0 || (warp >= 6 && warp < kClearWarp)) && lane == 0) {
     // ---------------------------------------------------------------- TMA producers
     // Warp 0 claims the work items and publishes them; warp 6 takes them from
     // the queue.  Both walk every k-block; k-block g of the launch (counted
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
       if (MODE == REDUCE && it.nk > 0) {
         r_e = it.ri.lb;
         r_d = reduce_entry(p, r_e);
-        r_q = r_d.z;
+        r_q = first_slice(r_d);
         if (r_e + 1 < it.ri.le) r_n = reduce_entry(p, r_e + 1);
       }
 
@@ -869,6 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
           } else {  // REDUCE: k-block kb = slice r_q of list entry r_e
             const CUtensorMap* ma = it.ri.kind == 0 ? &p.mA0 : &p.mA1;
             const CUtensorMap* mb = it.ri.kind == 0 ? &p.mB0 : &p.mB1;
+            if (ISO) rows_of[stage] = max(r_d.z - 64 * r_q, 0) | min(r_d.w - 64 * r_q, 64) << 8;
             mbar_expect_tx(bar, 2 * kBox64 + it.nc * kBox64);
             for (int i = 0; i < 2; ++i)
               tma_load(sA + i * kBox64, ma, bar, it.ri.block * 128 + 64 * i, r_d.y * kTileRows + 64 * r_q, pol_stream);
@@ -878,9 +881,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
           issued |= 1u << stage;
           issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
         }
-        if (MODE == REDUCE && ++r_q >= r_d.w && ++r_e < it.ri.le) {  // both warps walk the list
+        if (MODE == REDUCE && ++r_q >= end_slice(r_d) && ++r_e < it.ri.le) {  // both warps walk the list
           r_d = r_n;
-          r_q = r_d.z;
+          r_q = first_slice(r_d);
           if (r_e + 1 < it.ri.le) r_n = reduce_entry(p, r_e + 1);
         }
         if (++stage == n_stages) { stage = 0; phase ^= 1; }
@@ -897,79 +900,86 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
         }
       }
     }
-  } else if (warp == 1 && (lane == 0 || (MODE == REDUCE && p.isolate))) {
+  } else if (warp == 1 && lane == 0) {
     // ---------------------------------------------------------------- MMA issuer
-    // One lane.  REDUCE with isolate: the whole warp, which clears the rows of
-    // other segments in a slice before its MMAs (their zero in the low-rank
-    // block would make a NaN of an infinity); lane 0 issues.
-    const bool whole = MODE == REDUCE && p.isolate;
-    auto all = [&](bool v) { return whole ? __all_sync(0xffffffffu, v) != 0 : v; };
     int stage = 0;
     uint32_t phase = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
+    uint32_t cleared_par = 0;  // ISO: per stage, the phase of its cleared barrier
     bool ok = true;
     const uint32_t a_lbo = A_MN ? uint32_t(kBox64) : 16u, b_lbo = B_MN ? uint32_t(kBox64) : 16u;
     const uint32_t a_step = A_MN ? (16 * 128) >> 4 : 32 >> 4;  // descriptor units per UMMA_K = 16
     const uint32_t b_step = B_MN ? (16 * 128) >> 4 : 32 >> 4;
     SchedQ sq{sched_item, sched_full, sched_empty, 0, 0};
     for (int item = 0; ok;) {
-      if (!all(sched_take(sq, false, abort_flag, p.plan.err, item))) { ok = false; break; }
-      if (whole) __syncwarp();  // every lane has the item
+      if (!sched_take(sq, false, abort_flag, p.plan.err, item)) { ok = false; break; }
+      mbar_arrive(&sq.empty[sq.q]);
+      sq.advance();
+      if (item < 0) break;
+      const Item it = decode<MODE>(p, item, kUnits);
+      if (it.skip) continue;
+      if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(acc * kAccCols);
+      const uint32_t idesc = idesc_16(128, it.n, A_MN, B_MN, p.f16 != 0);
+      for (int kb = 0; kb < it.nk; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, p.plan.err)) { ok = false; break; }
+        if (ISO && rows_of[stage] != kWholeSlice) {
+          if (!mbar_wait(&cleared[stage], (cleared_par >> stage) & 1u, abort_flag, p.plan.err)) { ok = false; break; }
+          cleared_par ^= 1u << stage;
+        }
+        tc_fence_after();
+        const uint32_t sA = su32(smem + stage * stage_bytes);
+        const uint64_t ad = sdesc(sA, a_lbo, 1024);
+        const uint64_t bd = sdesc(sA + kA1Bytes, b_lbo, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma(d, ad + uint64_t(k * a_step), bd + uint64_t(k * b_step), idesc, (kb | k) != 0);
+        tc_commit(&empty[stage]);
+        if (++stage == n_stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) break;
+      tc_commit(&tfull[acc]);
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    // every issued MMA has completed once this commit lands
+    tc_commit(drain);
+    const unsigned long long t0 = now_ns();
+    while (!mbar_try(su32(drain), 0)) {
+      if (now_ns() - t0 > kTimeoutNs) { flag_error(p.plan.err, kErrTimeout); break; }
+    }
+  } else if (ISO && warp == kClearWarp) {
+    // ---------------------------------------------------------------- clearing of other segments' rows
+    // Looks at every slice (the stage is free again only after that) and clears
+    // the rows of those that the item's segment does not fill.  A warp of its
+    // own: the issuer must not fall behind the copies, or HBM idles (dB of 65,536
+    // x 11,008 and 8 jobs: 248 us; 240 without any clearing, 335 to 355 with it in
+    // the issuer's warp).
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto all = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
+    SchedQ sq{sched_item, sched_full, sched_empty, 0, 0};
+    for (int item = 0; ok;) {
+      if (!all(sched_take(sq, false, abort_flag, p.plan.err, item))) break;
+      __syncwarp();
       if (lane == 0) mbar_arrive(&sq.empty[sq.q]);
       sq.advance();
       if (item < 0) break;
       const Item it = decode<MODE>(p, item, kUnits);
       if (it.skip) continue;
-      if (!all(mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.plan.err))) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t d = tmem + uint32_t(acc * kAccCols);
-      const uint32_t idesc = idesc_16(128, it.n, A_MN, B_MN, p.f16 != 0);
-      // isolate: the walk over the item's entries, as the producers' (m_r: own rows)
-      int m_e = 0, m_q = 0;
-      int4 m_d = make_int4(0, 0, 0, 0), m_n = m_d;
-      int2 m_r = make_int2(0, 0), m_s = m_r;
-      if (whole && it.nk > 0) {
-        m_e = it.ri.lb;
-        m_d = reduce_entry(p, m_e);
-        m_r = reduce_rows(p, m_d);
-        m_q = m_d.z;
-        if (m_e + 1 < it.ri.le) { m_n = reduce_entry(p, m_e + 1); m_s = reduce_rows(p, m_n); }
-      }
       for (int kb = 0; kb < it.nk; ++kb) {
         if (!all(mbar_wait(&full[stage], phase, abort_flag, p.plan.err))) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t sA = su32(smem + stage * stage_bytes);
-        if (whole) {
-          clear_rows(sA, m_r.x - 64 * m_q, m_r.y - 64 * m_q, lane);
-          if (++m_q >= m_d.w && ++m_e < it.ri.le) {
-            m_d = m_n;
-            m_r = m_s;
-            m_q = m_d.z;
-            if (m_e + 1 < it.ri.le) { m_n = reduce_entry(p, m_e + 1); m_s = reduce_rows(p, m_n); }
-          }
+        const int rows = rows_of[stage];
+        if (rows != kWholeSlice) {
+          clear_rows(su32(smem + stage * stage_bytes), rows & 0xff, rows >> 8, lane);
+          if (lane == 0) mbar_arrive(&cleared[stage]);
         }
-        const uint64_t ad = sdesc(sA, a_lbo, 1024);
-        const uint64_t bd = sdesc(sA + kA1Bytes, b_lbo, 1024);
-        if (lane == 0) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma(d, ad + uint64_t(k * a_step), bd + uint64_t(k * b_step), idesc, (kb | k) != 0);
-          tc_commit(&empty[stage]);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
         if (++stage == n_stages) { stage = 0; phase ^= 1; }
-      }
-      if (!ok) break;
-      if (lane == 0) tc_commit(&tfull[acc]);
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
-    }
-    // every issued MMA has completed once this commit lands
-    if (lane == 0) {
-      tc_commit(drain);
-      const unsigned long long t0 = now_ns();
-      while (!mbar_try(su32(drain), 0)) {
-        if (now_ns() - t0 > kTimeoutNs) { flag_error(p.plan.err, kErrTimeout); break; }
       }
     }
   } else if (warp >= 2 && warp < 6) {
@@ -1012,6 +1022,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcPa
             float f[32];
 #pragma unroll
             for (int q = 0; q < 32; ++q) f[q] = in ? ch.scale * __uint_as_float(v[q]) : 0.f;
+            // rounded to the layer's type: it is an operand of the expand, of dX and
+            // of the reductions, whose other operand has that type, and it is what
+            // the forward keeps; float32 blocks would double both.  y and dx do not
+            // show it behind their own rounding; dA and dB are off by up to sqrt(2)
+            // of one rounding
             store32(dst + col, f, p.f16);
             if (MODE == SHRINK_BWD && p.dz8) {
               // the product with the saved integers has no rounding of its
@@ -1774,7 +1789,7 @@ cudaError_t launch_k(K kern, dim3 grid, int threads, int smem, cudaStream_t st, 
   return cudaLaunchKernelEx(&cfg, kern, prm);
 }
 
-template <int MODE>
+template <int MODE, bool ISO = false>
 int launch1(TcParams& prm, cudaStream_t st, int max_ctas, bool pdl = false) {
   if (prm.n_items <= 0) return MLORA_OK;
   if (prm.n_stages < 2 || prm.n_stages > kMaxStages1 || prm.stage_bytes % 1024 != 0 ||
@@ -1782,7 +1797,7 @@ int launch1(TcParams& prm, cudaStream_t st, int max_ctas, bool pdl = false) {
     return MLORA_ERR_INVALID_ARG;
   const int sms = cta_budget(max_ctas);
   if (sms <= 0) return MLORA_ERR_CUDA;
-  MLORA_CUDA_TRY(set_smem_once(reinterpret_cast<const void*>(&k_tc<MODE>), kSmem1));
+  MLORA_CUDA_TRY(set_smem_once(reinterpret_cast<const void*>(&k_tc<MODE, ISO>), kSmem1));
   prm.counter = prm.plan.counters + MODE;  // zeroed by the plan upload of this API call
   int grid = prm.n_items < sms ? prm.n_items : sms;
   if (MODE == SHRINK_FWD || MODE == SHRINK_BWD) {
@@ -1796,7 +1811,7 @@ int launch1(TcParams& prm, cudaStream_t st, int max_ctas, bool pdl = false) {
   const bool timed = timing_begin(st, ev);
   if (timed || !pdl_enabled()) pdl = false;  // events between the launches order them anyway
   prm.pdl_wait = pdl ? 1 : 0;
-  MLORA_CUDA_TRY(launch_k(k_tc<MODE>, dim3(grid), kThreads, kSmem1, st, pdl, prm));
+  MLORA_CUDA_TRY(launch_k(k_tc<MODE, ISO>, dim3(grid), kThreads1<ISO>, kSmem1, st, pdl, prm));
   count_launch();
   if (timed) timing_end(MODE, st, ev);
   return cudaGetLastError() == cudaSuccess ? MLORA_OK : MLORA_ERR_CUDA;
@@ -2030,11 +2045,11 @@ int tc_backward(const TcCall& a, cudaStream_t st) {
     prm.B_upd = db && (a.bwd_stages & MLORA_BWD_SGD_B)
                     ? reinterpret_cast<__nv_bfloat16*>(const_cast<void*>(a.B_pack)) : nullptr;
     prm.lr = a.lr;
-    prm.isolate = a.isolate ? 1 : 0;
     int nc = 1;
     for (const ReduceItem& r : a.host->reduce) nc = std::max(nc, int(r.nc));
     set_ring(prm, kA1Bytes, nc * kBox64);  // A: two 64x64 boxes
-    if ((s = launch1<REDUCE>(prm, st, a.max_ctas)) != MLORA_OK) return s;
+    s = a.isolate ? launch1<REDUCE, true>(prm, st, a.max_ctas) : launch1<REDUCE>(prm, st, a.max_ctas);
+    if (s != MLORA_OK) return s;
   }
   return MLORA_OK;
 }
