@@ -429,10 +429,11 @@ int mlora_q8_dequantize(const int8_t* q, const float* scale, int64_t rows, int64
  * prob gives rows, d_in, d_out, dtype (of X, bias, Y, dY, dX), max_ctas and
  * err_word.  max_ctas caps the tensor-core kernel, which takes CTAs in pairs
  * (with 1 the CUDA-core product serves); a forward of at most 16 rows streams
- * the weight through short blocks and takes no cap.  X (rows ld_x elements apart) is quantized into Xq / x_scale
- * first; with X NULL they hold the 8-bit rows already.  dY is quantized into
- * the scratch Gq [rows, mlora_q8_ld(d_out)] / g_scale [rows].  The integer
- * sums are exact; one rounding to dtype at the end. */
+ * the weight through short blocks and takes no cap.  X (rows ld_x elements
+ * apart) is quantized into Xq / x_scale first; with X NULL they hold the 8-bit
+ * rows already.  dY is quantized into the scratch Gq [rows, mlora_q8_ld(d_out)]
+ * / g_scale [rows]: dX is the gradient with dY in 8 bits too.  The integer sums
+ * are exact; one rounding to dtype at the end. */
 int mlora_q8_linear(const mlora_problem* prob, const void* X, int64_t ld_x, int8_t* Xq, float* x_scale,
                     const int8_t* Wq, const float* w_scale, const void* bias, void* Y, void* stream);
 int mlora_q8_linear_dx(const mlora_problem* prob, const void* dY, int8_t* Gq, float* g_scale, const int8_t* Wq,
@@ -463,7 +464,9 @@ int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, cons
 /* mlora_backward with dX through the 8-bit backbone (q8->Wq) and / or dA from
  * the saved 8-bit rows (q8->Xq):
  *     dA_a = sum_seg (s_a dY_seg B_a)^T (x_scale Xq)_seg.
- * X is read for dA only. */
+ * X is read for dA only.  What is not finite in a row of X or dY reaches the
+ * gradients of that row's adapter and no other's (mlora_backward sums rows in
+ * groups of 64, which it may share between adapters). */
 int mlora_backward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
                       const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
                       const void* zsave, void* dX, void* dA_pack, void* dB_pack, void* workspace,

@@ -256,8 +256,9 @@ template <int NV> constexpr int kQuantBlocks = NV == 6 ? 3 : NV == 8 ? 8 : NV ==
 // out per 16-bit element, if the work around each row is spread over enough
 // elements of a thread and enough rows are in flight (kQuantBlocks).  65,536 x
 // 4096 bf16: 122 us (its bytes: 123; 148 with twice the registers and half the
-// warps); with column scales 4096 columns 148 us, 11,008 columns 499 (331): two
-// more loads and a product an element, and values held in float32.
+// warps); float32 200 us (205).  With column scales bf16 4096 columns 148 us, 11,008
+// columns 499 (331), float32 4096 columns 232 (205): two more loads and a product
+// an element, and values held in float32.
 template <class T, bool VEC, bool CS, int NV>
 __global__ void __launch_bounds__(kQuantThreads<NV>, kQuantBlocks<NV>)
     k_quantize(const T* __restrict__ src, int64_t rows, int cols, int64_t ld,
@@ -567,9 +568,9 @@ __global__ void __launch_bounds__(NT) k_q8_main(Q8Main a, int nb0) {
 // pack row holds the ranks of one k).  A block takes kLowRows rows of one
 // chunk and its eight warps share out K; lane l sums ranks l and l + 32, the
 // warps' sums are added in their order.  Ranks past the adapter's are zero
-// without being computed.  640 rows, K = 1024, four jobs: 25 us forward, 14 us
-// backward (the 64 x 64 tile product of the CUDA-core family: 105 and 74, with
-// 24 blocks).  Latency of the operands' loads bounds it.
+// without being computed.  640 rows, K = 1024, four jobs: 17 us forward, 12 us
+// backward in a running step (the 64 x 64 tile product of the CUDA-core family:
+// 105 and 74, with 24 blocks; the bytes and operations: under 1).  Latency of the operands' loads bounds it.
 constexpr int kLowRows = 8, kLowWarps = 8, kLowStep = 32;
 
 template <bool BWD>
@@ -640,8 +641,9 @@ __global__ void __launch_bounds__(kLowWarps * 32) k_low32(PlanDev plan, const fl
 //   dA[r, col] = sum_i dZt[i, r] x[i, col],   dB[col, r] = sum_i Zt[i, r] dY[i, col].
 // The eight warps share out the rows of each tile, lane l holds columns 2 l and
 // 2 l + 1; their sums are added in order.  Only rows of the adapter's segments
-// are read.  640 rows x 1024, four jobs: 19 us (the CUDA-core family's
-// reduction: 98, over whole tiles with index tables in the inner loop).
+// are read.  640 rows x 1024, four jobs: 11 us for dA, 14 us for dB in a running
+// step (the CUDA-core family's reduction: 98, over whole tiles with index tables
+// in the inner loop; the bytes and operations: under 1).  zt is 16-byte aligned.
 constexpr int kSumRanks = 16, kSumCols = 64;
 template <int KIND, bool SRC8>
 __global__ void __launch_bounds__(256) k_sum32(PlanDev plan, const int8_t* __restrict__ Xq,

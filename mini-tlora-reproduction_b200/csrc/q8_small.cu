@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(kFewThreads) k_few_prep(const __grid_constant_
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) s += sums[w][j][threadIdx.x / kFewCh];
+      // rounded to the layer's type, as the tensor-core shrink leaves it: the same
+      // block serves the expand here and dB in the backward
       zt[int64_t(row) * kChunk + j] = from_f<T>(ck.scale * s);
     }
   }

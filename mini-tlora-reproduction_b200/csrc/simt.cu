@@ -163,7 +163,9 @@ __global__ void __launch_bounds__(NT) k_main(PlanDev plan, const T* __restrict__
       if (n >= N) continue;
       float v = acc[i][j];
       if (!BWD && bias) v += to_f(bias[n]);
-      if (add) v += to_f(out[orow * N + n]);  // onto a product already there
+      // onto a product already there, rounded to T (float32): one rounding more
+      // than a sum in registers would have, 2^-24 of the product
+      if (add) v += to_f(out[orow * N + n]);
       out[orow * N + n] = from_f<T>(v);
     }
   }
