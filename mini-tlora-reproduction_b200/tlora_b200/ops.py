@@ -37,8 +37,15 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _stream(device: torch.device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _stream(device):
+    """The current stream of a CUDA device (no other: it is where the calls'
+    pointers are checked to be a GPU's)."""
+    if not isinstance(device, torch.device):
+        device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"expected a CUDA device, not {device}")
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 class _on:

@@ -313,3 +313,19 @@ def test_bound_of_saved_dA_sees_a_lost_low_part(dt, n):
     assert bool(((saved.dA_both(x, B, 0.75, dy).double() - v).abs() <= bound).all())
     lost = (saved.dA_high_only(x, B, 0.75, dy).double() - v).abs() > bound
     assert int(lost.sum()) >= 16  # of 4096: elements whose terms nearly cancel
+
+
+# ------------------------------------------------------------------ devices and plain containers
+
+def test_streams_of_devices(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    assert ops._stream(torch.device("cuda", 1)) == 101
+    assert ops._stream(torch.device("cuda")) == 103 and ops._stream("cuda") == 103 and ops._stream("cuda:2") == 102
+    for bad in (torch.device("cpu"), torch.device("cpu", 0), "cpu"):  # host pointers must not reach a kernel
+        with pytest.raises(ValueError, match="CUDA"):
+            ops._stream(bad)
+    x, perm = torch.zeros(2, 16, device="cpu:0"), torch.zeros(2, dtype=torch.int32)
+    for call in (ops.gather_rows, ops.scatter_rows):
+        with pytest.raises(ValueError, match="CUDA"):
+            call(x, perm)
