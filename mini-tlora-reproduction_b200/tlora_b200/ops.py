@@ -539,8 +539,9 @@ class _CallArgs:
 def _call_key(rows, d_in, d_out, dtype, st: "LayerState") -> tuple:
     """All that the routing tables of a call are made from."""
     plan, table = st.plan, st.table
-    return (rows, d_in, d_out, dtype, st.impl, table.r_pack, table.rank.tobytes(), table.pack_off.tobytes(),
-            st.scaling.tobytes(), plan.seg_start.tobytes(), plan.seg_adapter.tobytes())
+    return (rows, d_in, d_out, dtype, st.impl, table.r_pack,
+            *[a.tobytes() if type(a) is np.ndarray else np.asarray(a).tobytes()
+              for a in (table.rank, table.pack_off, st.scaling, plan.seg_start, plan.seg_adapter)])
 
 
 class _Call:
@@ -558,9 +559,9 @@ class _Call:
         if kept is None:
             # copies: what is kept must not change with the caller's arrays
             args = _CallArgs(rows, d_in, d_out, dtype, st.impl,
-                             RoutePlan(plan.rows, plan.seg_start.copy(), plan.seg_adapter.copy()),
-                             AdapterTable(table.ids, table.rank.copy(), table.pack_off.copy(), table.r_pack),
-                             st.scaling.copy(), out_rows=perm)
+                             RoutePlan(plan.rows, np.array(plan.seg_start), np.array(plan.seg_adapter)),
+                             AdapterTable(table.ids, np.array(table.rank), np.array(table.pack_off), table.r_pack),
+                             np.array(st.scaling), out_rows=perm)
             kept = (args, args.sizes(), {})
             if len(plan.calls) >= 8:  # plans or scalings that change from call to call
                 plan.calls.clear()

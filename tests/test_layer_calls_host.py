@@ -329,3 +329,14 @@ def test_streams_of_devices(monkeypatch):
     for call in (ops.gather_rows, ops.scatter_rows):
         with pytest.raises(ValueError, match="CUDA"):
             call(x, perm)
+
+
+def test_plans_and_scalings_given_as_lists():
+    a = state()
+    b = state()
+    b.plan = ops.RoutePlan(40, [0, 20, 40], [0, 1])
+    b.scaling = [0.5, 0.75]
+    assert segments(call_of(a)) == segments(call_of(b))
+    assert [call_of(b).route.scaling[i] for i in range(2)] == [0.5, 0.75]
+    b.plan.seg_start[1] = 7
+    assert segments(call_of(b)) == ([0, 7, 40], [0, 1])
