@@ -539,16 +539,20 @@ class _CallArgs:
 def _call_key(rows, d_in, d_out, dtype, st: "LayerState") -> tuple:
     """All that the routing tables of a call are made from."""
     plan, table = st.plan, st.table
-    return (rows, d_in, d_out, dtype, st.impl, table.r_pack,
-            *[a.tobytes() if type(a) is np.ndarray else np.asarray(a).tobytes()
-              for a in (table.rank, table.pack_off, st.scaling, plan.seg_start, plan.seg_adapter)])
+    head = (rows, d_in, d_out, dtype, st.impl, table.r_pack)
+    try:
+        return (head, table.rank.tobytes(), table.pack_off.tobytes(), st.scaling.tobytes(), plan.seg_start.tobytes(),
+                plan.seg_adapter.tobytes())
+    except AttributeError:  # lists
+        return (head, *[np.asarray(a).tobytes() for a in (table.rank, table.pack_off, st.scaling, plan.seg_start,
+                                                          plan.seg_adapter)])
 
 
 class _Call:
     """One call made with a routing plan: a fresh mlora_problem over a
     mlora_routing and buffer sizes kept for the plan's present content."""
 
-    __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "key", "_scratch")
+    __slots__ = ("args", "prob", "route", "zbytes", "wbytes", "active", "key", "_scratch")
 
     def __init__(self, rows, d_in, d_out, dtype, st: "LayerState"):
         plan, table = st.plan, st.table
@@ -562,11 +566,13 @@ class _Call:
                              RoutePlan(plan.rows, np.array(plan.seg_start), np.array(plan.seg_adapter)),
                              AdapterTable(table.ids, np.array(table.rank), np.array(table.pack_off), table.r_pack),
                              np.array(st.scaling), out_rows=perm)
-            kept = (args, args.sizes(), {})
+            owners = set(args.seg_adapter[np.diff(args.seg_start) > 0].tolist())
+            kept = (args, args.sizes(), [i in owners for i in range(table.n)], {})
             if len(plan.calls) >= 8:  # plans or scalings that change from call to call
                 plan.calls.clear()
             plan.calls[key] = kept
-        self.args, (self.zbytes, self.wbytes), self._scratch = kept
+        # active: the adapters that own rows, whose gradients are written
+        self.args, (self.zbytes, self.wbytes), self.active, self._scratch = kept
         word = st.err_word
         if word is not None and (word.dtype != torch.int32 or word.device.type != "cuda"):
             raise ValueError("err_word must be a CUDA int32 tensor")
@@ -640,19 +646,19 @@ def _workspace(st: LayerState, args, wb, device):
 def check_base(x, A, B, W, bias, base8: Optional["Int8Rows"]) -> None:
     """The backbone's operands against the layer's packs: the kernels take all
     sizes from the packs."""
-    shape = (B.shape[0], A.shape[1])
-    if W is not None and W.shape != shape:
-        raise ValueError(f"backbone {tuple(W.shape)} in a layer of {shape}")
+    d_out, d_in = B.shape[0], A.shape[1]
+    if W is not None and W.shape != (d_out, d_in):
+        raise ValueError(f"backbone {tuple(W.shape)} in a layer of {(d_out, d_in)}")
     if bias is not None:
-        if bias.shape != shape[:1]:
-            raise ValueError(f"bias of shape {tuple(bias.shape)} in a layer of {shape[0]} outputs")
+        if bias.shape != (d_out,):
+            raise ValueError(f"bias of shape {tuple(bias.shape)} in a layer of {d_out} outputs")
         if bias.dtype != x.dtype or bias.device != x.device:
             raise RuntimeError(f"input {x.dtype} on {x.device} but bias {bias.dtype} on {bias.device}")
     if base8 is not None:
-        if base8.device != x.device:
+        if base8.q.device != x.device:
             raise RuntimeError(f"input on {x.device} but the 8-bit backbone on {base8.device}")
-        if base8.shape != shape:
-            raise ValueError(f"8-bit backbone {base8.shape} in a layer of {shape}")
+        if base8.cols != d_in or base8.q.shape[0] != d_out:
+            raise ValueError(f"8-bit backbone {base8.shape} in a layer of {(d_out, d_in)}")
 
 
 def forward_raw(x, W, bias, st: LayerState, x_sorted=None, rows8: Optional["Int8Rows"] = None):
@@ -773,31 +779,37 @@ def backward_raw(dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, wan
     if (xs is not None and (xs.shape != (rows, d_in) or xs.dtype != dt or xs.device != dev)) or (
             rows8 is not None and (rows8.shape != (rows, d_in) or rows8.device != dev)):
         raise ValueError(f"the saved input is not that of a call of {rows} rows and {d_in} features")
-    args = _Call(rows, d_in, d_out, mlora_dtype(dt), st)
-    if z.numel() * z.element_size() < args.zbytes:
-        raise ValueError(f"the saved intermediate has {z.numel() * z.element_size()} bytes, the call {args.zbytes}")
-    dy = dy.contiguous()
-    xs = xs.contiguous() if xs is not None else None
-    dys = gather_rows(dy, st.plan.perm) if st.plan.perm is not None else dy
-    wb = args.wbytes
-    ws, args.prob.flags = _workspace(st, args, wb, dev)
-    dx = torch.empty(rows, d_in, dtype=dy.dtype, device=dev) if want_dx else None
+    call = _Call(rows, d_in, d_out, mlora_dtype(dt), st)
+    if z.numel() * z.element_size() < call.zbytes:
+        raise ValueError(f"the saved intermediate has {z.numel() * z.element_size()} bytes, the call {call.zbytes}")
+    return _backward(call, dy.contiguous(), xs.contiguous() if xs is not None else None, W, z, st, want_dx, want_dA,
+                     want_dB, rows8)
+
+
+def _backward(call: _Call, dy, xs, W, z, st: LayerState, want_dx: bool, want_dA: bool, want_dB: bool, rows8):
+    """backward_raw of tensors that belong to the forward ``call``."""
+    p = call.prob
+    rows, dev, wb = p.rows, dy.device, call.wbytes
+    perm = call.args.out_rows
+    dys = gather_rows(dy, perm) if perm is not None else dy
+    ws, p.flags = _workspace(st, call, wb, dev)
+    dx = torch.empty(rows, p.d_in, dtype=dy.dtype, device=dev) if want_dx else None
     # every rank row / column of an adapter that owns rows is written; the
     # rest is never exposed (inactive adapters get None gradients)
     dA = torch.empty_like(st.A_pack) if want_dA else None
     dB = torch.empty_like(st.B_pack) if want_dB else None
     if st.base8 is not None or rows8 is not None:
-        grad8 = _Scratch8(rows, d_out, dev) if st.base8 is not None and want_dx else None
+        grad8 = _Scratch8(rows, p.d_out, dev) if st.base8 is not None and want_dx else None
         q8 = _q8_struct(st.base8, rows8, grad8)
         if rows8 is not None and want_dA:
-            q8.scratch_bytes = args.scratch8()
+            q8.scratch_bytes = call.scratch8()
             scratch = torch.empty(max(q8.scratch_bytes, 1), dtype=torch.uint8, device=dev)
             q8.scratch = scratch.data_ptr()
-        _lib.call("mlora_backward_q8", ctypes.byref(args.prob), ctypes.byref(args.route), ctypes.byref(q8),
+        _lib.call("mlora_backward_q8", ctypes.byref(p), ctypes.byref(call.route), ctypes.byref(q8),
                   _ptr(dys), _ptr(xs), _ptr(W), _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA),
                   _ptr(dB), _ptr(ws), wb, _stream(dev))
         return dx, dA, dB
-    _lib.call("mlora_backward", ctypes.byref(args.prob), ctypes.byref(args.route), _ptr(dys), _ptr(xs), _ptr(W),
+    _lib.call("mlora_backward", ctypes.byref(p), ctypes.byref(call.route), _ptr(dys), _ptr(xs), _ptr(W),
               _ptr(st.A_pack), _ptr(st.B_pack), _ptr(z), _ptr(dx), _ptr(dA), _ptr(dB), _ptr(ws), wb,
               _stream(dev))
     return dx, dA, dB
@@ -905,13 +917,13 @@ class MultiLoRAFunction(torch.autograd.Function):
     def forward(ctx, x, W, bias, st: LayerState, *adapter_params):
         ctx.st = st
         if st.base8 is None and not st.save8:
-            y, z, xs, _ = forward_raw(x, W, bias, st)
+            y, z, xs, ctx.call = forward_raw(x, W, bias, st)
             ctx.save_for_backward(xs, z, W, st.A_pack, st.B_pack)
             return y
         # dA alone reads the input in the backward: kept as it is, or in 8 bits
         keep = any(ctx.needs_input_grad[4::2])
         rows8 = _new_rows8(x.shape[0], x.shape[1], x.device) if keep and st.save8 else None
-        y, z, xs, _ = forward_raw(x, W, bias, st, rows8=rows8)
+        y, z, xs, ctx.call = forward_raw(x, W, bias, st, rows8=rows8)
         b8, r8 = st.base8, rows8
         ctx.save_for_backward(xs if keep and not st.save8 else None, z, W, st.A_pack, st.B_pack,
                               *((b8.q, b8.scale) if b8 is not None else (None, None)),
@@ -926,13 +938,15 @@ class MultiLoRAFunction(torch.autograd.Function):
         rows8 = _wrap8(kept[2], kept[3], ctx.d_in) if kept and kept[2] is not None else None
         need = ctx.needs_input_grad
         with _on(dy.device):
-            dx, dA, dB = backward_raw(dy, xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]), rows8)
+            # (autograd has checked dy against y; the plan is the forward's, whatever became of it since)
+            dx, dA, dB = _backward(ctx.call, dy.contiguous(), xs, W, z, st, need[0], any(need[4::2]), any(need[5::2]),
+                                   rows8)
         # one call cuts a pack into all adapters' gradients
         cut, place = st.table.pieces()
         pa = torch.unsafe_split_with_sizes(dA, cut, 0) if dA is not None else None
         pb = torch.unsafe_split_with_sizes(dB, cut, 1) if dB is not None else None
         grads = [None] * (2 * st.table.n)
-        for i, act in enumerate(st.plan.active.tolist()):
+        for i, act in enumerate(ctx.call.active):
             if not act:
                 continue
             if need[4 + 2 * i]:

@@ -193,6 +193,30 @@ def test_a_plan_that_changes_between_calls():
             assert all(torch.equal(u, v) for u, v in zip(a, b)) if isinstance(a, list) else torch.equal(a, b)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_plan_that_changes_before_the_backward(eight):
+    """The gradients are those of the forward that was made."""
+    m = layer(256, 192, RANKS, BF)
+    if eight:
+        m.quantize_base()
+        m.save_input = "int8"
+    x, dy = randn((len(IDS), 256), BF, 1), randn((len(IDS), 192), BF, 2, 0.1)
+    mixed = IDS[torch.randperm(len(IDS), generator=torch.Generator().manual_seed(3))]
+    for ids in (IDS, mixed):
+        want = step(m, x, ids, dy)
+        plan, other = m.route(ids), m.route(torch.full_like(ids, 2))
+        for ad in m.adapters.values():
+            ad.A.grad = ad.B.grad = None
+        xg = x.clone().requires_grad_(True)
+        y = m(xg, ids, plan=plan)
+        plan.seg_start, plan.seg_adapter, plan.perm, plan.active = (other.seg_start, other.seg_adapter, other.perm,
+                                                                    other.active)
+        y.backward(dy)
+        assert torch.equal(xg.grad, want[1])
+        for ad, a, b in zip(m.adapters.values(), want[2], want[3]):
+            assert torch.equal(ad.A.grad, a) and torch.equal(ad.B.grad, b)
+
+
 # ------------------------------------------------------------------ buffers of a native caller
 
 def odd(t):

@@ -340,3 +340,12 @@ def test_plans_and_scalings_given_as_lists():
     assert [call_of(b).route.scaling[i] for i in range(2)] == [0.5, 0.75]
     b.plan.seg_start[1] = 7
     assert segments(call_of(b)) == ([0, 7, 40], [0, 1])
+
+
+def test_active_adapters_of_a_call():
+    st = state()
+    assert call_of(st).active == [True, True]
+    st.plan.seg_start, st.plan.seg_adapter = np.array([0, 40, 40], np.int32), np.array([1, 0], np.int32)
+    assert call_of(st).active == [False, True]
+    st.plan.seg_start, st.plan.seg_adapter = np.array([0, 40], np.int32), np.array([-1], np.int32)
+    assert call_of(st).active == [False, False]
