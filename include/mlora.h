@@ -466,7 +466,7 @@ int mlora_forward_q8(const mlora_problem* prob, const mlora_routing* route, cons
  *     dA_a = sum_seg (s_a dY_seg B_a)^T (x_scale Xq)_seg.
  * X is read for dA only.  What is not finite in a row of X or dY reaches the
  * gradients of that row's adapter and no other's (mlora_backward sums rows in
- * groups of 64, which it may share between adapters). */
+ * groups of 64, or of a tile on the CUDA cores, that adapters may share). */
 int mlora_backward_q8(const mlora_problem* prob, const mlora_routing* route, const mlora_q8* q8,
                       const void* dY, const void* X, const void* W, const void* A_pack, const void* B_pack,
                       const void* zsave, void* dX, void* dA_pack, void* dB_pack, void* workspace,

@@ -21,8 +21,8 @@
 // k-blocks of the next tile, by which time the rewrite has finished.
 //
 // Bound by power on large shapes: the tensor pipe is active 70 to 82 % at 1.6 to
-// 1.65 GHz under the cap (65,536 x 4096 -> 11008: 1.97 ms, 3.0 P op/s; the
-// library's integer product 1.88 ms).  At the full rate a 256 x 256 tile also
+// 1.65 GHz under the cap (65,536 x 4096 -> 11008: 1.96 ms, 3.0 P op/s; the
+// library's integer product 1.81 ms; 8192 rows 297 and 240 us).  At the full rate a 256 x 256 tile also
 // takes 64 bytes a cycle into each SM, of which 57 are reached; tiles of 256 x
 // 512, which need 48, were built and timed in turn with these: 1 to 3 % faster
 // from K = 8192 on, none at K = 4096, slower with few tiles, and not kept.

@@ -523,7 +523,8 @@ __device__ __forceinline__ Item decode(const TcParams& p, int item, int units) {
 // out-of-range values (a corrupted plan) are flagged and clamped
 __device__ __forceinline__ int4 reduce_entry(const TcParams& p, int e) {
   int4 d = p.plan.list_desc[e];
-  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > kTileRows || d.z > d.w) {
+  if (d.x < 0 || d.x >= p.plan.n_chunks || d.y < 0 || d.y >= p.plan.n_tiles || d.z < 0 || d.w > kTileRows ||
+      d.z > d.w) {
     flag_error(p.plan.err, kErrBounds);
     d = make_int4(0, 0, 0, 0);
   }
@@ -767,7 +768,8 @@ __global__ void __launch_bounds__(kThreads1<ISO>, 1) k_tc(const __grid_constant_
     mbar_init(drain, 1);
     for (int q = 0; q < kSched; ++q) {
       mbar_init(&sched_full[q], 1);
-      mbar_init(&sched_empty[q], 1 + 4 + kProducers - 1 + (ISO ? 1 : 0));  // the MMA thread, the epilogue warps, the other producers
+      // the MMA thread, the epilogue warps, the other producers (and the clearing warp)
+      mbar_init(&sched_empty[q], 1 + 4 + kProducers - 1 + (ISO ? 1 : 0));
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
