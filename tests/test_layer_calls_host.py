@@ -170,6 +170,15 @@ def test_layers_of_one_shape_share_a_resident_plan(uploads):
     assert len(uploads) == 4 and resident(one) is make(one)
 
 
+def test_staged_calls_find_the_resident_plan(uploads):
+    st = state()
+    ws = make(st)
+    fw = ops.StagedForward(torch.zeros(40, 64, dtype=BF), None, None, st)
+    bw = ops.StagedBackward(torch.zeros(40, 48, dtype=BF), None, None, fw.z, st)
+    assert fw.ws is ws and bw.ws is ws
+    assert fw.args.prob.flags & _lib.PLAN_RESIDENT and bw.args.prob.flags & _lib.PLAN_RESIDENT
+
+
 def test_a_changed_plan_is_not_resident(uploads):
     st = state()
     make(st)
